@@ -551,6 +551,45 @@ typedef struct onebit_fused_in {
 int onebit_fused_gemv(const onebit_proj_t *projs, void *const *outs, int nproj, int prologue,
                       const onebit_fused_in_t *in, void *stream);
 
+/* ---- beam search: attention of hypotheses that share their prompt, the choice of the next ones, their states in place -----------------
+ * onebit_attention_shared_rows: attention of single-token rows (q_len = 1) of several sequences that share a PREFIX of their keys and
+ * values.  The rows come in groups that tile 0 .. rows - 1 in order (HOST array; it travels in the kernel arguments).  A row of group g
+ * attends to all g.len positions of slot g.slot of the PREFIX cache, read once for the group, and to positions g.first .. row_pos[row] of
+ * slot row_slot[row] (NULL: slot = row) of the OWN cache; o = softmax(q k^T / sqrt(D)) v over both together.  The two caches may be one
+ * allocation (hypotheses of one slot pool: g.first = g.len) or two (a long text stored once, short slots: g.first = 0).  g.len = 0: no prefix
+ * (its pointers may then be NULL).  A row whose slot or position lies outside the own cache is idle: its output stays as it is.  A row with
+ * row_pos < g.first has no position of its own; one without any key gets zeros.
+ *   fp16; q [rows, n_heads, D] post-RoPE, o [rows, n_heads * D] (x h_next [n_heads * D] if given), prefix cache
+ *   [n_prefix_slots][n_kv_heads][prefix_max_len][D], own cache [n_slots][n_kv_heads][max_len][D]; D a multiple of 8, at most 128.
+ *   max_own: bound on row_pos - g.first + 1 over the rows; positions beyond it are NOT attended.  Scores, statistics and sums fp32, the
+ *   weights rounded to fp16 before the value product.  Deterministic.
+ *   scratch: onebit_attention_shared_scratch_bytes() of the same groups and sizes, 16-byte aligned, its contents of no account; not shared by
+ *   calls that may run at the same time (0 bytes: the arguments are refused). */
+typedef struct onebit_prefix { int32_t row0, n, slot, len, first; } onebit_prefix_t;
+size_t onebit_attention_shared_scratch_bytes(const onebit_prefix_t *groups, int32_t n_groups, int64_t rows, int32_t n_heads, int32_t n_kv_heads,
+                                             int32_t head_dim, int64_t max_own);
+int onebit_attention_shared_rows(const void *q, const void *prefix_k, const void *prefix_v, const void *k_cache, const void *v_cache, void *o,
+                                 const void *h_next_or_null, const onebit_prefix_t *groups, int32_t n_groups, const int32_t *row_slot,
+                                 const int32_t *row_pos, int64_t rows, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                                 int64_t n_prefix_slots, int64_t prefix_max_len, int64_t n_slots, int64_t max_len, int64_t max_own,
+                                 void *scratch, size_t scratch_bytes, void *stream);
+/* onebit_beam_select: logits [groups * beams, vocab] (dtype, row pitch ld elements), scores fp32 [groups * beams] the hypotheses' sums of log
+ * probabilities.  Continuing hypothesis b of a group by token t is worth v = score_b + (x_t - ln sum_u e^{x_u}), in 64 bits; the group's `keep`
+ * best in the order (v descending, beam, logit descending, token) are written to out_scores (v rounded to fp32) / out_beams / out_tokens
+ * [groups, keep].  A continuation of v = -inf or NaN (a banned token, a dead hypothesis, a row with a NaN or +inf) is none; places that remain
+ * hold -inf, -1, -1.  beams 1 .. 32, keep 1 .. 64, vocab <= 2^20, groups * beams <= 65535.  scratch: onebit_beam_select_scratch_bytes(groups * beams, vocab, keep)
+ * bytes, 16-byte aligned, its contents of no account. */
+size_t onebit_beam_select_scratch_bytes(int64_t rows, int64_t vocab, int32_t keep);
+int onebit_beam_select(const void *logits, int64_t ld, int dtype, const float *scores, int64_t groups, int32_t beams, int64_t vocab, int32_t keep,
+                       float *out_scores, int32_t *out_beams, int32_t *out_tokens, void *scratch, size_t scratch_bytes, void *stream);
+/* onebit_reorder_slots: in every buffer (HOST array of device pointers, each to slot 0 of group 0) slot g * beams + b takes what slot
+ * g * beams + parents[g][b] held, for any map (parents: device int32 [groups, beams]; one outside 0 .. beams - 1 leaves the slot as it is).
+ * A slot is slot_bytes apart from the next and has `outer` rows, outer_bytes apart, of which bytes first_byte .. + n_bytes move: with caches
+ * [slots][n_kv_heads][max_len][head_dim] the positions that differ between hypotheses.  Whole 16 bytes everywhere (sizes and addresses) run
+ * fastest, whole 4 next.  Buffers do not overlap.  beams <= 32. */
+int onebit_reorder_slots(void *const *buffers, int32_t n_buffers, const int32_t *parents, int64_t groups, int32_t beams, int64_t slot_bytes,
+                         int64_t outer, int64_t outer_bytes, int64_t first_byte, int64_t n_bytes, void *stream);
+
 /* ---- train-mode layer: the reference's BitLinear + SignSTE on LATENT weights (bitnet.py:14-28, 58-68),
  * SURVEY.md section 8 rows a8 / f4 (forward and backward for knowledge-distillation training on MI355X).
  * All tensors of one call share `dtype` (ONEBIT_F16 / ONEBIT_F32); row-major, contiguous.

@@ -65,6 +65,11 @@ SYMBOLS = {
     "onebit_decode_step_ksharded": (_int, [_vp, _vp, ctypes.c_int32, ctypes.c_int32, _vp]),   # (model*, onebit_kshard_state_t*, layer, segment, stream)
     "onebit_debug_fill_lds": (_int, [ctypes.c_uint32, _vp]),
     "onebit_fused_gemv": (_int, [_vp, _vp, _int, _int, _vp, _vp]),
+    "onebit_attention_shared_scratch_bytes": (ctypes.c_size_t, [_vp, ctypes.c_int32, _i64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _i64]),
+    "onebit_attention_shared_rows": (_int, [_vp] * 8 + [ctypes.c_int32, _vp, _vp, _i64] + [ctypes.c_int32] * 3 + [_i64] * 5 + [_vp, ctypes.c_size_t, _vp]),
+    "onebit_beam_select_scratch_bytes": (ctypes.c_size_t, [_i64, _i64, ctypes.c_int32]),
+    "onebit_beam_select": (_int, [_vp, _i64, _int, _vp, _i64, ctypes.c_int32, _i64, ctypes.c_int32, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "onebit_reorder_slots": (_int, [_vp, ctypes.c_int32, _vp, _i64, ctypes.c_int32] + [_i64] * 5 + [_vp]),
     "onebit_train_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _int]),
     "onebit_train_least_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _int]),
     "onebit_train_forward_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _int]),

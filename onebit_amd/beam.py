@@ -1,0 +1,188 @@
+"""Beam search's operators on the native library (include/onebit.h): attention of hypotheses that share their prompt, the choice of the next
+hypotheses from their logits, and their states brought to the slots that go on with them.
+
+All three enqueue on the current stream of their tensors' device and never synchronise; they can be captured into a HIP graph (host
+arguments -- the groups, lengths, positions -- are fixed by the capture, device tensors are read by every replay).  A workspace may be kept
+between calls of the same sizes; calls that may run at the same time need one each.  There is no CPU fallback."""
+from __future__ import annotations
+
+import ctypes
+from typing import List, Optional, Sequence, Tuple
+
+import torch
+
+from . import _lib
+from .bitnet import _dtype_code, _require_gpu, _stream_ptr
+
+MAX_BEAMS, MAX_KEEP = 32, 64
+
+
+class _Prefix(ctypes.Structure):          # onebit_prefix_t
+    _fields_ = [("row0", ctypes.c_int32), ("n", ctypes.c_int32), ("slot", ctypes.c_int32), ("len", ctypes.c_int32), ("first", ctypes.c_int32)]
+
+
+def _prefixes(groups):
+    arr = (_Prefix * max(len(groups), 1))()
+    for a, g in zip(arr, groups):
+        if len(g) != 5:
+            raise ValueError(f"a group is (first row, rows, prefix slot, prefix length, first own position), not {tuple(g)!r}")
+        a.row0, a.n, a.slot, a.len, a.first = g
+    return arr
+
+
+def _same_device(device, what: str, *tensors):
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: tensors on {device} and {t.device}")
+
+
+def _rows_int32(t: Optional[torch.Tensor], rows: int, what: str):
+    if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != rows or not t.is_contiguous()):
+        raise ValueError(f"{what} must be a contiguous int32 tensor of {rows} entries")
+
+
+def shared_prefix_workspace(groups: Sequence[Tuple[int, int, int, int, int]], rows: int, heads: int, kv_heads: int, head_dim: int, max_own: int,
+                            device="cuda") -> torch.Tensor:
+    """Scratch memory for ``shared_prefix_attention`` calls of these groups and sizes."""
+    lib = _lib.load()
+    n = lib.onebit_attention_shared_scratch_bytes(_prefixes(groups), len(groups), rows, heads, kv_heads, head_dim, max_own)
+    if rows > 0 and n == 0:
+        raise ValueError(f"shared_prefix_workspace: {lib.onebit_last_error().decode('utf-8', 'replace')}")
+    return torch.empty(max(int(n), 1), dtype=torch.uint8, device=device)
+
+
+def shared_prefix_attention(q: torch.Tensor, prefix_k: Optional[torch.Tensor], prefix_v: Optional[torch.Tensor], k_cache: torch.Tensor, v_cache: torch.Tensor,
+                            groups: Sequence[Tuple[int, int, int, int, int]], row_slot: Optional[torch.Tensor], row_pos: torch.Tensor,
+                            max_own: Optional[int] = None, h_next: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                            workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of single-token rows over a prefix that they share and positions of their own (``onebit_attention_shared_rows``).
+
+    ``q`` [rows, heads, D] fp16 (D a multiple of 8, at most 128).  ``groups``: ``(first row, rows, slot, length, first)`` each, tiling the rows
+    in order; a group's rows attend to positions 0 .. length - 1 of ``slot`` in ``prefix_k`` / ``prefix_v`` [prefix slots, kv heads, prefix positions, D],
+    and row r to positions first .. row_pos[r] of slot ``row_slot[r]`` (None: slot r) in ``k_cache`` / ``v_cache`` [slots, kv heads, positions, D].  The two
+    pairs may be the same tensors; without any prefix the first may be None.  ``row_slot`` / ``row_pos``: int32 on the device; a row whose slot
+    or position lies outside is idle and keeps what ``out`` holds (zeros without ``out``).  ``max_own``: bound on the rows' own positions, those
+    beyond it are not attended (None: all that fit the cache).  ``h_next`` [heads * D]: the result times this."""
+    _require_gpu(q, "shared_prefix_attention")
+    if q.dim() != 3 or q.dtype != torch.float16 or not q.is_contiguous():
+        raise ValueError("shared_prefix_attention: q must be a contiguous float16 [rows, heads, D]")
+    rows, heads, dim = q.shape
+    if (prefix_k is None) != (prefix_v is None):
+        raise ValueError("shared_prefix_attention: prefix keys without values, or values without keys")
+    for name, kc, vc in (("prefix", prefix_k, prefix_v), ("own", k_cache, v_cache)):
+        if kc is None:
+            continue
+        if kc.dim() != 4 or kc.shape != vc.shape or kc.shape[3] != dim or kc.shape[1] != k_cache.shape[1]:
+            raise ValueError(f"shared_prefix_attention: {name} caches {tuple(kc.shape)} / {tuple(vc.shape)} for heads of {dim}")
+        if kc.dtype != q.dtype or vc.dtype != q.dtype or not kc.is_contiguous() or not vc.is_contiguous():
+            raise ValueError(f"shared_prefix_attention: the {name} caches must be contiguous float16")
+    _same_device(q.device, "shared_prefix_attention", prefix_k, prefix_v, k_cache, v_cache, row_slot, row_pos, h_next, out, workspace)
+    _rows_int32(row_slot, rows, "row_slot")
+    _rows_int32(row_pos, rows, "row_pos")
+    if row_pos is None:
+        raise ValueError("shared_prefix_attention: row_pos is needed")
+    if h_next is not None and (h_next.dtype != q.dtype or h_next.numel() != heads * dim or not h_next.is_contiguous()):
+        raise ValueError(f"shared_prefix_attention: h_next must be contiguous float16 of {heads * dim} entries")
+    if out is None:
+        out = torch.zeros_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError("shared_prefix_attention: out must be like q")
+    kv_heads = k_cache.shape[1]
+    if max_own is None:
+        max_own = max([0] + [k_cache.shape[2] - int(g[4]) for g in groups if len(g) == 5])
+    if workspace is None:
+        workspace = shared_prefix_workspace(groups, rows, heads, kv_heads, dim, max_own, q.device)
+    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        raise ValueError("shared_prefix_attention: the workspace must be contiguous uint8")
+    p_slots, p_len = (0, 0) if prefix_k is None else (prefix_k.shape[0], prefix_k.shape[2])
+    with torch.cuda.device(q.device):
+        rc = _lib.load().onebit_attention_shared_rows(
+            q.data_ptr(), None if prefix_k is None else prefix_k.data_ptr(), None if prefix_v is None else prefix_v.data_ptr(), k_cache.data_ptr(),
+            v_cache.data_ptr(), out.data_ptr(), None if h_next is None else h_next.data_ptr(), _prefixes(groups), len(groups),
+            None if row_slot is None else row_slot.data_ptr(), row_pos.data_ptr(), rows, heads, kv_heads, dim, p_slots, p_len, k_cache.shape[0],
+            k_cache.shape[2], max_own, workspace.data_ptr(), workspace.numel(), _stream_ptr(q.device))
+    _lib.check(rc, "onebit_attention_shared_rows")
+    return out
+
+
+def beam_select_workspace(rows: int, vocab: int, keep: int, device="cuda") -> torch.Tensor:
+    """Scratch memory for ``beam_select`` calls of these sizes."""
+    return torch.empty(max(int(_lib.load().onebit_beam_select_scratch_bytes(rows, vocab, keep)), 1), dtype=torch.uint8, device=device)
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, keep: int,
+                workspace: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The ``keep`` best continuations of every group of ``beams`` hypotheses (``onebit_beam_select``): ``logits`` [groups * beams, vocab] float16 or
+    float32 (rows may be strided), ``scores`` float32 [groups * beams], the hypotheses' sums of log probabilities.  Returns scores (float32), beams and
+    tokens (int32), [groups, keep] each, best first: views of one int32 tensor [3, groups, keep].  Values are ranked in 64 bits; equal ones by beam, logit,
+    token.  A continuation of probability zero is none: places that remain hold -inf, -1, -1."""
+    _require_gpu(logits, "beam_select")
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("beam_select: logits must be [rows, vocab] with adjacent columns")
+    rows, vocab = logits.shape
+    if not 1 <= beams <= MAX_BEAMS or rows % beams:
+        raise ValueError(f"beam_select: {rows} rows in groups of {beams} hypotheses (1 .. {MAX_BEAMS})")
+    if not 1 <= keep <= MAX_KEEP:
+        raise ValueError(f"beam_select: {keep} kept (1 .. {MAX_KEEP})")
+    if scores.dtype != torch.float32 or scores.numel() != rows or not scores.is_contiguous():
+        raise ValueError(f"beam_select: scores must be contiguous float32 of {rows} entries")
+    _same_device(logits.device, "beam_select", scores, workspace)
+    if workspace is None:
+        workspace = beam_select_workspace(rows, vocab, keep, logits.device)
+    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        raise ValueError("beam_select: the workspace must be contiguous uint8")
+    groups = rows // beams
+    packed = torch.empty(3, groups, keep, dtype=torch.int32, device=logits.device)
+    p = packed.data_ptr()
+    ld = logits.stride(0) if rows > 1 else max(logits.stride(0), vocab)
+    with torch.cuda.device(logits.device):
+        rc = _lib.load().onebit_beam_select(logits.data_ptr(), ld, _dtype_code(logits.dtype), scores.data_ptr(), groups, beams, vocab, keep, p,
+                                            p + 4 * groups * keep, p + 8 * groups * keep, workspace.data_ptr(), workspace.numel(), _stream_ptr(logits.device))
+    _lib.check(rc, "onebit_beam_select")
+    return packed[0].view(torch.float32), packed[1], packed[2]
+
+
+def reorder_slots(buffers: Sequence[torch.Tensor], parents: torch.Tensor, slot0: int = 0, first: int = 0, count: Optional[int] = None) -> None:
+    """In every buffer [slots, ...], slot ``slot0 + g * beams + b`` takes what slot ``slot0 + g * beams + parents[g, b]`` held, in place and for any map
+    (``onebit_reorder_slots``); ``parents`` int32 [groups, beams] on the device, an entry outside 0 .. beams - 1 leaves its slot as it is.  With ``count``,
+    buffers are caches [slots, heads, positions, D] of which positions ``first`` .. ``first + count - 1`` move.  Any dtype; buffers do not overlap."""
+    if parents.dim() != 2 or parents.dtype != torch.int32 or not parents.is_contiguous():
+        raise ValueError("reorder_slots: parents must be a contiguous int32 [groups, beams]")
+    _require_gpu(parents, "reorder_slots")
+    groups, beams = parents.shape
+    if not 1 <= beams <= MAX_BEAMS:
+        raise ValueError(f"reorder_slots: {beams} beams (1 .. {MAX_BEAMS})")
+    if count is None and first:
+        raise ValueError("reorder_slots: first without count")
+    if slot0 < 0 or first < 0 or (count is not None and count < 0):
+        raise ValueError("reorder_slots: negative slot0, first or count")
+    shapes: dict = {}
+    spans: List[Tuple[int, int]] = []
+    for t in buffers:
+        if not t.is_contiguous() or t.dim() < 1 or t.shape[0] < slot0 + groups * beams:
+            raise ValueError(f"reorder_slots: buffer {tuple(t.shape)} must be contiguous with {slot0 + groups * beams} slots")
+        if t.device != parents.device:
+            raise ValueError(f"reorder_slots: tensors on {parents.device} and {t.device}")
+        size = t.element_size()
+        slot = t.stride(0) * size if t.numel() else 0
+        if count is None:
+            geometry = (slot, 1, slot, 0, slot)
+        else:
+            if t.dim() != 4 or first + count > t.shape[2]:
+                raise ValueError(f"reorder_slots: positions {first} .. {first + count - 1} of a cache {tuple(t.shape)}")
+            row = t.shape[3] * size
+            geometry = (slot, t.shape[1], t.shape[2] * row, first * row, count * row)
+        if slot == 0 or groups == 0:
+            continue
+        p = t.data_ptr()
+        spans.append((p, p + t.shape[0] * slot))
+        shapes.setdefault(geometry, []).append(p + slot0 * slot)
+    spans.sort()
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise ValueError("reorder_slots: buffers overlap")
+    lib = _lib.load()
+    with torch.cuda.device(parents.device):
+        stream = _stream_ptr(parents.device)
+        for geometry, ptrs in shapes.items():
+            rc = lib.onebit_reorder_slots((ctypes.c_void_p * len(ptrs))(*ptrs), len(ptrs), parents.data_ptr(), groups, beams, *geometry, stream)
+            _lib.check(rc, "onebit_reorder_slots")

@@ -1,0 +1,238 @@
+// libonebit_hip.so, beam search's operators:
+//   onebit_attention_shared_rows   attention of single-token rows over a shared prefix and their own cache slots (ob_shattn.h)
+//   onebit_beam_select             the best continuations over beams and vocabulary (ob_beamsel.h)
+//   onebit_reorder_slots           surviving hypotheses' states brought to their slots, in place (ob_reorder.h)
+#include <hip/hip_runtime.h>
+#include <algorithm>
+#include <math.h>
+
+#include "../../include/onebit.h"
+#include "ob_host.h"
+#include "ob_shattn.h"
+#include "ob_beamsel.h"
+#include "ob_reorder.h"
+
+static inline int64_t ob_up(int64_t n, int64_t m) { return (n + m - 1) / m; }
+static const int64_t OB_MAX_WGS = 0xffffff;            // workgroups of 256 threads of one launch
+static const int64_t OB_SH_MAX_LEN = 1 << 30;         // (positions and their chunks are counted in 32 bits)
+
+// ------------------------------------------------------------------------------------------- attention over a shared prefix --
+struct ObShPlan { int mt, pchunk, ochunk, psplits, osplits, own_mb; };
+
+static ObShPlan ob_sh_plan(const onebit_prefix_t *groups, int32_t n_groups, int64_t rows, int32_t n_heads, int32_t n_kv_heads, int64_t max_own)
+{
+    ObShPlan p = {};
+    const int64_t rep = n_heads / n_kv_heads;
+    int64_t most = 1, longest = 0, work = 0;
+    for (int i = 0; i < n_groups; ++i) {
+        if (groups[i].len > 0) most = std::max<int64_t>(most, groups[i].n * rep);
+        longest = std::max<int64_t>(longest, groups[i].len);
+    }
+    p.mt = most <= 16 ? 1 : most <= 32 ? 2 : 4;
+    for (int i = 0; i < n_groups; ++i) work += ob_up(groups[i].n * rep, 16 * p.mt) * groups[i].len * n_kv_heads;
+    p.pchunk = (int)(128 * std::max<int64_t>(1, ob_up(work, 768 * 128)));
+    p.psplits = (int)ob_up(longest, p.pchunk);
+    p.own_mb = (int)ob_up(rep, 16);
+    p.ochunk = (int)(128 * std::max<int64_t>(1, ob_up(rows * n_kv_heads * p.own_mb * max_own, 1024 * 128)));
+    p.osplits = (int)ob_up(max_own, p.ochunk);
+    return p;
+}
+
+static int ob_sh_check(const onebit_prefix_t *groups, int32_t n_groups, int64_t rows, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int64_t max_own)
+{
+    if (n_groups < 0 || rows < 0 || n_heads <= 0 || n_kv_heads <= 0 || max_own < 0) return ob_fail(ONEBIT_E_ARG, "attention_shared_rows: bad size");
+    if (head_dim < 8 || head_dim % 8 != 0 || head_dim > 128 || n_heads % n_kv_heads != 0)
+        return ob_fail(ONEBIT_E_SHAPE, "attention_shared_rows: head_dim %d (multiple of 8, <= 128), heads %d / %d", head_dim, n_heads, n_kv_heads);
+    if (rows > 65535 || n_heads > 65535 || max_own > OB_SH_MAX_LEN) return ob_fail(ONEBIT_E_ARG, "attention_shared_rows: dimension too large");
+    if (rows > 0 && !groups) return ob_fail(ONEBIT_E_ARG, "attention_shared_rows: null pointer");
+    int64_t r = 0;
+    for (int i = 0; i < n_groups && rows > 0; ++i) {
+        const onebit_prefix_t &g = groups[i];
+        if (g.row0 != r || g.n < 1 || g.len < 0 || g.first < 0 || g.len > OB_SH_MAX_LEN || g.first > OB_SH_MAX_LEN)
+            return ob_fail(ONEBIT_E_SHAPE, "attention_shared_rows: group %d starts at row %d (expected %lld) with %d rows, a prefix of %d, own positions from %d", i,
+                           g.row0, (long long)r, g.n, g.len, g.first);
+        r += g.n;
+    }
+    if (r != rows) return ob_fail(ONEBIT_E_SHAPE, "attention_shared_rows: the groups have %lld rows of %lld", (long long)r, (long long)rows);
+    return 0;
+}
+
+extern "C" size_t onebit_attention_shared_scratch_bytes(const onebit_prefix_t *groups, int32_t n_groups, int64_t rows, int32_t n_heads, int32_t n_kv_heads,
+                                                        int32_t head_dim, int64_t max_own)
+{
+    if (rows <= 0 || ob_sh_check(groups, n_groups, rows, n_heads, n_kv_heads, head_dim, max_own)) return 0;
+    const ObShPlan p = ob_sh_plan(groups, n_groups, rows, n_heads, n_kv_heads, max_own);
+    return (size_t)rows * n_heads * (p.psplits + p.osplits) * (head_dim + 2) * 4 + 256;
+}
+
+template <int DP, int MT>
+static void ob_sh_launch(const ObShArgs &a, int64_t items, hipStream_t s)
+{
+    const dim3 grid((unsigned)(items * a.Hkv));
+    if (a.D == DP) hipLaunchKernelGGL((ob_sh_part_kernel<DP, MT, true>), grid, dim3(OB_SH_THREADS), 0, s, a);
+    else hipLaunchKernelGGL((ob_sh_part_kernel<DP, MT, false>), grid, dim3(OB_SH_THREADS), 0, s, a);
+}
+
+extern "C" int onebit_attention_shared_rows(const void *q, const void *prefix_k, const void *prefix_v, const void *k_cache, const void *v_cache, void *o,
+                                            const void *h_next, const onebit_prefix_t *groups, int32_t n_groups, const int32_t *row_slot,
+                                            const int32_t *row_pos, int64_t rows, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                                            int64_t n_prefix_slots, int64_t prefix_max_len, int64_t n_slots, int64_t max_len, int64_t max_own, void *scratch,
+                                            size_t scratch_bytes, void *stream)
+{
+    const int rc = ob_sh_check(groups, n_groups, rows, n_heads, n_kv_heads, head_dim, max_own);
+    if (rc) return rc;
+    if (n_prefix_slots < 0 || prefix_max_len < 0 || n_slots <= 0 || max_len <= 0 || n_slots > 0x7fffffffLL || max_len > OB_SH_MAX_LEN)
+        return ob_fail(ONEBIT_E_ARG, "attention_shared_rows: bad cache size");
+    bool prefixes = false;
+    for (int i = 0; i < n_groups && rows > 0; ++i) {
+        const onebit_prefix_t &g = groups[i];
+        prefixes = prefixes || g.len > 0;
+        if (g.len > 0 && (g.slot < 0 || g.slot >= n_prefix_slots || g.len > prefix_max_len))
+            return ob_fail(ONEBIT_E_SHAPE, "attention_shared_rows: group %d's prefix (slot %d, %d positions) outside %lld slots x %lld positions", i, g.slot, g.len,
+                           (long long)n_prefix_slots, (long long)prefix_max_len);
+    }
+    if (rows == 0) return 0;
+    if (!q || !k_cache || !v_cache || !o || !row_pos || (prefixes && (!prefix_k || !prefix_v))) return ob_fail(ONEBIT_E_ARG, "attention_shared_rows: null pointer");
+    if (!ob_aligned(q, 16) || !ob_aligned(k_cache, 16) || !ob_aligned(v_cache, 16) || !ob_aligned(o, 4) || (h_next && !ob_aligned(h_next, 2)) ||
+        (prefixes && (!ob_aligned(prefix_k, 16) || !ob_aligned(prefix_v, 16))))
+        return ob_fail(ONEBIT_E_ALIGN, "attention_shared_rows: q and the caches must be 16-byte aligned");
+    const size_t need = onebit_attention_shared_scratch_bytes(groups, n_groups, rows, n_heads, n_kv_heads, head_dim, max_own);
+    if (!scratch || scratch_bytes < need || !ob_aligned(scratch, 16)) return ob_fail(ONEBIT_E_WSPACE, "attention_shared_rows: needs %zu bytes of 16-byte aligned scratch", need);
+    const ObShPlan p = ob_sh_plan(groups, n_groups, rows, n_heads, n_kv_heads, max_own);
+    const int64_t rep = n_heads / n_kv_heads;
+    ObShArgs a = {};
+    a.q = (const _Float16 *)q; a.pk = (const _Float16 *)prefix_k; a.pv = (const _Float16 *)prefix_v; a.k = (const _Float16 *)k_cache; a.v = (const _Float16 *)v_cache;
+    a.o = (_Float16 *)o; a.h_next = (const _Float16 *)h_next; a.row_slot = row_slot; a.row_pos = row_pos;
+    a.p_max_len = prefix_max_len; a.max_len = max_len; a.H = n_heads; a.Hkv = n_kv_heads; a.rep = (int)rep; a.D = head_dim; a.n_slots = (int)n_slots;
+    a.pchunk = p.pchunk; a.ochunk = p.ochunk; a.psplits = p.psplits; a.osplits = p.osplits; a.own_mb = p.own_mb; a.max_own = (int)max_own;
+    a.scale_log2e = 1.4426950408889634f / sqrtf((float)head_dim);
+    const size_t parts = (size_t)rows * n_heads * (p.psplits + p.osplits);
+    a.part_o = (float *)scratch;
+    a.part_ml = a.part_o + parts * head_dim;
+    for (int g0 = 0; g0 < n_groups; g0 += OB_SH_GROUPS) {
+        a.n_groups = std::min(n_groups - g0, OB_SH_GROUPS);
+        a.row_base = groups[g0].row0; a.rows = 0;
+        int64_t items = 0;
+        for (int i = 0; i < a.n_groups; ++i) {
+            const onebit_prefix_t &g = groups[g0 + i];
+            const int64_t chunks = ob_up(g.len, p.pchunk);
+            items += chunks * ob_up(g.n * rep, 16 * p.mt);
+            a.g[i] = {g.row0, g.n, g.slot, g.len, g.first, (int)chunks, (int)items};
+            a.rows += g.n;
+        }
+        a.own_item0 = (int)items;
+        items += (int64_t)a.rows * p.own_mb * p.osplits;
+        if (items * n_kv_heads > OB_MAX_WGS) return ob_fail(ONEBIT_E_ARG, "attention_shared_rows: too many workgroups");
+        hipStream_t s = (hipStream_t)stream;
+        if (items > 0) {
+            if (head_dim > 64) {
+                if (p.mt == 1) ob_sh_launch<128, 1>(a, items, s);
+                else if (p.mt == 2) ob_sh_launch<128, 2>(a, items, s);
+                else ob_sh_launch<128, 4>(a, items, s);
+            } else {
+                if (p.mt == 1) ob_sh_launch<64, 1>(a, items, s);
+                else if (p.mt == 2) ob_sh_launch<64, 2>(a, items, s);
+                else ob_sh_launch<64, 4>(a, items, s);
+            }
+        }
+        hipLaunchKernelGGL(ob_sh_join_kernel, dim3((unsigned)ob_up((int64_t)a.rows * n_heads, OB_SH_THREADS / 64)), dim3(OB_SH_THREADS), 0, s, a);
+        const int rc2 = ob_launch_status("attention_shared_rows");
+        if (rc2) return rc2;
+    }
+    return 0;
+}
+
+// ---------------------------------------------------------------------------------------------- the choice of hypotheses --
+static int ob_bs_check(int64_t groups, int32_t beams, int64_t vocab, int32_t keep)
+{
+    if (groups < 0 || vocab < 1) return ob_fail(ONEBIT_E_ARG, "beam_select: bad size");
+    if (beams < 1 || beams > OB_RE_MAX_BEAMS || keep < 1 || keep > OB_BS_MAX_KEEP)
+        return ob_fail(ONEBIT_E_SHAPE, "beam_select: %d beams (1 .. %d), %d kept (1 .. %d)", beams, OB_RE_MAX_BEAMS, keep, OB_BS_MAX_KEEP);
+    if (vocab > (1 << 20) || groups > 65535 || groups * beams > 65535) return ob_fail(ONEBIT_E_ARG, "beam_select: dimension too large");
+    return 0;
+}
+
+extern "C" size_t onebit_beam_select_scratch_bytes(int64_t rows, int64_t vocab, int32_t keep)
+{
+    if (rows <= 0 || vocab <= 0 || keep <= 0) return 0;
+    const size_t chunks = (size_t)ob_up(vocab, OB_BS_CHUNK);
+    return (size_t)rows * chunks * (16 + 4 * (size_t)keep * 8) + 256;
+}
+
+extern "C" int onebit_beam_select(const void *logits, int64_t ld, int dtype, const float *scores, int64_t groups, int32_t beams, int64_t vocab, int32_t keep,
+                                  float *out_scores, int32_t *out_beams, int32_t *out_tokens, void *scratch, size_t scratch_bytes, void *stream)
+{
+    const int rc = ob_bs_check(groups, beams, vocab, keep);
+    if (rc) return rc;
+    if (dtype != ONEBIT_F16 && dtype != ONEBIT_F32) return ob_fail(ONEBIT_E_DTYPE, "beam_select: dtype %d", dtype);
+    if (ld < vocab) return ob_fail(ONEBIT_E_SHAPE, "beam_select: row pitch %lld below %lld logits", (long long)ld, (long long)vocab);
+    if (groups == 0) return 0;
+    if (!logits || !scores || !out_scores || !out_beams || !out_tokens) return ob_fail(ONEBIT_E_ARG, "beam_select: null pointer");
+    if (!ob_aligned(logits, dtype == ONEBIT_F16 ? 2 : 4) || !ob_aligned(scores, 4) || !ob_aligned(out_scores, 4) || !ob_aligned(out_beams, 4) || !ob_aligned(out_tokens, 4))
+        return ob_fail(ONEBIT_E_ALIGN, "beam_select: misaligned pointer");
+    const int64_t rows = groups * beams;
+    const size_t need = onebit_beam_select_scratch_bytes(rows, vocab, keep);
+    if (!scratch || scratch_bytes < need || !ob_aligned(scratch, 16)) return ob_fail(ONEBIT_E_WSPACE, "beam_select: needs %zu bytes of 16-byte aligned scratch", need);
+    ObBsArgs a = {};
+    a.logits = logits; a.ld = ld; a.scores = scores; a.beams = beams; a.keep = keep; a.vocab = (int)vocab; a.chunks = (int)ob_up(vocab, OB_BS_CHUNK);
+    a.sums = (double *)scratch;
+    a.list_x = (float *)(a.sums + (size_t)rows * a.chunks * 2);
+    a.list_t = (int *)(a.list_x + (size_t)rows * a.chunks * 4 * keep);
+    a.out_scores = out_scores; a.out_beams = out_beams; a.out_tokens = out_tokens;
+    hipStream_t s = (hipStream_t)stream;
+    const dim3 grid((unsigned)a.chunks, (unsigned)rows);
+    if (dtype == ONEBIT_F16) hipLaunchKernelGGL((ob_bs_scan_kernel<_Float16>), grid, dim3(OB_BS_THREADS), 0, s, a);
+    else hipLaunchKernelGGL((ob_bs_scan_kernel<float>), grid, dim3(OB_BS_THREADS), 0, s, a);
+    hipLaunchKernelGGL(ob_bs_pick_kernel, dim3((unsigned)groups), dim3(OB_BS_THREADS), (size_t)4 * a.chunks * beams, s, a);
+    return ob_launch_status("beam_select");
+}
+
+// ------------------------------------------------------------------------------------------------------ states reordered --
+template <typename U>
+static void ob_re_launch(const ObReArgs &a, const dim3 &grid, hipStream_t s)
+{
+    if (a.beams <= 4) hipLaunchKernelGGL((ob_re_kernel<4, U>), grid, dim3(OB_RE_THREADS), 0, s, a);
+    else if (a.beams <= 8) hipLaunchKernelGGL((ob_re_kernel<8, U>), grid, dim3(OB_RE_THREADS), 0, s, a);
+    else if (a.beams <= 16) hipLaunchKernelGGL((ob_re_kernel<16, U>), grid, dim3(OB_RE_THREADS), 0, s, a);
+    else hipLaunchKernelGGL((ob_re_kernel<32, U>), grid, dim3(OB_RE_THREADS), 0, s, a);
+}
+
+extern "C" int onebit_reorder_slots(void *const *buffers, int32_t n_buffers, const int32_t *parents, int64_t groups, int32_t beams, int64_t slot_bytes,
+                                    int64_t outer, int64_t outer_bytes, int64_t first_byte, int64_t n_bytes, void *stream)
+{
+    if (n_buffers < 0 || groups < 0 || outer < 0 || first_byte < 0 || n_bytes < 0 || outer_bytes < 0 || slot_bytes < 0)
+        return ob_fail(ONEBIT_E_ARG, "reorder_slots: negative size");
+    if (beams < 1 || beams > OB_RE_MAX_BEAMS || groups > 65535) return ob_fail(ONEBIT_E_SHAPE, "reorder_slots: %lld groups of %d beams (1 .. %d)", (long long)groups, beams, OB_RE_MAX_BEAMS);
+    const int64_t most = (int64_t)1 << 46;
+    if (slot_bytes > most || outer > most / std::max<int64_t>(n_bytes, 1) || (outer > 0 && first_byte + n_bytes > outer_bytes) ||
+        (outer > 0 && outer_bytes > slot_bytes / outer))
+        return ob_fail(ONEBIT_E_SHAPE, "reorder_slots: %lld rows of %lld bytes (%lld from %lld on) do not lie in slots of %lld", (long long)outer, (long long)outer_bytes,
+                       (long long)n_bytes, (long long)first_byte, (long long)slot_bytes);
+    if (n_buffers == 0 || groups == 0 || outer == 0 || n_bytes == 0) return 0;
+    if (!buffers || !parents) return ob_fail(ONEBIT_E_ARG, "reorder_slots: null pointer");
+    if (!ob_aligned(parents, 4)) return ob_fail(ONEBIT_E_ALIGN, "reorder_slots: misaligned parents");
+    uint64_t low = (uint64_t)(slot_bytes | outer_bytes | first_byte | n_bytes);
+    for (int i = 0; i < n_buffers; ++i) {
+        if (!buffers[i]) return ob_fail(ONEBIT_E_ARG, "reorder_slots: null buffer %d", i);
+        low |= (uint64_t)(uintptr_t)buffers[i];
+    }
+    const int unit = low % 16 == 0 ? 16 : low % 4 == 0 ? 4 : 1;
+    ObReArgs a = {};
+    a.parents = parents; a.slot_bytes = slot_bytes; a.outer_bytes = outer_bytes; a.first_byte = first_byte; a.beams = beams;
+    if (n_bytes / unit > 0x7fffffffLL) return ob_fail(ONEBIT_E_ARG, "reorder_slots: dimension too large");
+    a.units_per = (int)(n_bytes / unit);
+    a.units = outer * a.units_per;
+    const int64_t wgs = ob_up(a.units, OB_RE_THREADS);
+    if (wgs > OB_MAX_WGS) return ob_fail(ONEBIT_E_ARG, "reorder_slots: dimension too large");
+    for (int b0 = 0; b0 < n_buffers; b0 += OB_RE_BUFFERS) {
+        const int n = std::min(n_buffers - b0, OB_RE_BUFFERS);
+        for (int i = 0; i < n; ++i) a.buf[i] = (char *)buffers[b0 + i];
+        const dim3 grid((unsigned)wgs, (unsigned)groups, (unsigned)n);
+        if (unit == 16) ob_re_launch<ob_u32x4>(a, grid, (hipStream_t)stream);
+        else if (unit == 4) ob_re_launch<uint32_t>(a, grid, (hipStream_t)stream);
+        else ob_re_launch<uint8_t>(a, grid, (hipStream_t)stream);
+        const int rc = ob_launch_status("reorder_slots");
+        if (rc) return rc;
+    }
+    return 0;
+}

@@ -1,0 +1,93 @@
+"""Beam search's operators: what they refuse, before any launch (CPU)."""
+import ctypes
+
+import pytest
+import torch
+
+from onebit_amd import _lib
+from onebit_amd.beam import _Prefix, beam_select, reorder_slots, shared_prefix_attention, shared_prefix_workspace
+
+E_ARG, E_SHAPE, E_ALIGN, E_DTYPE, E_WSPACE = -1, -2, -3, -4, -5
+
+
+@pytest.fixture(scope="module")
+def buf():
+    b = ctypes.create_string_buffer(8192)
+    return (ctypes.addressof(b) + 255) & ~255, b
+
+
+def _attention(a, **kw):
+    lib = _lib.load()
+    g = kw.get("groups", [(0, 2, 0, 10, 0)])
+    arr = (_Prefix * max(len(g), 1))(*[_Prefix(*x) for x in g])
+    return lib.onebit_attention_shared_rows(kw.get("q", a), kw.get("pk", a), a, a, a, kw.get("o", a), None, kw.get("arr", arr), len(g), None, kw.get("pos", a),
+                                            kw.get("rows", 2), kw.get("H", 4), kw.get("hkv", 2), kw.get("D", 64), kw.get("pslots", 1), kw.get("plen", 10),
+                                            kw.get("slots", 2), kw.get("max_len", 16), kw.get("own", 16), kw.get("ws", a), kw.get("nb", 1 << 30), None)
+
+
+def test_attention_refuses(buf):
+    a, _ = buf
+    assert _attention(a, D=12) == E_SHAPE and _attention(a, D=136) == E_SHAPE and _attention(a, hkv=3) == E_SHAPE
+    assert _attention(a, rows=-1) == E_ARG and _attention(a, slots=0) == E_ARG and _attention(a, own=-1) == E_ARG
+    assert _attention(a, rows=0, groups=[]) == 0
+    for bad in ([(0, 1, 0, 10, 0)], [(0, 3, 0, 10, 0)], [(1, 2, 0, 10, 0)], [(0, 1, 0, 10, 0), (0, 1, 0, 10, 0)], [(0, 2, 1, 10, 0)], [(0, 2, -1, 10, 0)],
+                [(0, 2, 0, 11, 0)], [(0, 2, 0, -1, 0)], [(0, 2, 0, 10, -1)], [(0, 0, 0, 1, 0), (0, 2, 0, 1, 0)], []):
+        assert _attention(a, groups=bad) == E_SHAPE, bad
+    assert _attention(a, q=None) == E_ARG and _attention(a, pos=None) == E_ARG and _attention(a, pk=None) == E_ARG
+    assert _attention(a, q=a + 2) == E_ALIGN and _attention(a, pk=a + 8) == E_ALIGN and _attention(a, o=a + 2) == E_ALIGN
+    assert _attention(a, ws=None) == E_WSPACE and _attention(a, nb=100) == E_WSPACE and _attention(a, ws=a + 4) == E_WSPACE
+    assert _attention(a, max_len=1 << 31) == E_ARG and _attention(a, rows=70000, groups=[(0, 70000, 0, 10, 0)]) == E_ARG
+
+
+def test_attention_scratch_grows_with_its_parts():
+    f = lambda groups, rows, own: shared_prefix_workspace(groups, rows, 8, 8, 128, own, device="cpu").numel()
+    assert f([(0, 4, 0, 100, 0)], 4, 20) >= 4 * 8 * 2 * 130 * 4
+    assert f([(0, 4, 0, 100000, 0)], 4, 20) > f([(0, 4, 0, 100, 0)], 4, 20)
+    with pytest.raises(ValueError, match="rows"):
+        f([(0, 4, 0, 100, 0)], 5, 20)
+    with pytest.raises(ValueError, match="a group is"):
+        f([(0, 4, 0, 100)], 4, 20)
+
+
+def _select(a, **kw):
+    return _lib.load().onebit_beam_select(kw.get("x", a), kw.get("ld", 100), kw.get("dt", 0), a, kw.get("groups", 2), kw.get("beams", 4), kw.get("vocab", 100),
+                                          kw.get("keep", 8), kw.get("out", a), a, a, kw.get("ws", a), kw.get("nb", 1 << 30), None)
+
+
+def test_select_refuses(buf):
+    a, _ = buf
+    assert _select(a, groups=-1) == E_ARG and _select(a, vocab=0) == E_ARG and _select(a, groups=0) == 0
+    assert _select(a, beams=0) == E_SHAPE and _select(a, beams=33) == E_SHAPE and _select(a, keep=0) == E_SHAPE and _select(a, keep=65) == E_SHAPE
+    assert _select(a, vocab=1 << 21, ld=1 << 21) == E_ARG and _select(a, groups=20000) == E_ARG and _select(a, groups=1 << 62) == E_ARG
+    assert _select(a, dt=2) == E_DTYPE and _select(a, ld=99) == E_SHAPE and _select(a, x=None) == E_ARG and _select(a, out=None) == E_ARG
+    assert _select(a, x=a + 1) == E_ALIGN and _select(a, out=a + 2) == E_ALIGN
+    assert _select(a, ws=None) == E_WSPACE and _select(a, nb=64) == E_WSPACE
+
+
+def _reorder(a, **kw):
+    ptrs = (ctypes.c_void_p * 2)(a, kw.get("second", a + 4096))
+    return _lib.load().onebit_reorder_slots(ptrs, kw.get("n", 2), kw.get("parents", a), kw.get("groups", 1), kw.get("beams", 4), kw.get("slot", 256), kw.get("outer", 2),
+                                            kw.get("row", 128), kw.get("first", 0), kw.get("nb", 128), None)
+
+
+def test_reorder_refuses(buf):
+    a, _ = buf
+    assert _reorder(a, n=-1) == E_ARG and _reorder(a, first=-1) == E_ARG and _reorder(a, nb=-1) == E_ARG and _reorder(a, parents=None) == E_ARG
+    assert _reorder(a, second=None) == E_ARG and _reorder(a, parents=a + 1) == E_ALIGN
+    assert _reorder(a, beams=0) == E_SHAPE and _reorder(a, beams=33) == E_SHAPE and _reorder(a, groups=65536) == E_SHAPE
+    assert _reorder(a, first=16) == E_SHAPE and _reorder(a, slot=255) == E_SHAPE and _reorder(a, outer=3) == E_SHAPE
+    assert _reorder(a, outer=1 << 60) == E_SHAPE and _reorder(a, slot=1 << 60) == E_SHAPE
+    for nothing in (dict(n=0), dict(groups=0), dict(nb=0), dict(outer=0)):
+        assert _reorder(a, **nothing) == 0, nothing
+
+
+def test_python_checks_name_the_mistake():
+    q, c = torch.zeros(2, 4, 64, dtype=torch.float16), torch.zeros(2, 4, 16, 64, dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        shared_prefix_attention(q, None, None, c, c, [(0, 2, 0, 0, 0)], None, torch.zeros(2, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        beam_select(torch.zeros(4, 10), torch.zeros(4), 4, 8)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        reorder_slots([c], torch.zeros(1, 2, dtype=torch.int32))
+    with pytest.raises(ValueError, match="parents"):
+        reorder_slots([c], torch.zeros(1, 2))
