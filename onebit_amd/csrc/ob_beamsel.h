@@ -2,27 +2,35 @@
 // hypothesis; its continuation by token t is worth  v = score_r + (x_t - ln sum_u e^{x_u}),  and a group's `keep` best of beams x vocab
 // continuations are wanted in the order (v descending, beam, x descending, token).  v is a sum in 64 bits: two beams' values often lie closer
 // than fp32 resolves, while within a row the logits themselves order.
-//   ob_bs_scan_kernel   (row, chunk of the vocabulary): max and sum e^{x - max} of the chunk, and each wave's `keep` best of it, in order
-//   ob_bs_pick_kernel   (group): the rows' sums joined, then the best heads of the waves' lists, one after the other
+//   ob_bs_scan_kernel   (row, chunk of the vocabulary): max and sum e^{x - max} of the chunk, and a list of candidates that holds its `keep` best
+//   ob_bs_pick_kernel   (group): the rows' sums joined, then the `keep` best of the lists
+// Both find the best by a threshold instead of one after the other: every wave takes the largest values of its lanes, as many as its share of
+// `keep`, the least of them over the waves is one that at least `keep` candidates reach, and few more do; those few are listed (the scan) or ranked by
+// counting (the pick).  Where too many reach it (rows of equal logits), the best are taken one after the other.
 // The logits are read once.  e^x: the product x log2 e is carried in two parts, so a term is off by 2^-23 at most however far x lies below the
-// maximum; terms are added in fp32 over a thread's elements and in 64 bits from there on.  A row's elements belong to threads by their index
-// alone, not by the row's alignment: equal rows have equal sums, bit for bit.
+// maximum; terms are added in 64 bits.  A row's elements belong to threads by their index alone, not by the row's alignment: equal rows have equal
+// sums, bit for bit.
 #pragma once
 #include "ob_common.h"
 
 #define OB_BS_THREADS 256
-#define OB_BS_EPT 8                                // elements of a thread
-#define OB_BS_CHUNK (OB_BS_THREADS * OB_BS_EPT)    // elements of a workgroup
+#define OB_BS_PICK 1024                            // threads of the pick
 #define OB_BS_MAX_KEEP 64
+#define OB_BS_MAX_BEAMS 32
+#define OB_BS_RANKED 1024                          // candidates that the pick ranks by counting
+
+// room for the candidates of a chunk
+static inline __host__ __device__ int ob_bs_list(int keep) { return 2 * keep + 32; }
 
 struct ObBsArgs {
     const void *logits;
     long long ld;                    // row pitch, elements
     const float *scores;             // [groups * beams]
-    int beams, keep, vocab, chunks;
+    int beams, keep, vocab, chunks, vecs;                // vecs: pieces of 8 elements of a chunk
     double *sums;                    // [rows][chunks][2]  {max, sum}
-    float *list_x;                   // [rows][4 chunks][keep]
-    int *list_t;                     // token, or -1 behind the list's end
+    int *counts;                     // [rows][chunks]
+    float *list_x;                   // [rows][chunks][ob_bs_list(keep)]
+    int *list_t;
     float *out_scores; int *out_beams, *out_tokens;      // [groups][keep]
 };
 
@@ -41,93 +49,139 @@ __device__ __forceinline__ double ob_bs_wave_sum(double v)
     return v;
 }
 
-template <typename T>
+// the k-th largest of the lanes' values (equal ones count one by one), -inf if there are fewer
+__device__ __forceinline__ float ob_bs_kth(float v, int k)
+{
+    const int lane = threadIdx.x & 63;
+    float w = INFINITY;
+    for (int i = 0; i < k; ++i) {
+        w = ob_wave_max(v);
+        if (w == -INFINITY) break;
+        if (lane == __builtin_ctzll(__ballot(v == w))) v = -INFINITY;
+    }
+    return w;
+}
+
+// NV: pieces of 8 elements of a thread, OB_BS_THREADS apart
+template <typename T, int NV>
 __global__ __launch_bounds__(OB_BS_THREADS) void ob_bs_scan_kernel(const ObBsArgs A)
 {
-    __shared__ float red_m[4];
+    __shared__ float red_m[4], red_t[4];
     __shared__ double red_s[4];
+    __shared__ int n_s, red_i[4];
     const int chunk = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const T *x_row = (const T *)A.logits + (int64_t)row * A.ld;
-    const int t0 = chunk * OB_BS_CHUNK + tid * OB_BS_EPT;
-    float x[OB_BS_EPT];
-    if (t0 + OB_BS_EPT <= A.vocab) {
-        typedef T vec __attribute__((ext_vector_type(OB_BS_EPT)));
-        struct __attribute__((packed, aligned(sizeof(T)))) U { vec v; };
-        const vec v = reinterpret_cast<const U *>(x_row + t0)->v;
+    const int c0 = chunk * A.vecs * 8, c1 = min(A.vocab, c0 + A.vecs * 8);
+    float x[NV][8];
+    if (tid == 0) n_s = 0;
 #pragma unroll
-        for (int e = 0; e < OB_BS_EPT; ++e) x[e] = (float)v[e];
-    } else {
+    for (int j = 0; j < NV; ++j) {
+        const int t0 = c0 + 8 * (tid + OB_BS_THREADS * j);
+        if (t0 + 8 <= c1) {
+            typedef T vec __attribute__((ext_vector_type(8)));
+            struct __attribute__((packed, aligned(sizeof(T)))) U { vec v; };
+            const vec v = reinterpret_cast<const U *>(x_row + t0)->v;
 #pragma unroll
-        for (int e = 0; e < OB_BS_EPT; ++e) x[e] = t0 + e < A.vocab ? (float)x_row[t0 + e] : -INFINITY;
+            for (int e = 0; e < 8; ++e) x[j][e] = (float)v[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[j][e] = t0 + e < c1 ? (float)x_row[t0 + e] : -INFINITY;
+        }
     }
-    float m = x[0];
+    float best = -INFINITY;
 #pragma unroll
-    for (int e = 1; e < OB_BS_EPT; ++e) m = fmaxf(m, x[e]);
-    m = ob_wave_max(m);
-    if (lane == 0) red_m[wave] = m;
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) best = fmaxf(best, x[j][e]);
+    // this wave's share of `keep`, by its lanes that have elements: enough over all waves together
+    const int n_thr = min((c1 - c0 + 7) / 8, OB_BS_THREADS), n_wave = max(0, min(64, n_thr - 64 * wave));
+    const float wm = ob_wave_max(best);
+    const float wt = n_thr < A.keep ? -INFINITY : n_wave ? ob_bs_kth(best, (A.keep * n_wave + n_thr - 1) / n_thr) : INFINITY;
+    if (lane == 0) { red_m[wave] = wm; red_t[wave] = wt; }
     __syncthreads();
-    m = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3]));
-    float s = 0.f;
-    if (m != -INFINITY) {
+    const float m = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3])), t = fminf(fminf(red_t[0], red_t[1]), fminf(red_t[2], red_t[3]));
+    const int room = ob_bs_list(A.keep);
+    const int64_t list = (int64_t)row * A.chunks + chunk;
+    float *lx = A.list_x + list * room;
+    int *lt = A.list_t + list * room;
+    if (best >= t && best > -INFINITY) {
 #pragma unroll
-        for (int e = 0; e < OB_BS_EPT; ++e) s += ob_bs_exp(x[e] - m);           // (a NaN logit makes the row's sum NaN, +inf as well)
-    } else {
+        for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int e = 0; e < OB_BS_EPT; ++e) s += x[e] == -INFINITY ? 0.f : x[e];
+            for (int e = 0; e < 8; ++e)
+                if (x[j][e] >= t && x[j][e] > -INFINITY) {
+                    const int at = atomicAdd(&n_s, 1);
+                    if (at < room) { lx[at] = x[j][e]; lt[at] = c0 + 8 * (tid + OB_BS_THREADS * j) + e; }
+                }
     }
-    const double ds = ob_bs_wave_sum((double)s);
-    if (lane == 0) red_s[wave] = ds;
+    double s = 0.;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            s += (double)(m == -INFINITY ? (x[j][e] == -INFINITY ? 0.f : x[j][e]) : ob_bs_exp(x[j][e] - m));        // (a NaN makes the row's sum NaN, +inf as well)
+    s = ob_bs_wave_sum(s);
+    if (lane == 0) red_s[wave] = s;
     __syncthreads();
+    int n = n_s;
+    if (n > room) {                                                             // too many reach the threshold: one after the other
+        float px = INFINITY;
+        int pt = -1;
+        for (n = 0; n < A.keep; ++n) {
+            float bx = -INFINITY;
+            int bt = 0x7fffffff;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int tok = c0 + 8 * (tid + OB_BS_THREADS * j) + e;
+                    const float v = x[j][e];
+                    if ((v < px || (v == px && tok > pt)) && v > bx) { bx = v; bt = tok; }       // (a thread's tokens ascend)
+                }
+            const float w = ob_wave_max(bx);
+            int wt2 = bx == w ? bt : 0x7fffffff;
+#pragma unroll
+            for (int k = 32; k; k >>= 1) wt2 = min(wt2, __shfl_xor(wt2, k, 64));
+            __syncthreads();
+            if (lane == 0) { red_m[wave] = w; red_i[wave] = wt2; }
+            __syncthreads();
+            px = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3]));
+            pt = 0x7fffffff;
+#pragma unroll
+            for (int w2 = 0; w2 < 4; ++w2)
+                if (red_m[w2] == px) pt = min(pt, red_i[w2]);
+            if (px == -INFINITY) break;
+            if (tid == 0) { lx[n] = px; lt[n] = pt; }
+        }
+    }
     if (tid == 0) {
-        double *out = A.sums + ((int64_t)row * A.chunks + chunk) * 2;
-        out[0] = (double)m;
-        out[1] = (red_s[0] + red_s[1]) + (red_s[2] + red_s[3]);
-    }
-    // ---- the wave's best, one after the other: the largest of the lanes' largest, in the lowest lane that has it
-    const int64_t list = ((int64_t)row * 4 * A.chunks + 4 * chunk + wave) * A.keep;
-    float bx = -INFINITY;
-    int be = 0;
-    for (int e = OB_BS_EPT - 1; e >= 0; --e)
-        if (x[e] >= bx) { bx = x[e]; be = e; }
-    for (int k = 0; k < A.keep; ++k) {
-        const float w = ob_wave_max(bx);
-        const unsigned long long who = __ballot(bx == w);
-        if (w == -INFINITY || !who) {                                            // nothing is left: the list ends here
-            if (lane == 0) A.list_t[list + k] = -1;
-            break;
-        }
-        const int first = __builtin_ctzll(who);
-        if (lane == first) {
-            A.list_x[list + k] = bx;
-            A.list_t[list + k] = t0 + be;
-#pragma unroll
-            for (int e = 0; e < OB_BS_EPT; ++e)
-                if (e == be) x[e] = -INFINITY;
-            bx = -INFINITY;
-#pragma unroll
-            for (int e = OB_BS_EPT - 1; e >= 0; --e)
-                if (x[e] >= bx) { bx = x[e]; be = e; }
-        }
+        A.sums[2 * list] = (double)m;
+        A.sums[2 * list + 1] = (red_s[0] + red_s[1]) + (red_s[2] + red_s[3]);
+        A.counts[list] = n;
     }
 }
 
-// candidate a in front of candidate b?  (value, logit, list); lists of a beam come one after the other, in the order of their tokens
-__device__ __forceinline__ bool ob_bs_before(double va, float xa, int la, double vb, float xb, int lb, int lists)
+// candidate a in front of candidate b?  (value, beam, logit, token)
+struct ObBsCand { double v; float x; int beam, tok; };
+__device__ __forceinline__ bool ob_bs_before(const ObBsCand &a, const ObBsCand &b)
 {
-    if (va != vb) return va > vb;
-    return xa != xb && la / lists == lb / lists ? xa > xb : la < lb;
+    if (a.v != b.v) return a.v > b.v;
+    if (a.beam != b.beam) return a.beam < b.beam;
+    return a.x != b.x ? a.x > b.x : a.tok < b.tok;
 }
 
-__global__ __launch_bounds__(OB_BS_THREADS) void ob_bs_pick_kernel(const ObBsArgs A)
+__global__ __launch_bounds__(OB_BS_PICK) void ob_bs_pick_kernel(const ObBsArgs A)
 {
-    __shared__ double row_v[32];                                                 // score - lse of a beam; NaN: it offers nothing
-    __shared__ double best_v[4];
-    __shared__ float best_x[4];
-    __shared__ int best_l[4];
+    __shared__ double row_v[OB_BS_MAX_BEAMS];                                    // lse of a beam; NaN: it offers nothing
+    __shared__ float red_t[OB_BS_PICK / 64];
+    __shared__ ObBsCand cand[OB_BS_RANKED];
+    __shared__ int n_s;
     const int group = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int lists = 4 * A.chunks, total = lists * A.beams;
-    for (int b = wave; b < A.beams; b += 4) {
-        const double *sm = A.sums + ((int64_t)(group * A.beams + b) * A.chunks) * 2;
+    const int room = ob_bs_list(A.keep), per_beam = A.chunks * room, total = A.beams * per_beam;
+    const int64_t list0 = (int64_t)group * A.beams * A.chunks;
+    if (tid == 0) n_s = 0;
+    for (int b = wave; b < A.beams; b += OB_BS_PICK / 64) {
+        const double *sm = A.sums + (list0 + (int64_t)b * A.chunks) * 2;
         double M = -INFINITY, s = 0.;
         for (int c = lane; c < A.chunks; c += 64) M = fmax(M, sm[2 * c]);
 #pragma unroll
@@ -137,56 +191,65 @@ __global__ __launch_bounds__(OB_BS_THREADS) void ob_bs_pick_kernel(const ObBsArg
         if (lane == 0) row_v[b] = M + log(s);
     }
     __syncthreads();
-    // a thread's lists tid, tid + 256, ..: the best of their heads
-    const auto value = [&](int l, int at, float &x) -> double {
-        const int b = l / lists;
-        const int64_t i = ((int64_t)group * total + l) * A.keep + at;
-        if (at >= A.keep || A.list_t[i] < 0) return -INFINITY;
-        x = A.list_x[i];
-        const double v = (double)A.scores[group * A.beams + b] + ((double)x - row_v[b]);
-        return v > -INFINITY ? v : -INFINITY;                                    // (NaN: no candidate)
+    const auto at = [&](int i, ObBsCand &c) -> bool {                            // candidate place i: false where there is none
+        const int l = i / room;
+        if (i - l * room >= A.counts[list0 + l]) return false;
+        c.beam = l / A.chunks;
+        c.x = A.list_x[list0 * room + i];
+        c.tok = A.list_t[list0 * room + i];
+        c.v = (double)A.scores[group * A.beams + c.beam] + ((double)c.x - row_v[c.beam]);
+        return c.v > -INFINITY;                                                  // (NaN: none)
     };
-    extern __shared__ unsigned char at_s[];                                      // how many of a list are taken, [total]
-    for (int l = tid; l < total; l += OB_BS_THREADS) at_s[l] = 0;
-    double bv;
-    float bx;
-    int bl;
-    const auto rescan = [&]() {
-        bv = -INFINITY; bx = 0.f; bl = 0x7fffffff;
-        for (int l = tid; l < total; l += OB_BS_THREADS) {
-            float x = 0.f;
-            const double v = value(l, at_s[l], x);
-            if (v > -INFINITY && ob_bs_before(v, x, l, bv, bx, bl, lists)) { bv = v; bx = x; bl = l; }
-        }
-    };
-    rescan();
-    for (int k = 0; k < A.keep; ++k) {
-        double v = bv;
-        float x = bx;
-        int l = bl;
-#pragma unroll
-        for (int o = 32; o; o >>= 1) {
-            const double v2 = __shfl_xor(v, o, 64);
-            const float x2 = __shfl_xor(x, o, 64);
-            const int l2 = __shfl_xor(l, o, 64);
-            if (ob_bs_before(v2, x2, l2, v, x, l, lists)) { v = v2; x = x2; l = l2; }
-        }
-        if (lane == 0) { best_v[wave] = v; best_x[wave] = x; best_l[wave] = l; }
-        __syncthreads();
-        v = best_v[0]; x = best_x[0]; l = best_l[0];
-#pragma unroll
-        for (int w = 1; w < 4; ++w)
-            if (ob_bs_before(best_v[w], best_x[w], best_l[w], v, x, l, lists)) { v = best_v[w]; x = best_x[w]; l = best_l[w]; }
-        const int64_t out = (int64_t)group * A.keep + k;
-        if (v == -INFINITY) {
-            if (tid == 0) { A.out_scores[out] = -INFINITY; A.out_beams[out] = -1; A.out_tokens[out] = -1; }
-        } else if (bl == l) {
-            A.out_scores[out] = (float)v;
-            A.out_beams[out] = l / lists;
-            A.out_tokens[out] = A.list_t[((int64_t)group * total + l) * A.keep + at_s[l]];
-            at_s[l] = (unsigned char)(at_s[l] + 1);
-            rescan();
-        }
-        __syncthreads();
+    float best = -INFINITY;
+    for (int i = tid; i < total; i += OB_BS_PICK) {
+        ObBsCand c;
+        if (at(i, c)) best = fmaxf(best, __double2float_rd(c.v));                // (rounded down: what reaches the threshold reaches it in 64 bits, too)
     }
+    const int waves = min(OB_BS_PICK / 64, (total + 63) / 64);                   // that have candidate places
+    const float wt = wave < waves ? ob_bs_kth(best, (A.keep + waves - 1) / waves) : INFINITY;
+    if (lane == 0) red_t[wave] = wt;
+    __syncthreads();
+    float t = red_t[0];
+#pragma unroll
+    for (int w = 1; w < OB_BS_PICK / 64; ++w) t = fminf(t, red_t[w]);
+    if (best >= t && best > -INFINITY)
+        for (int i = tid; i < total; i += OB_BS_PICK) {
+            ObBsCand c;
+            if (at(i, c) && c.v >= (double)t) {
+                const int k = atomicAdd(&n_s, 1);
+                if (k < OB_BS_RANKED) cand[k] = c;
+            }
+        }
+    __syncthreads();
+    int n = n_s;
+    const int64_t out = (int64_t)group * A.keep;
+    const auto put = [&](int k, const ObBsCand &c) { A.out_scores[out + k] = (float)c.v; A.out_beams[out + k] = c.beam; A.out_tokens[out + k] = c.tok; };
+    if (n <= OB_BS_RANKED) {
+        if (tid < n) {
+            const ObBsCand c = cand[tid];
+            int rank = 0;
+            for (int k = 0; k < n; ++k) rank += ob_bs_before(cand[k], c);
+            if (rank < A.keep) put(rank, c);
+        }
+    } else {                                                                     // one after the other: the best behind the last one
+        ObBsCand last = {INFINITY, INFINITY, -1, -1};
+        for (n = 0; n < A.keep; ++n) {
+            ObBsCand b = {-INFINITY, -INFINITY, 0x7fffffff, 0x7fffffff};
+            for (int i = tid; i < total; i += OB_BS_PICK) {
+                ObBsCand c;
+                if (at(i, c) && ob_bs_before(last, c) && ob_bs_before(c, b)) b = c;
+            }
+            __syncthreads();
+            cand[tid] = b;
+            __syncthreads();
+            for (int h = OB_BS_PICK / 2; h; h >>= 1) {
+                if (tid < h && ob_bs_before(cand[tid + h], cand[tid])) cand[tid] = cand[tid + h];
+                __syncthreads();
+            }
+            last = cand[0];
+            if (last.v == -INFINITY) break;
+            if (tid == 0) put(n, last);
+        }
+    }
+    if (tid >= n && tid < A.keep) put(tid, {-INFINITY, 0.f, -1, -1});
 }

@@ -2,16 +2,16 @@
 // prefix (len rows of one slot of the prefix cache, stored once for all rows of the group) and to its own later positions (rows
 // first .. pos of its own slot):
 //   o = sum_j e^{s_j} v_j / sum_j e^{s_j},  s_j = q . k_j / sqrt(D),  j over prefix and own keys together
-// A key range is a PART: its maximum m, sum l = sum e^{s - m} and o = sum e^{s - m} v in fp32; parts join by
-//   M = max m_p,  l = sum e^{m_p - M} l_p,  o = sum e^{m_p - M} o_p / l          (ob_sh_join_kernel)
-// so prefix chunks and own chunks are workgroups of one launch, and the order of the join is the order of the parts.
+// A range of keys leaves a PART: its maximum m, l = sum e^{s - m} and o = sum e^{s - m} v in fp32.  A part is also a state of the running
+// softmax, so parts join by starting from them:  M = max m_p,  l = sum e^{m_p - M} l_p,  o = sum e^{m_p - M} o_p / l.
+//   ob_sh_prefix_kernel / ob_sh_wide_kernel   parts of the prefixes: (kv head) x (block of the group's queries) x (chunk of keys)
+//   ob_sh_own_kernel                          a row's own keys, started from the prefix's parts: the outputs, or, where a row's own keys are
+//                                             split as well, parts again, which ob_sh_join_kernel joins
+// Where a prefix is so short that every row may read it again, the own kernel does, alone.  Parts are joined in their order: deterministic.
 //
-// Workgroup = (16 MT queries of one kv head) x (one chunk of keys): the queries of a prefix chunk are the rows of the group times
-// the query heads of the kv head, those of an own chunk one row's query heads.  Four waves take 32 keys in turn, each with its
-// own (m, l, o), joined through LDS at the end: no barrier in the loop, a wave's next 32 keys and values are on their way in
-// registers while it computes.  Both products are computed transposed, S^T = K Q^T and O^T = V^T P^T (MFMA 16x16x32): a lane holds
-// 4 consecutive keys of one query per 16-key tile, which are, for two tiles, its 8 k elements of the second product; V stays
-// row-major in the wave's part of the LDS and is transposed by ds_read_b64_tr_b16.
+// Both products are computed transposed, S^T = K Q^T and O^T = V^T P^T (MFMA 16x16x32): a lane holds 4 consecutive keys of one query
+// per 16-key tile, which are, for two tiles, its 8 k elements of the second product; V lies row-major in the LDS and is transposed by
+// ds_read_b64_tr_b16.  The sum of the weights is one more such product, with ones in V's place.
 // Scores, maxima, sums and outputs are fp32.  The weights e^{s - m} enter the second product as fp16 (relative error 2^-11 each, which the
 // sum averages; the output is rounded to fp16 anyway), the denominator sums the same rounded weights.
 #pragma once
@@ -29,12 +29,13 @@ struct ObShArgs {
     _Float16 *o;                       // [rows][H][D]
     const _Float16 *h_next;            // optional [H * D]
     const int *row_slot, *row_pos;     // device [rows]; row_slot NULL: slot = row
-    float *part_o;                     // [rows][H][splits][D]
-    float *part_ml;                    // [rows][H][splits][2]   {max (log2 domain), sum}
+    float *part_o;                     // [rows][H][psplits + osplits][D]
+    float *part_ml;                    // [rows][H][psplits + osplits][2]   {max (log2 domain), sum}
     long long p_max_len, max_len;
     int H, Hkv, rep, D, n_slots, rows, row_base;      // rows: of this launch, from row_base on
-    int pchunk, ochunk, psplits, osplits;             // keys per chunk; parts of a row: psplits of the prefix, then osplits of its own
-    int own_item0, own_mb, max_own;                   // first item of the own chunks; query blocks per row; most own positions
+    int pchunk, ochunk, psplits, osplits;             // keys per chunk; parts of a row: psplits of the prefix, then osplits of its own (0: one chunk, no part)
+    int own_mb, max_own;                              // query blocks per row and kv head; most own positions
+    int inline_prefix;                                // the own kernel reads the prefixes itself
     float scale_log2e;                                // log2(e) / sqrt(D)
     int n_groups;
     ObShGroup g[OB_SH_GROUPS];
@@ -44,14 +45,7 @@ typedef short ob_sh_v4s __attribute__((ext_vector_type(4)));
 typedef short ob_sh_v8s __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) ob_sh_v4s ob_sh_lds_v4s;
 
-// v over the wave's four 16-lane rows (same lane & 15)
-__device__ __forceinline__ float ob_sh_rows_sum(float v)
-{
-    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
+// largest over the wave's four 16-lane rows (same lane & 15)
 __device__ __forceinline__ float ob_sh_rows_max(float v)
 {
     auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -61,94 +55,59 @@ __device__ __forceinline__ float ob_sh_rows_max(float v)
 }
 __device__ __forceinline__ float ob_sh_weight(float m, float M) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M); }
 
-// LDS of a workgroup, floats: four waves' V tiles [32][DP] fp16, later two output buffers of 16 MT queries; behind them the waves' statistics
-template <int DP, int MT> constexpr int ob_sh_body_floats() { return (4 * 32 * DP * 2 > 2 * MT * 16 * DP * 4 ? 4 * 32 * DP * 2 : 2 * MT * 16 * DP * 4) / 4; }
-template <int DP, int MT> constexpr int ob_sh_lds_floats() { return ob_sh_body_floats<DP, MT>() + 4 * MT * 16 * 2; }
+// LDS place (halves) of 16-byte piece p of row r of a tile of DP columns: pairs of pieces swizzled by the row
+template <int DP> __device__ __forceinline__ int ob_sh_place(int r, int p) { return r * DP + 8 * (2 * ((p >> 1) ^ (r & (DP / 16 - 1))) + (p & 1)); }
 
-// Keys k0 .. k1 - 1 of one slot and kv head (kb, vb: its rows) for queries qi0 .. of nq, query i = (row row0 + i / rep, head kvh rep + i % rep);
-// the result is part `split` of each.  DP: head size padded to 64 or 128 (EXACT: it is the head size).
+// The running softmax of 16 MT queries of a wave: query lane & 15 of each tile, output column 16 dt + 4 (lane >> 4) + i
 template <int DP, int MT, bool EXACT>
-__device__ __forceinline__ void ob_sh_body(const ObShArgs &A, const _Float16 *kb, const _Float16 *vb, int k0, int k1, int row0, int qi0, int nq, int kvh,
-                                           int split, float *sm)
-{
-    constexpr int DK = DP / 32, DT = DP / 16, PPR = DP / 8, RPL = 64 / PPR, NV = 32 / RPL;       // pieces of 16 bytes per row, rows per load, loads of a V tile
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, g = lane >> 4;
-    const int D = EXACT ? DP : A.D;
-    _Float16 *vt = reinterpret_cast<_Float16 *>(sm) + wave * 32 * DP;
+struct ObShWave {
+    static constexpr int DK = DP / 32, DT = DP / 16;
     ob_half8 qf[MT][DK];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        const int qi = min(qi0 + 16 * mt + lr, nq - 1);
-        const _Float16 *qr = A.q + ((int64_t)(row0 + qi / A.rep) * A.H + kvh * A.rep + qi % A.rep) * D;
-#pragma unroll
-        for (int j = 0; j < DK; ++j) {
-            const int d = 32 * j + 8 * g;
-            qf[mt][j] = EXACT || d < D ? *reinterpret_cast<const ob_half8 *>(qr + d) : (ob_half8)(_Float16)0;
-        }
-    }
-    float m[MT], l[MT];
+    ob_float4 m;                       // log2 domain, of the MT tiles (a vector: hipcc keeps an array of them in memory)
+    ob_float4 l[MT];                   // sum of the weights, in each of the four
     ob_float4 acc[MT][DT];
+
+    // query i of the block is query qi0 + i of nq: row row0 + (qi0 + i) / rep, head kvh rep + (qi0 + i) % rep
+    __device__ __forceinline__ void init(const ObShArgs &A, int row0, int qi0, int nq, int kvh)
+    {
+        const int lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4, D = EXACT ? DP : A.D;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        m[mt] = -INFINITY; l[mt] = 0.f;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) acc[mt][dt] = (ob_float4){0.f, 0.f, 0.f, 0.f};
-    }
-    ob_half8 kf[2][DK], vr[NV];
-    const int vrow = lane / PPR, vpc = lane % PPR;                     // this lane's piece of a V load: row vrow + RPL i, piece vpc
-    const auto load_k = [&](int base) {
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-            const _Float16 *r = kb + (int64_t)min(base + 16 * kt + lr, k1 - 1) * D;
+        for (int mt = 0; mt < MT; ++mt) {
+            const int qi = min(qi0 + 16 * mt + lr, nq - 1);
+            const _Float16 *qr = A.q + ((int64_t)(row0 + qi / A.rep) * A.H + kvh * A.rep + qi % A.rep) * D;
 #pragma unroll
             for (int j = 0; j < DK; ++j) {
                 const int d = 32 * j + 8 * g;
-                kf[kt][j] = EXACT || d < D ? *reinterpret_cast<const ob_half8 *>(r + d) : (ob_half8)(_Float16)0;
+                qf[mt][j] = EXACT || d < D ? *reinterpret_cast<const ob_half8 *>(qr + d) : (ob_half8)(_Float16)0;
             }
+            m[mt] = -INFINITY;
+            l[mt] = (ob_float4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) acc[mt][dt] = (ob_float4){0.f, 0.f, 0.f, 0.f};
         }
-    };
-    const auto load_v = [&](int base) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const _Float16 *r = vb + (int64_t)min(base + vrow + RPL * i, k1 - 1) * D + 8 * vpc;
-            vr[i] = EXACT || 8 * vpc < D ? *reinterpret_cast<const ob_half8 *>(r) : (ob_half8)(_Float16)0;
-        }
-    };
-    int base = k0 + 32 * wave;
-    if (base < k1) { load_k(base); load_v(base); }
-    for (; base < k1; base += 128) {
-        const bool tail = base + 32 > k1, more = base + 128 < k1;
-        // V tile into the LDS, pairs of pieces swizzled by the row; rows beyond the range as zeros (their weights are zero, their values may be anything)
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int row = vrow + RPL * i;
-            if (tail && base + row >= k1) vr[i] = (ob_half8)(_Float16)0;
-            *reinterpret_cast<ob_half8 *>(vt + row * DP + 8 * (2 * ((vpc >> 1) ^ (row & (DT - 1))) + (vpc & 1))) = vr[i];
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        if (more) load_v(base + 128);
-        ob_float4 s[MT][2];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-                s[mt][kt] = (ob_float4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int j = 0; j < DK; ++j) s[mt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[kt][j], qf[mt][j], s[mt][kt], 0, 0, 0);
-            }
-        if (more) load_k(base + 128);
-        ob_half8 pb[MT];
+    }
+
+    // Weights of 32 keys from key `base` on (kf: their rows); keys from `end` on count for nothing
+    __device__ __forceinline__ void weights(const ob_half8 (&kf)[2][DK], float scale, int base, int end, ob_half8 (&pb)[MT])
+    {
+        const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-            float x[8], mx = -INFINITY;
+            ob_float4 s[2];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[e] = s[mt][e >> 2][e & 3] * A.scale_log2e;
-                if (tail && base + 16 * (e >> 2) + 4 * g + (e & 3) >= k1) x[e] = -INFINITY;
-                mx = fmaxf(mx, x[e]);
+            for (int kt = 0; kt < 2; ++kt) {
+                s[kt] = (ob_float4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < DK; ++j) s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[kt][j], qf[mt][j], s[kt], 0, 0, 0);
             }
-            mx = ob_sh_rows_max(mx);
+            if (base + 32 > end)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (base + 16 * (e >> 2) + 4 * g + (e & 3) >= end) s[e >> 2][e & 3] = -INFINITY;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, s[e >> 2][e & 3]);
+            mx = ob_sh_rows_max(mx) * scale;
             // the running maximum moves only where a tile exceeds it by 2^8: the weights stay far inside fp16, the output is rescaled seldom
             if (__any(mx > m[mt] + 8.f)) {
                 const float mn = fmaxf(m[mt], mx), f = ob_sh_weight(m[mt], mn);
@@ -159,74 +118,237 @@ __device__ __forceinline__ void ob_sh_body(const ObShArgs &A, const _Float16 *kb
             }
             const float mu = m[mt] == -INFINITY ? 0.f : m[mt];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                pb[mt][e] = (_Float16)__builtin_amdgcn_exp2f(x[e] - mu);
-                l[mt] += (float)pb[mt][e];
-            }
+            for (int e = 0; e < 8; ++e) pb[mt][e] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 2][e & 3], scale, -mu));
         }
+    }
+
+    // acc += weights . values, vt: the 32 keys' rows in the LDS
+    __device__ __forceinline__ void values(const _Float16 *vt, const ob_half8 (&pb)[MT])
+    {
+        const int lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4;
+        const ob_half8 one = (ob_half8)(_Float16)1;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) l[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(one, pb[mt], l[mt], 0, 0, 0);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
             ob_sh_v4s a[2];
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-                const int row = 16 * kt + 4 * g + (lr >> 2);
-                a[kt] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (ob_sh_lds_v4s *)(vt + row * DP + 8 * (2 * (dt ^ (row & (DT - 1))) + ((lr & 3) >> 1)) + 4 * (lr & 1)));
-            }
+            for (int kt = 0; kt < 2; ++kt)
+                a[kt] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ob_sh_lds_v4s *)(vt + ob_sh_place<DP>(16 * kt + 4 * g + (lr >> 2), 2 * dt + ((lr & 3) >> 1)) + 4 * (lr & 1)));
             const ob_sh_v8s av = {a[0][0], a[0][1], a[0][2], a[0][3], a[1][0], a[1][1], a[1][2], a[1][3]};
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) acc[mt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ob_half8, av), pb[mt], acc[mt][dt], 0, 0, 0);
         }
+    }
+};
+
+// The keys of a workgroup's item: keys begin .. end - 1 of the rows from k, v on
+struct ObShRange { const _Float16 *k, *v; int begin, end; };
+__device__ __forceinline__ int ob_sh_tiles(int n) { return (n + 31) >> 5; }
+
+// A workgroup's four waves over the keys of two ranges one after the other, 32 in turn; each starts from what W holds, the four results are joined in wave 0's W.
+// K goes from memory to registers in the layout of its product, V by registers into the wave's own part of the LDS: no barrier in the loop, the
+// next 32 keys and values are on their way while a wave computes.
+template <int DP, int MT, bool EXACT> constexpr int ob_sh_body_floats() { return (4 * 32 * DP * 2 > 2 * MT * 16 * DP * 4 ? 4 * 32 * DP * 2 : 2 * MT * 16 * DP * 4) / 4; }
+template <int DP, int MT, bool EXACT> constexpr int ob_sh_lds_floats() { return ob_sh_body_floats<DP, MT, EXACT>() + 4 * MT * 16 * 2; }
+
+template <int DP, int MT, bool EXACT>
+__device__ __forceinline__ void ob_sh_sweep(const ObShArgs &A, const ObShRange &R0, const ObShRange &R1, ObShWave<DP, MT, EXACT> &W, float *sm)
+{
+    constexpr int DK = DP / 32, DT = DP / 16, PPR = DP / 8, RPL = 64 / PPR, NV = 32 / RPL;       // pieces of 16 bytes per row, rows per load, loads of a V tile
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 15, g = lane >> 4;
+    const int D = EXACT ? DP : A.D;
+    _Float16 *vt = reinterpret_cast<_Float16 *>(sm) + wave * 32 * DP;
+    ob_half8 kf[2][DK], vr[NV];
+    const int vrow = lane / PPR, vpc = lane % PPR;                     // this lane's piece of a V load: row vrow + RPL i, piece vpc
+    const int n0 = ob_sh_tiles(R0.end - R0.begin), n = n0 + ob_sh_tiles(R1.end - R1.begin);
+    const auto load_k = [&](int t) {
+        const bool one = t < n0;
+        const int last = (one ? R0.end : R1.end) - 1, base = one ? R0.begin + 32 * t : R1.begin + 32 * (t - n0);
+        const _Float16 *kb = one ? R0.k : R1.k;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            const _Float16 *p = kb + (int64_t)min(base + 16 * kt + lr, last) * D;
+#pragma unroll
+            for (int j = 0; j < DK; ++j) {
+                const int d = 32 * j + 8 * g;
+                kf[kt][j] = EXACT || d < D ? *reinterpret_cast<const ob_half8 *>(p + d) : (ob_half8)(_Float16)0;
+            }
+        }
+    };
+    const auto load_v = [&](int t) {
+        const bool one = t < n0;
+        const int last = (one ? R0.end : R1.end) - 1, base = one ? R0.begin + 32 * t : R1.begin + 32 * (t - n0);
+        const _Float16 *vb = one ? R0.v : R1.v;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const _Float16 *p = vb + (int64_t)min(base + vrow + RPL * i, last) * D + 8 * vpc;
+            vr[i] = EXACT || 8 * vpc < D ? *reinterpret_cast<const ob_half8 *>(p) : (ob_half8)(_Float16)0;
+        }
+    };
+    if (wave < n) { load_v(wave); load_k(wave); }                      // (values first, as in the loop: what waits for them lets the keys come)
+    for (int t = wave; t < n; t += 4) {
+        const bool one = t < n0;
+        const int end = one ? R0.end : R1.end, base = one ? R0.begin + 32 * t : R1.begin + 32 * (t - n0);
+        // rows beyond the range as zeros (their weights are zero, their values may be anything)
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int row = vrow + RPL * i;
+            if (base + 32 > end && base + row >= end) vr[i] = (ob_half8)(_Float16)0;
+            *reinterpret_cast<ob_half8 *>(vt + ob_sh_place<DP>(row, vpc)) = vr[i];
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (t + 4 < n) load_v(t + 4);
+        ob_half8 pb[MT];
+        W.weights(kf, A.scale_log2e, base, end, pb);
+        if (t + 4 < n) load_k(t + 4);
+        W.values(vt, pb);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
     // ---- join the four waves: statistics, then the outputs in two steps through two buffers
-    float *st = sm + ob_sh_body_floats<DP, MT>();                      // [4 waves][16 MT][2]
+    float *st = sm + ob_sh_body_floats<DP, MT, EXACT>();               // [4 waves][16 MT][2]
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        l[mt] = ob_sh_rows_sum(l[mt]);
-        if (g == 0) { st[(wave * 16 * MT + 16 * mt + lr) * 2] = m[mt]; st[(wave * 16 * MT + 16 * mt + lr) * 2 + 1] = l[mt]; }
-    }
+    for (int mt = 0; mt < MT; ++mt)
+        if (g == 0) *reinterpret_cast<ob_float2 *>(st + (wave * 16 * MT + 16 * mt + lr) * 2) = (ob_float2){W.m[mt], W.l[mt][0]};
     __syncthreads();
     ob_float4 *buf = reinterpret_cast<ob_float4 *>(sm);                // [2][MT][DT][64]
-    float M[MT], lt[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         const float *sq = st + (16 * mt + lr) * 2;
-        M[mt] = fmaxf(fmaxf(sq[0], sq[32 * MT]), fmaxf(sq[64 * MT], sq[96 * MT]));
-        lt[mt] = 0.f;
+        const float M = fmaxf(fmaxf(sq[0], sq[32 * MT]), fmaxf(sq[64 * MT], sq[96 * MT])), f = ob_sh_weight(W.m[mt], M);
+        float lt = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) lt[mt] += sq[32 * MT * w + 1] * ob_sh_weight(sq[32 * MT * w], M[mt]);
-        const float f = ob_sh_weight(m[mt], M[mt]);
+        for (int w = 0; w < 4; ++w) lt += sq[32 * MT * w + 1] * ob_sh_weight(sq[32 * MT * w], M);
+        W.m[mt] = M;
+        W.l[mt][0] = lt;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-            acc[mt][dt] *= f;
-            if (wave >= 2) buf[((wave - 2) * MT * DT + mt * DT + dt) * 64 + lane] = acc[mt][dt];
-        }
+        for (int dt = 0; dt < DT; ++dt) W.acc[mt][dt] *= f;
+    }
+    if (wave >= 2)
+#pragma unroll
+        for (int i = 0; i < MT * DT; ++i) buf[((wave - 2) * MT * DT + i) * 64 + lane] = W.acc[i / DT][i % DT];
+    __syncthreads();
+    if (wave < 2) {
+#pragma unroll
+        for (int i = 0; i < MT * DT; ++i) W.acc[i / DT][i % DT] += buf[(wave * MT * DT + i) * 64 + lane];
+        if (wave == 1)
+#pragma unroll
+            for (int i = 0; i < MT * DT; ++i) buf[(MT * DT + i) * 64 + lane] = W.acc[i / DT][i % DT];
     }
     __syncthreads();
-    if (wave < 2)
+    if (wave == 0)
 #pragma unroll
-        for (int i = 0; i < MT * DT; ++i) {
-            acc[i / DT][i % DT] += buf[(wave * MT * DT + i) * 64 + lane];
-            if (wave == 1) buf[(MT * DT + i) * 64 + lane] = acc[i / DT][i % DT];
-        }
-    __syncthreads();
-    if (wave == 0) {
-        const int splits = A.psplits + A.osplits;
+        for (int i = 0; i < MT * DT; ++i) W.acc[i / DT][i % DT] += buf[(MT * DT + i) * 64 + lane];
+}
+
+// What W holds of the queries qi0 .. of nq as their part `split`
+template <int DP, int MT, bool EXACT>
+__device__ __forceinline__ void ob_sh_store(const ObShArgs &A, const ObShWave<DP, MT, EXACT> &W, int row0, int qi0, int nq, int kvh, int split)
+{
+    const int lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4, D = EXACT ? DP : A.D;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            const int qi = qi0 + 16 * mt + lr;
-            if (qi < nq) {
-                const int64_t p = ((int64_t)(row0 + qi / A.rep) * A.H + kvh * A.rep + qi % A.rep) * splits + split;
-                if (g == 0) *reinterpret_cast<ob_float2 *>(A.part_ml + 2 * p) = (ob_float2){M[mt], lt[mt]};
+    for (int mt = 0; mt < MT; ++mt) {
+        const int qi = qi0 + 16 * mt + lr;
+        if (qi >= nq) continue;
+        const int64_t p = ((int64_t)(row0 + qi / A.rep) * A.H + kvh * A.rep + qi % A.rep) * (A.psplits + A.osplits) + split;
+        if (g == 0) *reinterpret_cast<ob_float2 *>(A.part_ml + 2 * p) = (ob_float2){W.m[mt], W.l[mt][0]};
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-                    if (EXACT || 16 * dt + 4 * g < D)
-                        *reinterpret_cast<ob_float4 *>(A.part_o + p * D + 16 * dt + 4 * g) = acc[mt][dt] + buf[((MT + mt) * DT + dt) * 64 + lane];
-            }
-        }
+        for (int dt = 0; dt < DP / 16; ++dt)
+            if (EXACT || 16 * dt + 4 * g < D) *reinterpret_cast<ob_float4 *>(A.part_o + p * D + 16 * dt + 4 * g) = W.acc[mt][dt];
     }
+}
+
+// a prefix item: kv head kvh, keys k0 .. k1 - 1 of the group's prefix (rows from kb, vb on), chunk and block of `per` queries
+struct ObShItem { int kvh, chunk, qi0, k0, k1; const _Float16 *kb, *vb; };
+__device__ __forceinline__ ObShItem ob_sh_item(const ObShArgs &A, int per, ObShGroup &G)
+{
+    ObShItem I;
+    const int item = blockIdx.x / A.Hkv;
+    I.kvh = blockIdx.x - item * A.Hkv;
+    int gi = 0;
+    while (item >= A.g[gi].item_end) ++gi;
+    G = A.g[gi];
+    const int at = item - (gi ? A.g[gi - 1].item_end : 0), mb = at / G.chunks;
+    I.chunk = at - mb * G.chunks;
+    I.qi0 = per * mb;
+    I.k0 = I.chunk * A.pchunk;
+    I.k1 = min(G.len, I.k0 + A.pchunk);
+    const int64_t row = ((int64_t)G.slot * A.Hkv + I.kvh) * A.p_max_len * A.D;
+    I.kb = A.pk + row;
+    I.vb = A.pv + row;
+    return I;
+}
+
+// Up to 32 queries of a group and kv head: the four waves share the keys out.
+template <int DP, int MT, bool EXACT>
+__global__ __launch_bounds__(OB_SH_THREADS, 2) void ob_sh_prefix_kernel(const ObShArgs A)
+{
+    __shared__ __attribute__((aligned(16))) float sm[ob_sh_lds_floats<DP, MT, EXACT>()];
+    ObShGroup G;
+    const ObShItem I = ob_sh_item(A, 16 * MT, G);
+    ObShWave<DP, MT, EXACT> W;
+    W.init(A, G.row0, I.qi0, G.n * A.rep, I.kvh);
+    ob_sh_sweep<DP, MT, EXACT>(A, {I.kb, I.vb, I.k0, I.k1}, {I.kb, I.vb, 0, 0}, W, sm);
+    if (threadIdx.x < 64) ob_sh_store<DP, MT, EXACT>(A, W, G.row0, I.qi0, G.n * A.rep, I.kvh, I.chunk);
+}
+
+// More queries: the four waves share the queries out, 16 MT each, over tiles of 64 keys and values that they read from the LDS together (two tiles there,
+// a third on its way in registers; one barrier a tile).
+template <int DP, int MT, bool EXACT>
+__global__ __launch_bounds__(OB_SH_THREADS, MT < 4 ? 2 : 1) void ob_sh_wide_kernel(const ObShArgs A)
+{
+    constexpr int DK = DP / 32, PPR = DP / 8, NP = 64 * PPR / OB_SH_THREADS, RPL = OB_SH_THREADS / PPR;      // pieces of a thread, rows apart
+    __shared__ __attribute__((aligned(16))) _Float16 kv[2][2][64 * DP];
+    ObShGroup G;
+    const ObShItem I = ob_sh_item(A, 64 * MT, G);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, g = lane >> 4;
+    const int D = EXACT ? DP : A.D, qi0 = I.qi0 + 16 * MT * wave, nq = G.n * A.rep;
+    ObShWave<DP, MT, EXACT> W;
+    W.init(A, G.row0, qi0, nq, I.kvh);
+    ob_half8 kr[NP], vr[NP];
+    const int prow = tid / PPR, ppc = tid % PPR;
+    const bool there = EXACT || 8 * ppc < D;
+    const auto load = [&](int base) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int64_t at = (int64_t)min(base + prow + RPL * i, I.k1 - 1) * D + 8 * ppc;
+            kr[i] = there ? *reinterpret_cast<const ob_half8 *>(I.kb + at) : (ob_half8)(_Float16)0;
+            vr[i] = there ? *reinterpret_cast<const ob_half8 *>(I.vb + at) : (ob_half8)(_Float16)0;
+        }
+    };
+    const auto store = [&](int base, int b) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int row = prow + RPL * i;
+            if (base + 64 > I.k1 && base + row >= I.k1) vr[i] = (ob_half8)(_Float16)0;
+            *reinterpret_cast<ob_half8 *>(&kv[b][0][ob_sh_place<DP>(row, ppc)]) = kr[i];
+            *reinterpret_cast<ob_half8 *>(&kv[b][1][ob_sh_place<DP>(row, ppc)]) = vr[i];
+        }
+    };
+    load(I.k0);
+    store(I.k0, 0);
+    if (I.k0 + 64 < I.k1) load(I.k0 + 64);
+    __syncthreads();
+    int b = 0;
+    for (int base = I.k0; base < I.k1; base += 64, b ^= 1) {
+        if (base + 64 < I.k1) store(base + 64, b ^ 1);
+        if (base + 128 < I.k1) load(base + 128);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (base + 32 * h >= I.k1) break;
+            ob_half8 kf[2][DK], pb[MT];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int j = 0; j < DK; ++j) kf[kt][j] = *reinterpret_cast<const ob_half8 *>(&kv[b][0][ob_sh_place<DP>(32 * h + 16 * kt + lr, 4 * j + g)]);
+            W.weights(kf, A.scale_log2e, base + 32 * h, I.k1, pb);
+            W.values(&kv[b][1][32 * h * DP], pb);
+        }
+        __syncthreads();
+    }
+    ob_sh_store<DP, MT, EXACT>(A, W, G.row0, qi0, nq, I.kvh, I.chunk);
 }
 
 // own keys of a row (0: none), false for an idle row
@@ -239,27 +361,67 @@ __device__ __forceinline__ bool ob_sh_row(const ObShArgs &A, int row, int first,
     return true;
 }
 
-template <int DP, int MT, bool EXACT>
-__global__ __launch_bounds__(OB_SH_THREADS) void ob_sh_part_kernel(const ObShArgs A)
+// One row's queries of a kv head (16 of them: block mb) over its own keys.  osplits 0: all of them, started from the prefix's parts (the waves take
+// them in turn) or from its keys; the output.  Else chunk `split` of them as a part.
+template <int DP, bool EXACT>
+__global__ __launch_bounds__(OB_SH_THREADS, 2) void ob_sh_own_kernel(const ObShArgs A)
 {
-    __shared__ __attribute__((aligned(16))) float sm[ob_sh_lds_floats<DP, MT>()];
-    const int item = blockIdx.x / A.Hkv, kvh = blockIdx.x % A.Hkv;
-    if (item < A.own_item0) {
-        int gi = 0;
-        while (item >= A.g[gi].item_end) ++gi;
-        const ObShGroup G = A.g[gi];
-        const int at = item - (gi ? A.g[gi - 1].item_end : 0), chunk = at % G.chunks, mb = at / G.chunks;
-        const int64_t row = ((int64_t)G.slot * A.Hkv + kvh) * A.p_max_len * A.D;
-        ob_sh_body<DP, MT, EXACT>(A, A.pk + row, A.pv + row, chunk * A.pchunk, min(G.len, (chunk + 1) * A.pchunk), G.row0, 16 * MT * mb, G.n * A.rep, kvh, chunk, sm);
-        return;
-    }
-    const int at = item - A.own_item0, r = A.row_base + at % A.rows, mb = at / A.rows % A.own_mb, split = at / A.rows / A.own_mb;
+    constexpr int DT = DP / 16;
+    __shared__ __attribute__((aligned(16))) float sm[ob_sh_lds_floats<DP, 1, EXACT>()];
+    const int item = blockIdx.x / A.Hkv, kvh = blockIdx.x - item * A.Hkv;
+    const int at = item / A.rows, r = A.row_base + item - at * A.rows, split = at / A.own_mb, mb = at - split * A.own_mb;
     int gi = 0, slot, own;
     while (r >= A.g[gi].row0 + A.g[gi].n) ++gi;
-    const int first = A.g[gi].first;
-    if (!ob_sh_row(A, r, first, slot, own) || split * A.ochunk >= own) return;
+    const ObShGroup &G = A.g[gi];
+    const int first = G.first;
+    if (!ob_sh_row(A, r, first, slot, own)) return;                               // idle: its output stays as it is
+    const bool parts = A.osplits > 0;
+    if (parts && split * A.ochunk >= own) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, g = lane >> 4, D = EXACT ? DP : A.D;
+    ObShWave<DP, 1, EXACT> W;
+    W.init(A, r, 16 * mb, A.rep, kvh);
+    const int qi = 16 * mb + lr, head = kvh * A.rep + qi;
+    const bool mine = qi < A.rep;
+    if (!parts && !A.inline_prefix) {
+        const int64_t p0 = ((int64_t)r * A.H + (mine ? head : 0)) * A.psplits;
+        for (int s = wave; s < G.chunks; s += 4) {
+            const ob_float2 ml = mine ? *reinterpret_cast<const ob_float2 *>(A.part_ml + 2 * (p0 + s)) : (ob_float2){-INFINITY, 0.f};
+            const float M = fmaxf(W.m[0], ml[0]), f = ob_sh_weight(W.m[0], M), x = ob_sh_weight(ml[0], M);
+            W.m[0] = M;
+            W.l[0] = W.l[0] * f + x * ml[1];
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const bool in = mine && (EXACT || 16 * dt + 4 * g < D);
+                const ob_float4 o = in ? *reinterpret_cast<const ob_float4 *>(A.part_o + (p0 + s) * D + 16 * dt + 4 * g) : (ob_float4){0.f, 0.f, 0.f, 0.f};
+                W.acc[0][dt] = W.acc[0][dt] * f + o * x;
+            }
+        }
+    }
     const int64_t row = ((int64_t)slot * A.Hkv + kvh) * A.max_len * A.D;
-    ob_sh_body<DP, 1, EXACT>(A, A.k + row, A.v + row, first + split * A.ochunk, first + min(own, (split + 1) * A.ochunk), r, 16 * mb, A.rep, kvh, A.psplits + split, sm);
+    const int64_t prow = A.inline_prefix ? ((int64_t)G.slot * A.Hkv + kvh) * A.p_max_len * A.D : 0;
+    const int k0 = first + (parts ? split * A.ochunk : 0), k1 = first + (parts ? min(own, (split + 1) * A.ochunk) : own);
+    ob_sh_sweep<DP, 1, EXACT>(A, {A.pk + prow, A.pv + prow, 0, A.inline_prefix ? G.len : 0}, {A.k + row, A.v + row, k0, k1}, W, sm);
+    if (wave) return;
+    if (parts) {
+        ob_sh_store<DP, 1, EXACT>(A, W, r, 16 * mb, A.rep, kvh, A.psplits + split);
+        return;
+    }
+    if (!mine) return;
+    const bool any = G.len > 0 || own > 0;                                         // no key at all: zeros
+    const float inv = 1.f / W.l[0][0];
+    _Float16 *out = A.o + ((int64_t)r * A.H + head) * D;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+        const int d = 16 * dt + 4 * g;
+        if (!EXACT && d >= D) continue;
+        ob_half4 y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            y[i] = (_Float16)(any ? W.acc[0][dt][i] * inv : 0.f);
+            if (A.h_next) y[i] *= A.h_next[head * D + d + i];
+        }
+        *reinterpret_cast<ob_half4 *>(out + d) = y;
+    }
 }
 
 // A wave per (row, head): its parts in order, two output columns a lane.
@@ -303,5 +465,5 @@ __global__ __launch_bounds__(OB_SH_THREADS) void ob_sh_join_kernel(const ObShArg
     ob_half2 y = {(_Float16)0, (_Float16)0};                                       // no key at all: zeros
     if (n) { y[0] = (_Float16)(o[0] / l); y[1] = (_Float16)(o[1] / l); }
     if (A.h_next) { y[0] *= A.h_next[head * A.D + d]; y[1] *= A.h_next[head * A.D + d + 1]; }
-    out[0] = y[0]; out[1] = y[1];
+    *reinterpret_cast<ob_half2 *>(out) = y;
 }

@@ -17,24 +17,33 @@ static const int64_t OB_MAX_WGS = 0xffffff;            // workgroups of 256 thre
 static const int64_t OB_SH_MAX_LEN = 1 << 30;         // (positions and their chunks are counted in 32 bits)
 
 // ------------------------------------------------------------------------------------------- attention over a shared prefix --
-struct ObShPlan { int mt, pchunk, ochunk, psplits, osplits, own_mb; };
+// form: 0, 1: ob_sh_prefix_kernel of 16, 32 queries; 2, 3, 4: ob_sh_wide_kernel of 64, 128, 256; osplits 0: a row's own keys are one chunk
+struct ObShPlan { int form, per, pchunk, ochunk, psplits, osplits, own_mb, inline_prefix; };
 
 static ObShPlan ob_sh_plan(const onebit_prefix_t *groups, int32_t n_groups, int64_t rows, int32_t n_heads, int32_t n_kv_heads, int64_t max_own)
 {
     ObShPlan p = {};
     const int64_t rep = n_heads / n_kv_heads;
-    int64_t most = 1, longest = 0, work = 0;
+    int64_t most = 1, longest = 0, again = 0, work = 0;
     for (int i = 0; i < n_groups; ++i) {
         if (groups[i].len > 0) most = std::max<int64_t>(most, groups[i].n * rep);
         longest = std::max<int64_t>(longest, groups[i].len);
+        again += (int64_t)groups[i].n * groups[i].len;
     }
-    p.mt = most <= 16 ? 1 : most <= 32 ? 2 : 4;
-    for (int i = 0; i < n_groups; ++i) work += ob_up(groups[i].n * rep, 16 * p.mt) * groups[i].len * n_kv_heads;
-    p.pchunk = (int)(128 * std::max<int64_t>(1, ob_up(work, 768 * 128)));
-    p.psplits = (int)ob_up(longest, p.pchunk);
     p.own_mb = (int)ob_up(rep, 16);
-    p.ochunk = (int)(128 * std::max<int64_t>(1, ob_up(rows * n_kv_heads * p.own_mb * max_own, 1024 * 128)));
-    p.osplits = (int)ob_up(max_own, p.ochunk);
+    const int64_t own = rows * n_kv_heads * p.own_mb;                    // workgroups of one chunk per row
+    if (own < 256 && max_own > 512) {
+        p.ochunk = (int)(128 * std::max<int64_t>(2, ob_up(own * max_own, 512 * 128)));
+        p.osplits = (int)ob_up(max_own, p.ochunk);
+    }
+    if (p.osplits <= 1) { p.osplits = 0; p.ochunk = 1; }
+    p.inline_prefix = p.osplits == 0 && longest <= 256 && again * n_kv_heads * p.own_mb <= 64 * 1024;
+    if (p.inline_prefix) return p;
+    p.form = most <= 16 ? 0 : most <= 32 ? 1 : most <= 64 ? 2 : most <= 128 ? 3 : 4;
+    p.per = 16 << p.form;
+    for (int i = 0; i < n_groups; ++i) work += ob_up(groups[i].n * rep, p.per) * groups[i].len * n_kv_heads;
+    p.pchunk = (int)(128 * std::max<int64_t>(1, ob_up(work, (p.form == 4 ? 256 : 512) * 128)));
+    p.psplits = (int)ob_up(longest, p.pchunk);
     return p;
 }
 
@@ -62,15 +71,21 @@ extern "C" size_t onebit_attention_shared_scratch_bytes(const onebit_prefix_t *g
 {
     if (rows <= 0 || ob_sh_check(groups, n_groups, rows, n_heads, n_kv_heads, head_dim, max_own)) return 0;
     const ObShPlan p = ob_sh_plan(groups, n_groups, rows, n_heads, n_kv_heads, max_own);
-    return (size_t)rows * n_heads * (p.psplits + p.osplits) * (head_dim + 2) * 4 + 256;
+    return (size_t)rows * n_heads * (p.psplits + p.osplits) * (head_dim + 2) * 4 + 16;
 }
 
-template <int DP, int MT>
-static void ob_sh_launch(const ObShArgs &a, int64_t items, hipStream_t s)
+template <int DP, bool EXACT>
+static void ob_sh_launch(const ObShArgs &a, int form, int64_t prefix_items, int64_t own_items, hipStream_t s)
 {
-    const dim3 grid((unsigned)(items * a.Hkv));
-    if (a.D == DP) hipLaunchKernelGGL((ob_sh_part_kernel<DP, MT, true>), grid, dim3(OB_SH_THREADS), 0, s, a);
-    else hipLaunchKernelGGL((ob_sh_part_kernel<DP, MT, false>), grid, dim3(OB_SH_THREADS), 0, s, a);
+    const dim3 block(OB_SH_THREADS), pg((unsigned)(prefix_items * a.Hkv)), og((unsigned)(own_items * a.Hkv));
+    if (prefix_items > 0) {
+        if (form == 0) hipLaunchKernelGGL((ob_sh_prefix_kernel<DP, 1, EXACT>), pg, block, 0, s, a);
+        else if (form == 1) hipLaunchKernelGGL((ob_sh_prefix_kernel<DP, 2, EXACT>), pg, block, 0, s, a);
+        else if (form == 2) hipLaunchKernelGGL((ob_sh_wide_kernel<DP, 1, EXACT>), pg, block, 0, s, a);
+        else if (form == 3) hipLaunchKernelGGL((ob_sh_wide_kernel<DP, 2, EXACT>), pg, block, 0, s, a);
+        else hipLaunchKernelGGL((ob_sh_wide_kernel<DP, 4, EXACT>), pg, block, 0, s, a);
+    }
+    hipLaunchKernelGGL((ob_sh_own_kernel<DP, EXACT>), og, block, 0, s, a);
 }
 
 extern "C" int onebit_attention_shared_rows(const void *q, const void *prefix_k, const void *prefix_v, const void *k_cache, const void *v_cache, void *o,
@@ -93,7 +108,7 @@ extern "C" int onebit_attention_shared_rows(const void *q, const void *prefix_k,
     }
     if (rows == 0) return 0;
     if (!q || !k_cache || !v_cache || !o || !row_pos || (prefixes && (!prefix_k || !prefix_v))) return ob_fail(ONEBIT_E_ARG, "attention_shared_rows: null pointer");
-    if (!ob_aligned(q, 16) || !ob_aligned(k_cache, 16) || !ob_aligned(v_cache, 16) || !ob_aligned(o, 4) || (h_next && !ob_aligned(h_next, 2)) ||
+    if (!ob_aligned(q, 16) || !ob_aligned(k_cache, 16) || !ob_aligned(v_cache, 16) || !ob_aligned(o, 8) || (h_next && !ob_aligned(h_next, 2)) ||
         (prefixes && (!ob_aligned(prefix_k, 16) || !ob_aligned(prefix_v, 16))))
         return ob_fail(ONEBIT_E_ALIGN, "attention_shared_rows: q and the caches must be 16-byte aligned");
     const size_t need = onebit_attention_shared_scratch_bytes(groups, n_groups, rows, n_heads, n_kv_heads, head_dim, max_own);
@@ -105,6 +120,7 @@ extern "C" int onebit_attention_shared_rows(const void *q, const void *prefix_k,
     a.o = (_Float16 *)o; a.h_next = (const _Float16 *)h_next; a.row_slot = row_slot; a.row_pos = row_pos;
     a.p_max_len = prefix_max_len; a.max_len = max_len; a.H = n_heads; a.Hkv = n_kv_heads; a.rep = (int)rep; a.D = head_dim; a.n_slots = (int)n_slots;
     a.pchunk = p.pchunk; a.ochunk = p.ochunk; a.psplits = p.psplits; a.osplits = p.osplits; a.own_mb = p.own_mb; a.max_own = (int)max_own;
+    a.inline_prefix = p.inline_prefix;
     a.scale_log2e = 1.4426950408889634f / sqrtf((float)head_dim);
     const size_t parts = (size_t)rows * n_heads * (p.psplits + p.osplits);
     a.part_o = (float *)scratch;
@@ -115,27 +131,20 @@ extern "C" int onebit_attention_shared_rows(const void *q, const void *prefix_k,
         int64_t items = 0;
         for (int i = 0; i < a.n_groups; ++i) {
             const onebit_prefix_t &g = groups[g0 + i];
-            const int64_t chunks = ob_up(g.len, p.pchunk);
-            items += chunks * ob_up(g.n * rep, 16 * p.mt);
+            const int64_t chunks = p.inline_prefix ? 0 : ob_up(g.len, p.pchunk);
+            items += chunks ? chunks * ob_up(g.n * rep, p.per) : 0;
             a.g[i] = {g.row0, g.n, g.slot, g.len, g.first, (int)chunks, (int)items};
             a.rows += g.n;
         }
-        a.own_item0 = (int)items;
-        items += (int64_t)a.rows * p.own_mb * p.osplits;
-        if (items * n_kv_heads > OB_MAX_WGS) return ob_fail(ONEBIT_E_ARG, "attention_shared_rows: too many workgroups");
+        const int64_t own_items = (int64_t)a.rows * p.own_mb * std::max(p.osplits, 1);
+        if (items * n_kv_heads > OB_MAX_WGS || own_items * n_kv_heads > OB_MAX_WGS) return ob_fail(ONEBIT_E_ARG, "attention_shared_rows: too many workgroups");
         hipStream_t s = (hipStream_t)stream;
-        if (items > 0) {
-            if (head_dim > 64) {
-                if (p.mt == 1) ob_sh_launch<128, 1>(a, items, s);
-                else if (p.mt == 2) ob_sh_launch<128, 2>(a, items, s);
-                else ob_sh_launch<128, 4>(a, items, s);
-            } else {
-                if (p.mt == 1) ob_sh_launch<64, 1>(a, items, s);
-                else if (p.mt == 2) ob_sh_launch<64, 2>(a, items, s);
-                else ob_sh_launch<64, 4>(a, items, s);
-            }
-        }
-        hipLaunchKernelGGL(ob_sh_join_kernel, dim3((unsigned)ob_up((int64_t)a.rows * n_heads, OB_SH_THREADS / 64)), dim3(OB_SH_THREADS), 0, s, a);
+        if (head_dim == 128) ob_sh_launch<128, true>(a, p.form, items, own_items, s);
+        else if (head_dim == 64) ob_sh_launch<64, true>(a, p.form, items, own_items, s);
+        else if (head_dim > 64) ob_sh_launch<128, false>(a, p.form, items, own_items, s);
+        else ob_sh_launch<64, false>(a, p.form, items, own_items, s);
+        if (p.osplits)
+            hipLaunchKernelGGL(ob_sh_join_kernel, dim3((unsigned)ob_up((int64_t)a.rows * n_heads, OB_SH_THREADS / 64)), dim3(OB_SH_THREADS), 0, s, a);
         const int rc2 = ob_launch_status("attention_shared_rows");
         if (rc2) return rc2;
     }
@@ -146,17 +155,28 @@ extern "C" int onebit_attention_shared_rows(const void *q, const void *prefix_k,
 static int ob_bs_check(int64_t groups, int32_t beams, int64_t vocab, int32_t keep)
 {
     if (groups < 0 || vocab < 1) return ob_fail(ONEBIT_E_ARG, "beam_select: bad size");
-    if (beams < 1 || beams > OB_RE_MAX_BEAMS || keep < 1 || keep > OB_BS_MAX_KEEP)
-        return ob_fail(ONEBIT_E_SHAPE, "beam_select: %d beams (1 .. %d), %d kept (1 .. %d)", beams, OB_RE_MAX_BEAMS, keep, OB_BS_MAX_KEEP);
+    if (beams < 1 || beams > OB_BS_MAX_BEAMS || keep < 1 || keep > OB_BS_MAX_KEEP)
+        return ob_fail(ONEBIT_E_SHAPE, "beam_select: %d beams (1 .. %d), %d kept (1 .. %d)", beams, OB_BS_MAX_BEAMS, keep, OB_BS_MAX_KEEP);
     if (vocab > (1 << 20) || groups > 65535 || groups * beams > 65535) return ob_fail(ONEBIT_E_ARG, "beam_select: dimension too large");
     return 0;
 }
 
+// pieces of 8 elements per thread, chunks of a row and pieces of a chunk (as even as they go)
+struct ObBsPlan { int nv, chunks, vecs; };
+static ObBsPlan ob_bs_plan(int64_t rows, int64_t vocab)
+{
+    const int64_t all = ob_up(vocab, 8);
+    ObBsPlan p;
+    p.nv = rows * ob_up(all, OB_BS_THREADS) > 2048 ? 4 : 1;
+    p.chunks = (int)ob_up(all, p.nv * OB_BS_THREADS);
+    p.vecs = (int)ob_up(all, p.chunks);
+    return p;
+}
+
 extern "C" size_t onebit_beam_select_scratch_bytes(int64_t rows, int64_t vocab, int32_t keep)
 {
-    if (rows <= 0 || vocab <= 0 || keep <= 0) return 0;
-    const size_t chunks = (size_t)ob_up(vocab, OB_BS_CHUNK);
-    return (size_t)rows * chunks * (16 + 4 * (size_t)keep * 8) + 256;
+    if (rows <= 0 || vocab <= 0 || keep <= 0 || rows > 65535 || vocab > (1 << 20) || keep > OB_BS_MAX_KEEP) return 0;
+    return (size_t)rows * ob_bs_plan(rows, vocab).chunks * (16 + 4 + 8 * (size_t)ob_bs_list(keep)) + 256;
 }
 
 extern "C" int onebit_beam_select(const void *logits, int64_t ld, int dtype, const float *scores, int64_t groups, int32_t beams, int64_t vocab, int32_t keep,
@@ -174,16 +194,24 @@ extern "C" int onebit_beam_select(const void *logits, int64_t ld, int dtype, con
     const size_t need = onebit_beam_select_scratch_bytes(rows, vocab, keep);
     if (!scratch || scratch_bytes < need || !ob_aligned(scratch, 16)) return ob_fail(ONEBIT_E_WSPACE, "beam_select: needs %zu bytes of 16-byte aligned scratch", need);
     ObBsArgs a = {};
-    a.logits = logits; a.ld = ld; a.scores = scores; a.beams = beams; a.keep = keep; a.vocab = (int)vocab; a.chunks = (int)ob_up(vocab, OB_BS_CHUNK);
+    const ObBsPlan p = ob_bs_plan(rows, vocab);
+    a.logits = logits; a.ld = ld; a.scores = scores; a.beams = beams; a.keep = keep; a.vocab = (int)vocab; a.chunks = p.chunks; a.vecs = p.vecs;
+    const size_t lists = (size_t)rows * p.chunks;
     a.sums = (double *)scratch;
-    a.list_x = (float *)(a.sums + (size_t)rows * a.chunks * 2);
-    a.list_t = (int *)(a.list_x + (size_t)rows * a.chunks * 4 * keep);
+    a.counts = (int *)(a.sums + 2 * lists);
+    a.list_x = (float *)(a.counts + lists);
+    a.list_t = (int *)(a.list_x + lists * ob_bs_list(keep));
     a.out_scores = out_scores; a.out_beams = out_beams; a.out_tokens = out_tokens;
     hipStream_t s = (hipStream_t)stream;
-    const dim3 grid((unsigned)a.chunks, (unsigned)rows);
-    if (dtype == ONEBIT_F16) hipLaunchKernelGGL((ob_bs_scan_kernel<_Float16>), grid, dim3(OB_BS_THREADS), 0, s, a);
-    else hipLaunchKernelGGL((ob_bs_scan_kernel<float>), grid, dim3(OB_BS_THREADS), 0, s, a);
-    hipLaunchKernelGGL(ob_bs_pick_kernel, dim3((unsigned)groups), dim3(OB_BS_THREADS), (size_t)4 * a.chunks * beams, s, a);
+    const dim3 grid((unsigned)a.chunks, (unsigned)rows), block(OB_BS_THREADS);
+    if (dtype == ONEBIT_F16) {
+        if (p.nv == 1) hipLaunchKernelGGL((ob_bs_scan_kernel<_Float16, 1>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((ob_bs_scan_kernel<_Float16, 4>), grid, block, 0, s, a);
+    } else {
+        if (p.nv == 1) hipLaunchKernelGGL((ob_bs_scan_kernel<float, 1>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((ob_bs_scan_kernel<float, 4>), grid, block, 0, s, a);
+    }
+    hipLaunchKernelGGL(ob_bs_pick_kernel, dim3((unsigned)groups), dim3(OB_BS_PICK), 0, s, a);
     return ob_launch_status("beam_select");
 }
 

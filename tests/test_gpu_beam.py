@@ -218,9 +218,9 @@ def test_one_workspace_for_calls_of_many_sizes_in_turn():
 
 
 def test_attention_python_refusals():
-    c = _case([70], [3], [5, 1, 20], 4, 4, 64)
+    c = _case([700], [3], [5, 1, 20], 4, 4, 64)
     bad = [dict(q=c["q"].float()), dict(q=c["q"][:, :, :32]), dict(k=c["k"].float()), dict(pk=None), dict(row_pos=c["row_pos"].long()), dict(row_pos=c["row_pos"][:2]),
-           dict(groups=[(0, 3, 5, 70, 0)]), dict(groups=[(0, 2, 0, 70, 0)]), dict(row_slot=c["row_slot"].cpu()), dict(v=c["v"][:, :2])]
+           dict(groups=[(0, 3, 5, 700, 0)]), dict(groups=[(0, 2, 0, 700, 0)]), dict(row_slot=c["row_slot"].cpu()), dict(v=c["v"][:, :2])]
     for b in bad:
         with pytest.raises(ValueError):
             _call({**c, **b})
