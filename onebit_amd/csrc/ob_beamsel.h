@@ -4,9 +4,9 @@
 // than fp32 resolves, while within a row the logits themselves order.
 //   ob_bs_scan_kernel   (row, chunk of the vocabulary): max and sum e^{x - max} of the chunk, and a list of candidates that holds its `keep` best
 //   ob_bs_pick_kernel   (group): the rows' sums joined, then the `keep` best of the lists
-// Both find the best by a threshold instead of one after the other: every wave takes the largest values of its lanes, as many as its share of
-// `keep`, the least of them over the waves is one that at least `keep` candidates reach, and few more do; those few are listed (the scan) or ranked by
-// counting (the pick).  Where too many reach it (rows of equal logits), the best are taken one after the other.
+// Both find the best by a threshold instead of one after the other: every wave publishes the largest of its lanes' largest values, its share of `keep` and
+// two more; at least `keep` candidates reach the keep-th of all published, and few more do; those are listed (the scan) or ranked by counting (the
+// pick).  Where too many reach it (rows of equal logits), the best are taken one after the other.
 // The logits are read once.  e^x: the product x log2 e is carried in two parts, so a term is off by 2^-23 at most however far x lies below the
 // maximum; terms are added in 64 bits.  A row's elements belong to threads by their index alone, not by the row's alignment: equal rows have equal
 // sums, bit for bit.
@@ -20,7 +20,7 @@
 #define OB_BS_RANKED 1024                          // candidates that the pick ranks by counting
 
 // room for the candidates of a chunk
-static inline __host__ __device__ int ob_bs_list(int keep) { return 2 * keep + 32; }
+static inline __host__ __device__ int ob_bs_list(int keep) { return keep + keep / 2 + 16; }
 
 struct ObBsArgs {
     const void *logits;
@@ -49,31 +49,38 @@ __device__ __forceinline__ double ob_bs_wave_sum(double v)
     return v;
 }
 
-// the k-th largest of the lanes' values (equal ones count one by one), -inf if there are fewer
-__device__ __forceinline__ float ob_bs_kth(float v, int k)
+// the k largest of the lanes' values (equal ones one by one; -inf where there are fewer), in order, to out
+__device__ __forceinline__ void ob_bs_publish(float v, int k, float *out)
 {
     const int lane = threadIdx.x & 63;
-    float w = INFINITY;
     for (int i = 0; i < k; ++i) {
-        w = ob_wave_max(v);
-        if (w == -INFINITY) break;
-        if (lane == __builtin_ctzll(__ballot(v == w))) v = -INFINITY;
+        const float w = ob_wave_max(v);
+        if (lane == 0) out[i] = w;
+        if (w > -INFINITY && lane == __builtin_ctzll(__ballot(v == w))) v = -INFINITY;
     }
-    return w;
+}
+// thread i < n: the i-th of the n published values is the keep-th largest (equal ones in their order)?
+__device__ __forceinline__ bool ob_bs_is_kth(const float *pub, int n, int keep, int i)
+{
+    if (i >= n) return false;
+    const float v = pub[i];
+    int rank = 0;
+    for (int k = 0; k < n; ++k) rank += pub[k] > v || (pub[k] == v && k < i);
+    return rank == keep - 1;
 }
 
 // NV: pieces of 8 elements of a thread, OB_BS_THREADS apart
 template <typename T, int NV>
 __global__ __launch_bounds__(OB_BS_THREADS) void ob_bs_scan_kernel(const ObBsArgs A)
 {
-    __shared__ float red_m[4], red_t[4];
+    __shared__ float red_m[4], pub[4 * (OB_BS_MAX_KEEP + 2)], t_s;
     __shared__ double red_s[4];
     __shared__ int n_s, red_i[4];
     const int chunk = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const T *x_row = (const T *)A.logits + (int64_t)row * A.ld;
     const int c0 = chunk * A.vecs * 8, c1 = min(A.vocab, c0 + A.vecs * 8);
     float x[NV][8];
-    if (tid == 0) n_s = 0;
+    if (tid == 0) { n_s = 0; t_s = -INFINITY; }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int t0 = c0 + 8 * (tid + OB_BS_THREADS * j);
@@ -93,13 +100,14 @@ __global__ __launch_bounds__(OB_BS_THREADS) void ob_bs_scan_kernel(const ObBsArg
     for (int j = 0; j < NV; ++j)
 #pragma unroll
         for (int e = 0; e < 8; ++e) best = fmaxf(best, x[j][e]);
-    // this wave's share of `keep`, by its lanes that have elements: enough over all waves together
-    const int n_thr = min((c1 - c0 + 7) / 8, OB_BS_THREADS), n_wave = max(0, min(64, n_thr - 64 * wave));
+    const int n_thr = min((c1 - c0 + 7) / 8, OB_BS_THREADS), share = min(64, (A.keep * min(64, n_thr) + n_thr - 1) / n_thr + 2);     // (of a wave all of whose lanes have elements)
     const float wm = ob_wave_max(best);
-    const float wt = n_thr < A.keep ? -INFINITY : n_wave ? ob_bs_kth(best, (A.keep * n_wave + n_thr - 1) / n_thr) : INFINITY;
-    if (lane == 0) { red_m[wave] = wm; red_t[wave] = wt; }
+    if (lane == 0) red_m[wave] = wm;
+    ob_bs_publish(best, share, pub + wave * share);
     __syncthreads();
-    const float m = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3])), t = fminf(fminf(red_t[0], red_t[1]), fminf(red_t[2], red_t[3]));
+    if (ob_bs_is_kth(pub, 4 * share, A.keep, tid)) t_s = pub[tid];
+    __syncthreads();
+    const float m = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3])), t = t_s;
     const int room = ob_bs_list(A.keep);
     const int64_t list = (int64_t)row * A.chunks + chunk;
     float *lx = A.list_x + list * room;
@@ -172,15 +180,35 @@ __device__ __forceinline__ bool ob_bs_before(const ObBsCand &a, const ObBsCand &
 
 __global__ __launch_bounds__(OB_BS_PICK) void ob_bs_pick_kernel(const ObBsArgs A)
 {
-    __shared__ double row_v[OB_BS_MAX_BEAMS];                                    // lse of a beam; NaN: it offers nothing
-    __shared__ float red_t[OB_BS_PICK / 64];
+    constexpr int WAVES = OB_BS_PICK / 64, NS = 8;                                // candidate places of a thread that stay in registers
+    __shared__ double row_v[OB_BS_MAX_BEAMS], cand_v[OB_BS_RANKED];               // lse of a beam; NaN: it offers nothing
+    __shared__ float pub[WAVES * (OB_BS_MAX_KEEP + 2)], t_s;
     __shared__ ObBsCand cand[OB_BS_RANKED];
     __shared__ int n_s;
     const int group = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int room = ob_bs_list(A.keep), per_beam = A.chunks * room, total = A.beams * per_beam;
+    const int room = ob_bs_list(A.keep), total = A.beams * A.chunks * room;
     const int64_t list0 = (int64_t)group * A.beams * A.chunks;
-    if (tid == 0) n_s = 0;
-    for (int b = wave; b < A.beams; b += OB_BS_PICK / 64) {
+    if (tid == 0) { n_s = 0; t_s = -INFINITY; }
+    struct Place { float x, score; int tok, n, beam, e; };
+    const auto fetch = [&](int i, Place &p) {                                    // (all of it at once: what lies behind a list's end is memory of the list, not used)
+        const int l = min(i, total - 1) / room;
+        p.e = i < total ? i - l * room : 0x7fffffff;
+        p.beam = l / A.chunks;
+        p.n = A.counts[list0 + l];
+        p.x = A.list_x[list0 * room + min(i, total - 1)];
+        p.tok = A.list_t[list0 * room + min(i, total - 1)];
+        p.score = A.scores[group * A.beams + p.beam];
+    };
+    const auto value = [&](const Place &p, ObBsCand &c) -> bool {                // false where there is no candidate
+        c = {(double)p.score + ((double)p.x - row_v[p.beam]), p.x, p.beam, p.tok};
+        return p.e < p.n && c.v > -INFINITY;                                     // (NaN: none)
+    };
+    Place place[NS];
+#pragma unroll
+    for (int k = 0; k < NS; ++k)
+        if (OB_BS_PICK * k < total) fetch(tid + OB_BS_PICK * k, place[k]);
+        else place[k] = {0.f, 0.f, 0, 0, 0, 0};
+    for (int b = wave; b < A.beams; b += WAVES) {
         const double *sm = A.sums + (list0 + (int64_t)b * A.chunks) * 2;
         double M = -INFINITY, s = 0.;
         for (int c = lane; c < A.chunks; c += 64) M = fmax(M, sm[2 * c]);
@@ -191,35 +219,33 @@ __global__ __launch_bounds__(OB_BS_PICK) void ob_bs_pick_kernel(const ObBsArgs A
         if (lane == 0) row_v[b] = M + log(s);
     }
     __syncthreads();
-    const auto at = [&](int i, ObBsCand &c) -> bool {                            // candidate place i: false where there is none
-        const int l = i / room;
-        if (i - l * room >= A.counts[list0 + l]) return false;
-        c.beam = l / A.chunks;
-        c.x = A.list_x[list0 * room + i];
-        c.tok = A.list_t[list0 * room + i];
-        c.v = (double)A.scores[group * A.beams + c.beam] + ((double)c.x - row_v[c.beam]);
-        return c.v > -INFINITY;                                                  // (NaN: none)
+    // f over all candidate places of this thread
+    const auto each = [&](auto f) {
+        ObBsCand c;
+#pragma unroll
+        for (int k = 0; k < NS; ++k)
+            if (value(place[k], c)) f(c);
+        for (int i = tid + OB_BS_PICK * NS; i < total; i += OB_BS_PICK) {
+            Place p;
+            fetch(i, p);
+            if (value(p, c)) f(c);
+        }
     };
     float best = -INFINITY;
-    for (int i = tid; i < total; i += OB_BS_PICK) {
-        ObBsCand c;
-        if (at(i, c)) best = fmaxf(best, __double2float_rd(c.v));                // (rounded down: what reaches the threshold reaches it in 64 bits, too)
-    }
-    const int waves = min(OB_BS_PICK / 64, (total + 63) / 64);                   // that have candidate places
-    const float wt = wave < waves ? ob_bs_kth(best, (A.keep + waves - 1) / waves) : INFINITY;
-    if (lane == 0) red_t[wave] = wt;
+    each([&](const ObBsCand &c) { best = fmaxf(best, __double2float_rd(c.v)); });      // (rounded down: what reaches the threshold reaches it in 64 bits, too)
+    const int waves = min(WAVES, (total + 63) / 64), share = min(64, (A.keep + waves - 1) / waves + 2);
+    if (wave < waves) ob_bs_publish(best, share, pub + wave * share);
     __syncthreads();
-    float t = red_t[0];
-#pragma unroll
-    for (int w = 1; w < OB_BS_PICK / 64; ++w) t = fminf(t, red_t[w]);
-    if (best >= t && best > -INFINITY)
-        for (int i = tid; i < total; i += OB_BS_PICK) {
-            ObBsCand c;
-            if (at(i, c) && c.v >= (double)t) {
+    if (ob_bs_is_kth(pub, waves * share, A.keep, tid)) t_s = pub[tid];
+    __syncthreads();
+    const double t = t_s;
+    if (best >= t_s)
+        each([&](const ObBsCand &c) {
+            if (c.v >= t) {
                 const int k = atomicAdd(&n_s, 1);
-                if (k < OB_BS_RANKED) cand[k] = c;
+                if (k < OB_BS_RANKED) { cand_v[k] = c.v; cand[k] = c; }
             }
-        }
+        });
     __syncthreads();
     int n = n_s;
     const int64_t out = (int64_t)group * A.keep;
@@ -228,17 +254,19 @@ __global__ __launch_bounds__(OB_BS_PICK) void ob_bs_pick_kernel(const ObBsArgs A
         if (tid < n) {
             const ObBsCand c = cand[tid];
             int rank = 0;
-            for (int k = 0; k < n; ++k) rank += ob_bs_before(cand[k], c);
+#pragma unroll 4
+            for (int k = 0; k < n; ++k) {
+                const double v = cand_v[k];
+                rank += v > c.v;
+                if (v == c.v && k != tid) rank += ob_bs_before(cand[k], c);
+            }
             if (rank < A.keep) put(rank, c);
         }
     } else {                                                                     // one after the other: the best behind the last one
         ObBsCand last = {INFINITY, INFINITY, -1, -1};
         for (n = 0; n < A.keep; ++n) {
             ObBsCand b = {-INFINITY, -INFINITY, 0x7fffffff, 0x7fffffff};
-            for (int i = tid; i < total; i += OB_BS_PICK) {
-                ObBsCand c;
-                if (at(i, c) && ob_bs_before(last, c) && ob_bs_before(c, b)) b = c;
-            }
+            each([&](const ObBsCand &c) { if (ob_bs_before(last, c) && ob_bs_before(c, b)) b = c; });
             __syncthreads();
             cand[tid] = b;
             __syncthreads();
