@@ -7,12 +7,12 @@ between calls of the same sizes; calls that may run at the same time need one ea
 from __future__ import annotations
 
 import ctypes
-from typing import List, Optional, Sequence, Tuple
+from typing import Optional, Sequence, Tuple
 
 import torch
 
 from . import _lib
-from .bitnet import _dtype_code, _require_gpu, _stream_ptr
+from .bitnet import _dtype_code, _raw_stream as _raw, _require_gpu, _stream_ptr
 
 MAX_BEAMS, MAX_KEEP = 32, 64
 
@@ -22,23 +22,47 @@ class _Prefix(ctypes.Structure):          # onebit_prefix_t
 
 
 def _prefixes(groups):
-    arr = (_Prefix * max(len(groups), 1))()
-    for a, g in zip(arr, groups):
-        if len(g) != 5:
-            raise ValueError(f"a group is (first row, rows, prefix slot, prefix length, first own position), not {tuple(g)!r}")
-        a.row0, a.n, a.slot, a.len, a.first = g
-    return arr
+    n = len(groups)
+    flat = [v for g in groups for v in g]
+    if len(flat) != 5 * n or any(len(g) != 5 for g in groups):
+        raise ValueError(f"groups are (first row, rows, prefix slot, prefix length, first own position) each, not {list(groups)!r}")
+    return (ctypes.c_int32 * (5 * n))(*flat)
 
 
-def _same_device(device, what: str, *tensors):
+def _call(name: str, index: int, *args):
+    """The library's function on the current stream of device ``index``."""
+    lib = _lib.load()
+    if index == torch.cuda.current_device():
+        rc = getattr(lib, name)(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = getattr(lib, name)(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc, name)
+
+
+def _raw_stream(index: int) -> int:
+    return _stream_ptr(torch.device("cuda", index)) if _raw is None else _raw(index)
+
+
+def _on(index: int, what: str, *tensors):
     for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"{what}: tensors on {device} and {t.device}")
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{what}: tensors on cuda:{index} and {t.device}")
 
 
-def _rows_int32(t: Optional[torch.Tensor], rows: int, what: str):
-    if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != rows or not t.is_contiguous()):
+def _rows_int32(t: torch.Tensor, rows: int, what: str):
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != rows or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous int32 tensor of {rows} entries")
+
+
+def _caches(what: str, name: str, kc: torch.Tensor, vc: torch.Tensor, kv_heads: int, dim: int):
+    shape = kc.shape
+    if len(shape) != 4 or vc.shape != shape or shape[3] != dim or shape[1] != kv_heads:
+        raise ValueError(f"{what}: {name} caches {tuple(shape)} / {tuple(vc.shape)} for {kv_heads} heads of {dim}")
+    if kc.dtype != torch.float16 or vc.dtype != torch.float16 or not kc.is_contiguous() or not vc.is_contiguous():
+        raise ValueError(f"{what}: the {name} caches must be contiguous float16")
+    return shape
 
 
 def shared_prefix_workspace(groups: Sequence[Tuple[int, int, int, int, int]], rows: int, heads: int, kv_heads: int, head_dim: int, max_own: int,
@@ -63,45 +87,43 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: Optional[torch.Tensor], p
     pairs may be the same tensors; without any prefix the first may be None.  ``row_slot`` / ``row_pos``: int32 on the device; a row whose slot
     or position lies outside is idle and keeps what ``out`` holds (zeros without ``out``).  ``max_own``: bound on the rows' own positions, those
     beyond it are not attended (None: all that fit the cache).  ``h_next`` [heads * D]: the result times this."""
-    _require_gpu(q, "shared_prefix_attention")
+    what = "shared_prefix_attention"
+    _require_gpu(q, what)
     if q.dim() != 3 or q.dtype != torch.float16 or not q.is_contiguous():
-        raise ValueError("shared_prefix_attention: q must be a contiguous float16 [rows, heads, D]")
+        raise ValueError(f"{what}: q must be a contiguous float16 [rows, heads, D]")
     rows, heads, dim = q.shape
-    if (prefix_k is None) != (prefix_v is None):
-        raise ValueError("shared_prefix_attention: prefix keys without values, or values without keys")
-    for name, kc, vc in (("prefix", prefix_k, prefix_v), ("own", k_cache, v_cache)):
-        if kc is None:
-            continue
-        if kc.dim() != 4 or kc.shape != vc.shape or kc.shape[3] != dim or kc.shape[1] != k_cache.shape[1]:
-            raise ValueError(f"shared_prefix_attention: {name} caches {tuple(kc.shape)} / {tuple(vc.shape)} for heads of {dim}")
-        if kc.dtype != q.dtype or vc.dtype != q.dtype or not kc.is_contiguous() or not vc.is_contiguous():
-            raise ValueError(f"shared_prefix_attention: the {name} caches must be contiguous float16")
-    _same_device(q.device, "shared_prefix_attention", prefix_k, prefix_v, k_cache, v_cache, row_slot, row_pos, h_next, out, workspace)
-    _rows_int32(row_slot, rows, "row_slot")
-    _rows_int32(row_pos, rows, "row_pos")
+    if k_cache.dim() != 4:
+        raise ValueError(f"{what}: own caches {tuple(k_cache.shape)} for heads of {dim}")
+    slots, kv_heads, max_len, _ = _caches(what, "own", k_cache, v_cache, k_cache.shape[1], dim)
+    p_slots = p_len = p_k = p_v = 0
+    if prefix_k is not None and prefix_v is not None:
+        p_slots, _, p_len, _ = _caches(what, "prefix", prefix_k, prefix_v, kv_heads, dim)
+        p_k, p_v = prefix_k.data_ptr(), prefix_v.data_ptr()
+    elif prefix_k is not None or prefix_v is not None:
+        raise ValueError(f"{what}: prefix keys without values, or values without keys")
     if row_pos is None:
-        raise ValueError("shared_prefix_attention: row_pos is needed")
-    if h_next is not None and (h_next.dtype != q.dtype or h_next.numel() != heads * dim or not h_next.is_contiguous()):
-        raise ValueError(f"shared_prefix_attention: h_next must be contiguous float16 of {heads * dim} entries")
+        raise ValueError(f"{what}: row_pos is needed")
+    _rows_int32(row_pos, rows, "row_pos")
+    if row_slot is not None:
+        _rows_int32(row_slot, rows, "row_slot")
+    if h_next is not None and (h_next.dtype != torch.float16 or h_next.numel() != heads * dim or not h_next.is_contiguous()):
+        raise ValueError(f"{what}: h_next must be contiguous float16 of {heads * dim} entries")
     if out is None:
         out = torch.zeros_like(q)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
-        raise ValueError("shared_prefix_attention: out must be like q")
-    kv_heads = k_cache.shape[1]
+    elif out.shape != q.shape or out.dtype != torch.float16 or not out.is_contiguous():
+        raise ValueError(f"{what}: out must be like q")
+    arr = _prefixes(groups)
     if max_own is None:
-        max_own = max([0] + [k_cache.shape[2] - int(g[4]) for g in groups if len(g) == 5])
+        max_own = max([0] + [max_len - int(g[4]) for g in groups])
     if workspace is None:
         workspace = shared_prefix_workspace(groups, rows, heads, kv_heads, dim, max_own, q.device)
     elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
-        raise ValueError("shared_prefix_attention: the workspace must be contiguous uint8")
-    p_slots, p_len = (0, 0) if prefix_k is None else (prefix_k.shape[0], prefix_k.shape[2])
-    with torch.cuda.device(q.device):
-        rc = _lib.load().onebit_attention_shared_rows(
-            q.data_ptr(), None if prefix_k is None else prefix_k.data_ptr(), None if prefix_v is None else prefix_v.data_ptr(), k_cache.data_ptr(),
-            v_cache.data_ptr(), out.data_ptr(), None if h_next is None else h_next.data_ptr(), _prefixes(groups), len(groups),
-            None if row_slot is None else row_slot.data_ptr(), row_pos.data_ptr(), rows, heads, kv_heads, dim, p_slots, p_len, k_cache.shape[0],
-            k_cache.shape[2], max_own, workspace.data_ptr(), workspace.numel(), _stream_ptr(q.device))
-    _lib.check(rc, "onebit_attention_shared_rows")
+        raise ValueError(f"{what}: the workspace must be contiguous uint8")
+    index = q.get_device()
+    _on(index, what, prefix_k, prefix_v, k_cache, v_cache, row_slot, row_pos, h_next, out, workspace)
+    _call("onebit_attention_shared_rows", index, q.data_ptr(), p_k, p_v, k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
+          None if h_next is None else h_next.data_ptr(), arr, len(groups), None if row_slot is None else row_slot.data_ptr(), row_pos.data_ptr(), rows, heads,
+          kv_heads, dim, p_slots, p_len, slots, max_len, max_own, workspace.data_ptr(), workspace.numel())
     return out
 
 
@@ -126,20 +148,21 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, keep: in
         raise ValueError(f"beam_select: {keep} kept (1 .. {MAX_KEEP})")
     if scores.dtype != torch.float32 or scores.numel() != rows or not scores.is_contiguous():
         raise ValueError(f"beam_select: scores must be contiguous float32 of {rows} entries")
-    _same_device(logits.device, "beam_select", scores, workspace)
     if workspace is None:
         workspace = beam_select_workspace(rows, vocab, keep, logits.device)
     elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
         raise ValueError("beam_select: the workspace must be contiguous uint8")
+    index = logits.get_device()
+    _on(index, "beam_select", scores, workspace)
     groups = rows // beams
-    packed = torch.empty(3, groups, keep, dtype=torch.int32, device=logits.device)
-    p = packed.data_ptr()
-    ld = logits.stride(0) if rows > 1 else max(logits.stride(0), vocab)
-    with torch.cuda.device(logits.device):
-        rc = _lib.load().onebit_beam_select(logits.data_ptr(), ld, _dtype_code(logits.dtype), scores.data_ptr(), groups, beams, vocab, keep, p,
-                                            p + 4 * groups * keep, p + 8 * groups * keep, workspace.data_ptr(), workspace.numel(), _stream_ptr(logits.device))
-    _lib.check(rc, "onebit_beam_select")
-    return packed[0].view(torch.float32), packed[1], packed[2]
+    packed = torch.empty((3, groups, keep), dtype=torch.int32, device=logits.device)
+    p, ld = packed.data_ptr(), logits.stride(0)
+    if rows == 1:
+        ld = max(ld, vocab)
+    _call("onebit_beam_select", index, logits.data_ptr(), ld, _dtype_code(logits.dtype), scores.data_ptr(), groups, beams, vocab, keep, p,
+          p + 4 * groups * keep, p + 8 * groups * keep, workspace.data_ptr(), workspace.numel())
+    values, beam, token = packed.unbind(0)
+    return values.view(torch.float32), beam, token
 
 
 def reorder_slots(buffers: Sequence[torch.Tensor], parents: torch.Tensor, slot0: int = 0, first: int = 0, count: Optional[int] = None) -> None:
@@ -156,33 +179,33 @@ def reorder_slots(buffers: Sequence[torch.Tensor], parents: torch.Tensor, slot0:
         raise ValueError("reorder_slots: first without count")
     if slot0 < 0 or first < 0 or (count is not None and count < 0):
         raise ValueError("reorder_slots: negative slot0, first or count")
+    index, slots = parents.get_device(), slot0 + groups * beams
     shapes: dict = {}
-    spans: List[Tuple[int, int]] = []
+    shape = dtype = into = None
     for t in buffers:
-        if not t.is_contiguous() or t.dim() < 1 or t.shape[0] < slot0 + groups * beams:
-            raise ValueError(f"reorder_slots: buffer {tuple(t.shape)} must be contiguous with {slot0 + groups * beams} slots")
-        if t.device != parents.device:
-            raise ValueError(f"reorder_slots: tensors on {parents.device} and {t.device}")
-        size = t.element_size()
-        slot = t.stride(0) * size if t.numel() else 0
-        if count is None:
-            geometry = (slot, 1, slot, 0, slot)
-        else:
-            if t.dim() != 4 or first + count > t.shape[2]:
-                raise ValueError(f"reorder_slots: positions {first} .. {first + count - 1} of a cache {tuple(t.shape)}")
-            row = t.shape[3] * size
-            geometry = (slot, t.shape[1], t.shape[2] * row, first * row, count * row)
-        if slot == 0 or groups == 0:
-            continue
-        p = t.data_ptr()
-        spans.append((p, p + t.shape[0] * slot))
-        shapes.setdefault(geometry, []).append(p + slot0 * slot)
-    spans.sort()
-    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        if not t.is_contiguous() or t.get_device() != index:
+            raise ValueError(f"reorder_slots: a buffer {tuple(t.shape)} on {t.device} must be contiguous and on {parents.device}")
+        if t.shape != shape or t.dtype != dtype:
+            shape, dtype = t.shape, t.dtype
+            if t.dim() < 1 or shape[0] < slots:
+                raise ValueError(f"reorder_slots: a buffer {tuple(shape)} must have {slots} slots")
+            size = t.element_size()
+            slot = t.stride(0) * size if t.numel() else 0
+            if count is None:
+                geometry = (slot, 1, slot, 0, slot)
+            elif len(shape) != 4 or first + count > shape[2]:
+                raise ValueError(f"reorder_slots: positions {first} .. {first + count - 1} of a cache {tuple(shape)}")
+            else:
+                row = shape[3] * size
+                geometry = (slot, shape[1], shape[2] * row, first * row, count * row)
+            into = shapes.setdefault((shape[0] * slot, geometry), [])
+        into.append(t.data_ptr())
+    if groups == 0:
+        return
+    ends = sorted((p, p + n) for (n, _), ptrs in shapes.items() if n for p in ptrs)
+    if any(a[1] > b[0] for a, b in zip(ends, ends[1:])):
         raise ValueError("reorder_slots: buffers overlap")
-    lib = _lib.load()
-    with torch.cuda.device(parents.device):
-        stream = _stream_ptr(parents.device)
-        for geometry, ptrs in shapes.items():
-            rc = lib.onebit_reorder_slots((ctypes.c_void_p * len(ptrs))(*ptrs), len(ptrs), parents.data_ptr(), groups, beams, *geometry, stream)
-            _lib.check(rc, "onebit_reorder_slots")
+    for (n, geometry), ptrs in shapes.items():
+        if n:
+            arr = (ctypes.c_void_p * len(ptrs))(*([p + slot0 * geometry[0] for p in ptrs] if slot0 else ptrs))
+            _call("onebit_reorder_slots", index, arr, len(ptrs), parents.data_ptr(), groups, beams, *geometry)

@@ -45,7 +45,7 @@ def test_attention_scratch_grows_with_its_parts():
     assert f([(0, 4, 0, 100000, 0)], 4, 20) > f([(0, 4, 0, 5000, 0)], 4, 20)
     with pytest.raises(ValueError, match="rows"):
         f([(0, 4, 0, 100, 0)], 5, 20)
-    with pytest.raises(ValueError, match="a group is"):
+    with pytest.raises(ValueError, match="groups are"):
         f([(0, 4, 0, 100)], 4, 20)
 
 
