@@ -521,6 +521,12 @@ typedef struct onebit_mixed_state {
 /* max_dec_rows = state->n_slots of the steps that will use the workspace (the attention scratch is laid out for that many rows). */
 size_t onebit_mixed_workspace_bytes(const onebit_model_t *model, int64_t max_rows, int32_t max_dec_rows, int32_t attn_chunk);
 int onebit_mixed_step(const onebit_model_t *model, const onebit_mixed_state_t *state, void *stream);
+/* The same step where the single-token rows share prefixes (onebit_attention_shared_rows, with the model's caches as both of its caches):
+ * `groups` tile rows 0 .. n_dec - 1; group g's rows attend to the first g.len positions of slot g.slot, and from position g.first on to their own
+ * slot.  attn_chunk / dec_ctx are not used.  scratch: onebit_attention_shared_scratch_bytes(groups, n_groups, n_dec, .., max_own). */
+struct onebit_prefix;
+int onebit_mixed_step_shared(const onebit_model_t *model, const onebit_mixed_state_t *state, const struct onebit_prefix *groups, int32_t n_groups,
+                             int64_t max_own, void *scratch, size_t scratch_bytes, void *stream);
 
 /* One fused decode GEMV launch (the building block of onebit_decode_step, exposed so that a
  * single kernel can be measured and tested in isolation): up to 3 projections sharing the input

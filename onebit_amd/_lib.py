@@ -57,6 +57,7 @@ SYMBOLS = {
                                                             ctypes.c_int32, _f, _vp, ctypes.c_size_t, _vp]),
     "onebit_mixed_workspace_bytes": (ctypes.c_size_t, [_vp, _i64, ctypes.c_int32, ctypes.c_int32]),
     "onebit_mixed_step": (_int, [_vp, _vp, _vp]),     # (onebit_model_t*, onebit_mixed_state_t*, stream)
+    "onebit_mixed_step_shared": (_int, [_vp, _vp, _vp, ctypes.c_int32, _i64, _vp, ctypes.c_size_t, _vp]),
     "onebit_attn_scratch_bytes": (ctypes.c_size_t, [_vp, _int]),
     "onebit_decode_stats_floats": (ctypes.c_size_t, [_vp]),
     "onebit_batch_stats_floats": (ctypes.c_size_t, [_vp, ctypes.c_int32]),

@@ -29,13 +29,16 @@ def main(argv=None) -> int:
     ap = argparse.ArgumentParser(prog="onebit_amd", description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     sub = ap.add_subparsers(dest="command", required=True)
     _trace_args(sub.add_parser("trace", help="replay a trace from standard input"))
-    g = sub.add_parser("generate", help="greedy generation")
+    g = sub.add_parser("generate", help="generation, greedy or by beam search")
     g.add_argument("--model", required=True)
     g.add_argument("--dtype", choices=["bfloat16", "float16", "float32"], help="default: the family's serving format")
     g.add_argument("--prompt", action="append", required=True, help="token ids, comma-separated; repeat for more requests")
     g.add_argument("--max-new-tokens", type=int, default=32)
     g.add_argument("--max-batch", type=int, default=32)
     g.add_argument("--prefill-chunk", type=int, help="prompt tokens of a request per step (default: whole prompts)")
+    g.add_argument("--num-beams", type=int, default=1, help="hypotheses per prompt of a beam search (default: greedy)")
+    g.add_argument("--length-penalty", type=float, default=1.0)
+    g.add_argument("--eos", type=int, action="append", help="end token of a beam search; repeat for more")
     a = ap.parse_args(argv)
     if a.command == "trace":
         from .trace import run
@@ -46,6 +49,13 @@ def main(argv=None) -> int:
     from .serving import ContinuousBatcher
     model = load_model(a.model, dtype=None if a.dtype is None else getattr(torch, a.dtype))
     prompts = [[int(t) for t in p.replace(",", " ").split()] for p in a.prompt]
+    if a.num_beams != 1:
+        from .registry import find_family
+        from .search import beam_rows
+        rows = beam_rows(model, prompts, a.max_new_tokens, find_family(a.model).max_positions(model), {}, a.num_beams, set(a.eos) if a.eos else None, a.length_penalty)
+        for i, row in enumerate(rows):
+            print(json.dumps({"request": i, "tokens": row}))
+        return 0
     cb = ContinuousBatcher(model, max_batch=min(a.max_batch, max(len(prompts), 2)), max_len=max(len(p) for p in prompts) + a.max_new_tokens,
                            prefill_chunk=a.prefill_chunk)
     ids = [cb.add_request(p, a.max_new_tokens) for p in prompts]

@@ -219,7 +219,10 @@ extern "C" size_t onebit_mixed_workspace_bytes(const onebit_model_t *m, int64_t 
     return ob_mixed_carve(m, max_rows, std::max<int32_t>(max_dec_rows, 1), OB_MIXED_MAX_SPLITS, nullptr).total;
 }
 
-extern "C" int onebit_mixed_step(const onebit_model_t *m, const onebit_mixed_state_t *st, void *stream)
+// the decode rows' groups of onebit_mixed_step_shared
+struct ObSharedRows { const onebit_prefix_t *groups; int32_t n_groups; int64_t max_own; void *scratch; size_t scratch_bytes; };
+
+static int ob_mixed_run(const onebit_model_t *m, const onebit_mixed_state_t *st, const ObSharedRows *shared, void *stream)
 {
     if (!m || !st) return ob_fail(ONEBIT_E_ARG, "mixed_step: null model/state");
     if (st->struct_size != sizeof(onebit_mixed_state_t))
@@ -246,7 +249,7 @@ extern "C" int onebit_mixed_step(const onebit_model_t *m, const onebit_mixed_sta
     if (r != T) return ob_fail(ONEBIT_E_SHAPE, "mixed_step: %d decode rows + the segments' rows = %lld, n_rows = %d", ND, (long long)r, T);
     const int chunk = st->attn_chunk > 0 ? st->attn_chunk : 256;
     int nsplit = ob_mixed_splits(m, chunk, st->dec_ctx);
-    if (nsplit > OB_MIXED_MAX_SPLITS) return ob_fail(ONEBIT_E_SHAPE, "mixed_step: %d attention splits (attn_chunk %d too small for this context)", nsplit, chunk);
+    if (!shared && nsplit > OB_MIXED_MAX_SPLITS) return ob_fail(ONEBIT_E_SHAPE, "mixed_step: %d attention splits (attn_chunk %d too small for this context)", nsplit, chunk);
     if (!ob_aligned(st->workspace, 256)) return ob_fail(ONEBIT_E_ALIGN, "mixed_step: workspace must be 256-byte aligned");
     const ObMixedWs w = ob_mixed_carve(m, T, st->n_slots, nsplit, st->workspace);
     if (st->workspace_bytes < w.total) return ob_fail(ONEBIT_E_WSPACE, "mixed_step: workspace %zu < %zu bytes", st->workspace_bytes, w.total);
@@ -375,7 +378,12 @@ extern "C" int onebit_mixed_step(const onebit_model_t *m, const onebit_mixed_sta
         if (NS > 0 && (rc = onebit_attention_ragged(w.q, L.k_cache, L.v_cache, w.attn, h_o, st->segs, NS, m->n_heads, m->n_kv_heads, D,
                                                     st->n_slots, m->max_len, s)))
             return rc;
-        if (ND > 0 && (rc = ob_fdec_launch(w.q, L.k_cache, L.v_cache, w.attn, h_o, st->row_slot, st->row_pos, ND, st->n_slots /* scratch rows */,
+        if (ND > 0 && shared) {
+            if ((rc = onebit_attention_shared_rows(w.q, L.k_cache, L.v_cache, L.k_cache, L.v_cache, w.attn, h_o, shared->groups, shared->n_groups, st->row_slot,
+                                                   st->row_pos, ND, m->n_heads, m->n_kv_heads, D, st->n_slots, m->max_len, st->n_slots, m->max_len,
+                                                   shared->max_own, shared->scratch, shared->scratch_bytes, s)))
+                return rc;
+        } else if (ND > 0 && (rc = ob_fdec_launch(w.q, L.k_cache, L.v_cache, w.attn, h_o, st->row_slot, st->row_pos, ND, st->n_slots /* scratch rows */,
                                            m->n_heads, m->n_kv_heads, D, st->n_slots, m->max_len, chunk, nsplit, w.attn_scratch, s)))
             return rc;
         // 5. o_proj
@@ -425,4 +433,24 @@ extern "C" int onebit_mixed_step(const onebit_model_t *m, const onebit_mixed_sta
         if ((rc = ob_lm_head_argmax(w.xh, m->lm_head, lg, st->part_val, st->part_idx, st->next_tokens + o0, no, H, m->vocab, s))) return rc;
     }
     return 0;
+}
+
+extern "C" int onebit_mixed_step(const onebit_model_t *m, const onebit_mixed_state_t *st, void *stream) { return ob_mixed_run(m, st, nullptr, stream); }
+
+extern "C" int onebit_mixed_step_shared(const onebit_model_t *m, const onebit_mixed_state_t *st, const onebit_prefix_t *groups, int32_t n_groups, int64_t max_own,
+                                        void *scratch, size_t scratch_bytes, void *stream)
+{
+    const ObSharedRows shared = {groups, n_groups, max_own, scratch, scratch_bytes};
+    if (m && st && st->struct_size == sizeof(onebit_mixed_state_t) && m->n_heads > 0 && m->n_kv_heads > 0) {
+        // (what the layers' calls would refuse is refused here, before the first launch)
+        const size_t need = onebit_attention_shared_scratch_bytes(groups, n_groups, st->n_dec, m->n_heads, m->n_kv_heads, m->head_dim, max_own);
+        if (st->n_dec > 0 && need == 0) return ONEBIT_E_SHAPE;
+        if (st->n_dec > 0 && (!scratch || scratch_bytes < need || !ob_aligned(scratch, 16)))
+            return ob_fail(ONEBIT_E_WSPACE, "mixed_step_shared: needs %zu bytes of 16-byte aligned scratch", need);
+        for (int i = 0; i < n_groups && st->n_dec > 0; ++i)
+            if (groups[i].len > 0 && (groups[i].slot < 0 || groups[i].slot >= st->n_slots || groups[i].len > m->max_len))
+                return ob_fail(ONEBIT_E_SHAPE, "mixed_step_shared: group %d's prefix (slot %d, %d positions) outside %d slots x %d positions", i, groups[i].slot,
+                               groups[i].len, st->n_slots, m->max_len);
+    }
+    return ob_mixed_run(m, st, &shared, stream);
 }

@@ -672,6 +672,7 @@ class MixedStep:
         self.lib.onebit_mixed_step.argtypes = [ctypes.POINTER(_Model), ctypes.POINTER(_MixedState), _vp]
         self._rows = 0
         self._stage = ItemStage(dev, self.n_slots, self.max_len, cfg.vocab_size)
+        self._shared_ws = None
         self._ensure(int(max_rows))
         self.launches = 0
 
@@ -696,13 +697,15 @@ class MixedStep:
             self.logits = torch.zeros(max(n, self.n_slots), self.cfg.vocab_size, dtype=torch.float16, device=self.dev)
 
     @torch.no_grad()
-    def launch(self, items) -> torch.Tensor:
+    def launch(self, items, prefixes=None) -> torch.Tensor:
         """Enqueue one step on the current stream.  ``items``: ``(slot, start, tokens)`` per scheduled request (distinct slots):
         ``tokens`` enter the request's cache slot at positions ``start ...``.  Returns the device tensor of greedy next tokens,
         one per item in the order given (the token after the item's LAST row: for a prompt chunk that is not the prompt's last one
         the caller ignores it).  An item may carry a fourth element ``k`` (default 1): lm_head runs on its last ``k`` rows (the
         evaluation caller scores a request's continuation rows) and the item contributes ``k`` consecutive entries to the returned
-        tokens and to ``logits``; or the list of the item's rows that lm_head runs on.  Asynchronous: synchronise before reading."""
+        tokens and to ``logits``; or the list of the item's rows that lm_head runs on.  Asynchronous: synchronise before reading.
+        ``prefixes``: ``(items, slot, length)`` for every run of single-token items, in their order: the first ``length`` positions of these items are those
+        of ``slot``, read there once for all of them, and only what follows lies in their own slots (``onebit_mixed_step_shared``)."""
         self._ensure(sum(len(it[2]) for it in items))
         self._ensure_logits(sum((len(it[3]) if isinstance(it[3], (list, tuple)) else int(it[3])) if len(it) > 3 else 1 for it in items))
         g = self._stage.stage(items)
@@ -712,7 +715,32 @@ class MixedStep:
                             None if self.logits is None else self.logits.data_ptr(), self._part_val.data_ptr(), self._part_idx.data_ptr(),
                             self._ws.data_ptr() + self._ws_off, self._ws.numel() - self._ws_off)
         with torch.cuda.device(self.dev):
-            rc = self.lib.onebit_mixed_step(ctypes.byref(self._model), ctypes.byref(state), torch.cuda.current_stream(self.dev).cuda_stream)
+            stream = torch.cuda.current_stream(self.dev).cuda_stream
+            if prefixes is None:
+                rc = self.lib.onebit_mixed_step(ctypes.byref(self._model), ctypes.byref(state), stream)
+            else:
+                rc = self._launch_shared(state, items, prefixes, stream)
         _lib.check(rc, "onebit_mixed_step")
         self.launches += 1
         return self.next_tokens[:g.n_out]
+
+    def _launch_shared(self, state, items, prefixes, stream) -> int:
+        from .beam import _prefixes, shared_prefix_workspace
+        starts = [it[1] for it in items if len(it[2]) == 1]
+        groups, row, most = [], 0, 0
+        for n, slot, length in prefixes:
+            if n < 1 or row + n > len(starts) or not 0 <= slot < self.n_slots or not 0 <= length <= self.max_len:
+                raise ValueError(f"step: a prefix of {length} positions in slot {slot} for {n} items")
+            if min(starts[row:row + n]) < length:
+                raise ValueError(f"step: an item starts at {min(starts[row:row + n])}, inside its prefix of {length} positions")
+            groups.append((row, n, slot, length, length))
+            most = max(most, max(starts[row:row + n]) + 1 - length)
+            row += n
+        if row != len(starts):
+            raise ValueError(f"step: prefixes for {row} of {len(starts)} single-token items")
+        c = self.cfg
+        nb = shared_prefix_workspace(groups, row, c.num_attention_heads, c.num_key_value_heads, c.head_dim, most, "meta").numel()
+        if self._shared_ws is None or self._shared_ws.numel() < nb:
+            self._shared_ws = torch.empty(2 * nb, dtype=torch.uint8, device=self.dev)
+        return self.lib.onebit_mixed_step_shared(ctypes.byref(self._model), ctypes.byref(state), _prefixes(groups), len(groups), most,
+                                                 self._shared_ws.data_ptr(), self._shared_ws.numel(), stream)

@@ -477,8 +477,13 @@ class HybridDecoder:
     __call__ = forward
 
     @torch.no_grad()
-    def generate(self, input_ids: torch.Tensor, max_new_tokens: int, eos_token_id=None, pad_token_id=None) -> torch.Tensor:
-        """Greedy search as ``OneBitLlamaForCausalLM.generate`` (same arguments and result), one batcher slot per row."""
+    def generate(self, input_ids: torch.Tensor, max_new_tokens: int, eos_token_id=None, pad_token_id=None, num_beams: int = 1,
+                 length_penalty: float = 1.0, early_stopping: bool = False) -> torch.Tensor:
+        """Greedy search as ``OneBitLlamaForCausalLM.generate`` (same arguments and result), one batcher slot per row.  ``num_beams`` > 1: beam search
+        (``search.beam_search``), the best hypothesis of every row."""
+        if num_beams != 1:
+            from .search import generate_beams
+            return generate_beams(self, input_ids, max_new_tokens, eos_token_id, pad_token_id, num_beams, length_penalty, early_stopping, self._engines)
         from .serving import generate_batched
         return generate_batched(self, input_ids, max_new_tokens, eos_token_id, pad_token_id, self._engines)
 

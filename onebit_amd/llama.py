@@ -467,13 +467,15 @@ class OneBitLlamaForCausalLM(nn.Module):
         return torch.cat(out, dim=1)
 
 
-def _generate_native(self, input_ids: torch.Tensor, max_new_tokens: int, eos_token_id=None, pad_token_id=None) -> torch.Tensor:
+def _generate_native(self, input_ids: torch.Tensor, max_new_tokens: int, eos_token_id=None, pad_token_id=None, num_beams: int = 1,
+                     length_penalty: float = 1.0, early_stopping: bool = False) -> torch.Tensor:
     """``generate`` on the native engines, same return contract: B = 1 -> ``DecodeEngine`` (the prompt through ``onebit_mixed_step``,
     every further token one HIP-graph replay of ``onebit_decode_step``); B > 1 -> ``ContinuousBatcher`` with one slot per row (the
     prompts enter in ONE mixed step, decode-only steps replay the batched step's graph).  The steps are enqueued without looking at
     the tokens; EOS is applied afterwards exactly as ``generate`` applies it (a finished row continues with ``pad_token_id``, the
     output ends where every row is finished: generation/utils.py:2543-2570).  Engines are kept per (batch, max_len) on the model.
-    Greedy tokens equal ``generate``'s up to fp16 near-ties of the logits (the engines' kernels sum in another order)."""
+    Greedy tokens equal ``generate``'s up to fp16 near-ties of the logits (the engines' kernels sum in another order).
+    ``num_beams`` > 1: beam search (``search.beam_search``), the best hypothesis of every row."""
     from .engine import DecodeEngine
     from .serving import batched_rows, cut_at_eos, eos_set
     if input_ids.dim() != 2:
@@ -484,7 +486,10 @@ def _generate_native(self, input_ids: torch.Tensor, max_new_tokens: int, eos_tok
     eos, pad_token_id = eos_set(eos_token_id, pad_token_id, B)
     dev, limit = self.lm_head.weight.device, self.config.max_position_embeddings
     engines = self.__dict__.setdefault("_native_engines", {})
-    if B == 1:
+    if num_beams != 1:
+        from .search import beam_rows
+        rows = beam_rows(self, input_ids.tolist(), max_new_tokens, limit, engines, num_beams, eos, length_penalty, early_stopping)
+    elif B == 1:
         if S + max_new_tokens > limit:
             raise ValueError("prompt + max_new_tokens exceeds max_position_embeddings")
         key = (B, min(-(-(S + max_new_tokens) // 256) * 256, limit))

@@ -91,3 +91,59 @@ def test_python_checks_name_the_mistake():
         reorder_slots([c], torch.zeros(1, 2, dtype=torch.int32))
     with pytest.raises(ValueError, match="parents"):
         reorder_slots([c], torch.zeros(1, 2))
+
+
+def test_shared_step_refuses(buf):
+    from onebit_amd.engine import _Layer, _MixedState, _Model
+    a, _ = buf
+    lib = _lib.load()
+    m = _Model(1, 128, 352, 2, 2, 64, 96, 32, 1e-6, 1e-5, (_Layer * 1)(), a, a, a, a, a)
+    st = _MixedState(ctypes.sizeof(_MixedState), 2, 2, 0, 1, 4, 0, 0, a, a, a, None, a, a, None, a, a, a, 1 << 30)
+
+    def call(groups, own=8, ws=a, nb=1 << 20):
+        arr = (_Prefix * max(len(groups), 1))(*[_Prefix(*g) for g in groups])
+        return lib.onebit_mixed_step_shared(ctypes.byref(m), ctypes.byref(st), arr, len(groups), own, ws, nb, None)
+    assert call([(0, 2, 4, 10, 10)]) == E_SHAPE and b"prefix" in lib.onebit_last_error()           # slot 4 of 4
+    assert call([(0, 2, 0, 33, 33)]) == E_SHAPE and call([(0, 1, 0, 10, 10)]) == E_SHAPE and call([]) == E_SHAPE
+    assert call([(0, 2, 0, 10, 10)], ws=None) == E_WSPACE and call([(0, 2, 0, 10, 10)], nb=1) == E_WSPACE
+    assert lib.onebit_mixed_step_shared(None, ctypes.byref(st), None, 0, 0, None, 0, None) == E_ARG
+    st.struct_size = 8
+    assert call([(0, 2, 0, 10, 10)]) == E_ARG and b"struct_size" in lib.onebit_last_error()
+
+
+class _Slots:
+    """A search's bookkeeping alone: candidates in, slots out."""
+
+    def __init__(self, beams, penalty=1.0, early=False):
+        from onebit_amd.search import _Prompt
+        self.p = _Prompt(beams, penalty, early)
+
+
+def test_hypotheses_keep_their_slots():
+    p = _Slots(3).p
+    p.take([(-1.0, 0, 5), (-2.0, 0, 6), (-3.0, 0, 7), (-4.0, 0, 8)], None)
+    assert [(t, s) for _, t, s in p.live] == [([5], 0), ([6], 1), ([7], 2)]
+    # the second goes on twice, the first not at all: its slot takes the second's state
+    assert p.take([(-2.5, 1, 1), (-3.5, 2, 2), (-3.6, 1, 3)], None) == [1, 1, 2]
+    assert [(t, s) for _, t, s in p.live] == [([6, 1], 1), ([7, 2], 2), ([6, 3], 0)]
+    # a beam is a rank, not a slot
+    assert p.take([(-4.0, 2, 0), (-4.1, 2, 1), (-4.2, 2, 2)], None) == [0, 0, 0]
+    assert [s for _, _, s in p.live] == [0, 1, 2]
+
+
+def test_finished_hypotheses():
+    p = _Slots(2).p
+    p.take([(-1.0, 0, 9), (-1.5, 0, 4), (-1.6, 0, 5), (-9.0, 0, 6)], {9})
+    assert p.finished == [(-1.0, [9])] and [t for _, t, _ in p.live] == [[4], [5]] and not p.done
+    p.take([(-1.7, 1, 4), (-1.8, 0, 4), (-1.9, 0, 9)], {9})
+    assert len(p.finished) == 1                                        # an end behind all that could go on is none
+    p.take([(-2.0, 0, 9), (-2.1, 1, 4), (-2.2, 1, 5)], {9})
+    assert [t for _, t in p.finished] == [[5, 4, 9], [9]] and not p.done       # -2/3, -1; live ones at -0.7
+    p.take([(-7.0, 0, 4), (-7.5, 1, 5)], {9})
+    assert p.done and p.results() == p.finished
+    early = _Slots(1, early=True).p
+    early.take([(-5.0, 0, 9), (-5.1, 0, 4)], {9})
+    assert early.done
+    empty = _Slots(2).p
+    empty.take([(float("-inf"), -1, -1)] * 4, None)
+    assert empty.done and empty.results() == []
