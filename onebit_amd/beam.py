@@ -21,18 +21,24 @@ class _Prefix(ctypes.Structure):          # onebit_prefix_t
     _fields_ = [("row0", ctypes.c_int32), ("n", ctypes.c_int32), ("slot", ctypes.c_int32), ("len", ctypes.c_int32), ("first", ctypes.c_int32)]
 
 
+_ARRAYS: dict = {}          # ctypes array types by length
+
+
 def _prefixes(groups):
-    n = len(groups)
-    flat = [v for g in groups for v in g]
-    if len(flat) != 5 * n or any(len(g) != 5 for g in groups):
+    flat = groups[0] if len(groups) == 1 else [v for g in groups for v in g]
+    n = len(flat)
+    if n != 5 * len(groups) or any(len(g) != 5 for g in groups):
         raise ValueError(f"groups are (first row, rows, prefix slot, prefix length, first own position) each, not {list(groups)!r}")
-    return (ctypes.c_int32 * (5 * n))(*flat)
+    t = _ARRAYS.get(n)
+    if t is None:
+        t = _ARRAYS[n] = ctypes.c_int32 * n
+    return t(*flat)
 
 
 def _call(name: str, index: int, *args):
     """The library's function on the current stream of device ``index``."""
-    lib = _lib.load()
-    if index == torch.cuda.current_device():
+    lib = _lib._lib or _lib.load()
+    if index == _get_device():
         rc = getattr(lib, name)(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -41,8 +47,9 @@ def _call(name: str, index: int, *args):
         _lib.check(rc, name)
 
 
-def _raw_stream(index: int) -> int:
-    return _stream_ptr(torch.device("cuda", index)) if _raw is None else _raw(index)
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = _raw if _raw is not None else lambda index: _stream_ptr(torch.device("cuda", index))
+_F16, _F32, _I32, _U8 = torch.float16, torch.float32, torch.int32, torch.uint8
 
 
 def _on(index: int, what: str, *tensors):
@@ -51,28 +58,21 @@ def _on(index: int, what: str, *tensors):
             raise ValueError(f"{what}: tensors on cuda:{index} and {t.device}")
 
 
-def _rows_int32(t: torch.Tensor, rows: int, what: str):
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != rows or not t.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous int32 tensor of {rows} entries")
-
-
-def _caches(what: str, name: str, kc: torch.Tensor, vc: torch.Tensor, kv_heads: int, dim: int):
-    shape = kc.shape
-    if len(shape) != 4 or vc.shape != shape or shape[3] != dim or shape[1] != kv_heads:
-        raise ValueError(f"{what}: {name} caches {tuple(shape)} / {tuple(vc.shape)} for {kv_heads} heads of {dim}")
-    if kc.dtype != torch.float16 or vc.dtype != torch.float16 or not kc.is_contiguous() or not vc.is_contiguous():
-        raise ValueError(f"{what}: the {name} caches must be contiguous float16")
-    return shape
+def _check_rows(what: str, rows: int, **tensors):
+    for name, t in tensors.items():
+        if t is not None and not (t.dtype is _I32 and t.shape == (rows,) and t.is_contiguous()):
+            raise ValueError(f"{what}: {name} must be a contiguous int32 tensor of {rows} entries")
 
 
 def shared_prefix_workspace(groups: Sequence[Tuple[int, int, int, int, int]], rows: int, heads: int, kv_heads: int, head_dim: int, max_own: int,
                             device="cuda") -> torch.Tensor:
-    """Scratch memory for ``shared_prefix_attention`` calls of these groups and sizes."""
+    """Scratch memory for ``shared_prefix_attention`` calls of these groups and sizes, and of any that need no more: zero-filled once, every call leaves
+    its counters at zero."""
     lib = _lib.load()
     n = lib.onebit_attention_shared_scratch_bytes(_prefixes(groups), len(groups), rows, heads, kv_heads, head_dim, max_own)
     if rows > 0 and n == 0:
         raise ValueError(f"shared_prefix_workspace: {lib.onebit_last_error().decode('utf-8', 'replace')}")
-    return torch.empty(max(int(n), 1), dtype=torch.uint8, device=device)
+    return torch.zeros(max(int(n), 1), dtype=torch.uint8, device=device)
 
 
 def shared_prefix_attention(q: torch.Tensor, prefix_k: Optional[torch.Tensor], prefix_v: Optional[torch.Tensor], k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -89,41 +89,51 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: Optional[torch.Tensor], p
     beyond it are not attended (None: all that fit the cache).  ``h_next`` [heads * D]: the result times this."""
     what = "shared_prefix_attention"
     _require_gpu(q, what)
-    if q.dim() != 3 or q.dtype != torch.float16 or not q.is_contiguous():
+    shape = q.shape
+    if len(shape) != 3 or q.dtype is not _F16 or not q.is_contiguous():
         raise ValueError(f"{what}: q must be a contiguous float16 [rows, heads, D]")
-    rows, heads, dim = q.shape
-    if k_cache.dim() != 4:
-        raise ValueError(f"{what}: own caches {tuple(k_cache.shape)} for heads of {dim}")
-    slots, kv_heads, max_len, _ = _caches(what, "own", k_cache, v_cache, k_cache.shape[1], dim)
+    rows, heads, dim = shape
+    own = k_cache.shape
+    if not (len(own) == 4 and own[3] == dim and v_cache.shape == own and k_cache.dtype is _F16 and v_cache.dtype is _F16 and k_cache.is_contiguous() and
+            v_cache.is_contiguous()):
+        raise ValueError(f"{what}: own caches must be contiguous float16 [slots, kv heads, positions, {dim}], not {tuple(own)} / {tuple(v_cache.shape)}")
+    slots, kv_heads, max_len, _ = own
+    index = q.get_device()
     p_slots = p_len = p_k = p_v = 0
     if prefix_k is not None and prefix_v is not None:
-        p_slots, _, p_len, _ = _caches(what, "prefix", prefix_k, prefix_v, kv_heads, dim)
+        pre = prefix_k.shape
+        if not (len(pre) == 4 and pre[3] == dim and pre[1] == kv_heads and prefix_v.shape == pre and prefix_k.dtype is _F16 and prefix_v.dtype is _F16 and
+                prefix_k.is_contiguous() and prefix_v.is_contiguous() and prefix_k.get_device() == index and prefix_v.get_device() == index):
+            raise ValueError(f"{what}: prefix caches must be contiguous float16 [slots, {kv_heads}, positions, {dim}] on {q.device}, not {tuple(pre)} / "
+                             f"{tuple(prefix_v.shape)} on {prefix_k.device}")
+        p_slots, _, p_len, _ = pre
         p_k, p_v = prefix_k.data_ptr(), prefix_v.data_ptr()
     elif prefix_k is not None or prefix_v is not None:
         raise ValueError(f"{what}: prefix keys without values, or values without keys")
     if row_pos is None:
         raise ValueError(f"{what}: row_pos is needed")
-    _rows_int32(row_pos, rows, "row_pos")
-    if row_slot is not None:
-        _rows_int32(row_slot, rows, "row_slot")
-    if h_next is not None and (h_next.dtype != torch.float16 or h_next.numel() != heads * dim or not h_next.is_contiguous()):
-        raise ValueError(f"{what}: h_next must be contiguous float16 of {heads * dim} entries")
+    if not (row_pos.dtype is _I32 and row_pos.shape == (rows,) and row_pos.is_contiguous()) or row_slot is not None:
+        _check_rows(what, rows, row_pos=row_pos, row_slot=row_slot)
+    scale = None
+    if h_next is not None:
+        if h_next.dtype is not _F16 or h_next.numel() != heads * dim or not h_next.is_contiguous():
+            raise ValueError(f"{what}: h_next must be contiguous float16 of {heads * dim} entries")
+        scale = h_next.data_ptr()
     if out is None:
         out = torch.zeros_like(q)
-    elif out.shape != q.shape or out.dtype != torch.float16 or not out.is_contiguous():
+    elif out.shape != shape or out.dtype is not _F16 or not out.is_contiguous():
         raise ValueError(f"{what}: out must be like q")
     arr = _prefixes(groups)
     if max_own is None:
         max_own = max([0] + [max_len - int(g[4]) for g in groups])
     if workspace is None:
         workspace = shared_prefix_workspace(groups, rows, heads, kv_heads, dim, max_own, q.device)
-    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+    elif workspace.dtype is not _U8 or not workspace.is_contiguous():
         raise ValueError(f"{what}: the workspace must be contiguous uint8")
-    index = q.get_device()
-    _on(index, what, prefix_k, prefix_v, k_cache, v_cache, row_slot, row_pos, h_next, out, workspace)
-    _call("onebit_attention_shared_rows", index, q.data_ptr(), p_k, p_v, k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
-          None if h_next is None else h_next.data_ptr(), arr, len(groups), None if row_slot is None else row_slot.data_ptr(), row_pos.data_ptr(), rows, heads,
-          kv_heads, dim, p_slots, p_len, slots, max_len, max_own, workspace.data_ptr(), workspace.numel())
+    _on(index, what, k_cache, v_cache, row_slot, row_pos, h_next, out, workspace)
+    _call("onebit_attention_shared_rows", index, q.data_ptr(), p_k, p_v, k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), scale, arr, len(groups),
+          None if row_slot is None else row_slot.data_ptr(), row_pos.data_ptr(), rows, heads, kv_heads, dim, p_slots, p_len, slots, max_len, max_own,
+          workspace.data_ptr(), workspace.numel())
     return out
 
 
@@ -139,37 +149,38 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, keep: in
     tokens (int32), [groups, keep] each, best first: views of one int32 tensor [3, groups, keep].  Values are ranked in 64 bits; equal ones by beam, logit,
     token.  A continuation of probability zero is none: places that remain hold -inf, -1, -1."""
     _require_gpu(logits, "beam_select")
-    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    shape = logits.shape
+    if len(shape) != 2 or (shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("beam_select: logits must be [rows, vocab] with adjacent columns")
-    rows, vocab = logits.shape
+    rows, vocab = shape
     if not 1 <= beams <= MAX_BEAMS or rows % beams:
         raise ValueError(f"beam_select: {rows} rows in groups of {beams} hypotheses (1 .. {MAX_BEAMS})")
     if not 1 <= keep <= MAX_KEEP:
         raise ValueError(f"beam_select: {keep} kept (1 .. {MAX_KEEP})")
-    if scores.dtype != torch.float32 or scores.numel() != rows or not scores.is_contiguous():
+    if scores.dtype is not _F32 or scores.numel() != rows or not scores.is_contiguous():
         raise ValueError(f"beam_select: scores must be contiguous float32 of {rows} entries")
     if workspace is None:
         workspace = beam_select_workspace(rows, vocab, keep, logits.device)
-    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+    elif workspace.dtype is not _U8 or not workspace.is_contiguous():
         raise ValueError("beam_select: the workspace must be contiguous uint8")
     index = logits.get_device()
     _on(index, "beam_select", scores, workspace)
     groups = rows // beams
-    packed = torch.empty((3, groups, keep), dtype=torch.int32, device=logits.device)
+    packed = torch.empty((3, groups, keep), dtype=_I32, device=logits.device)
     p, ld = packed.data_ptr(), logits.stride(0)
     if rows == 1:
         ld = max(ld, vocab)
     _call("onebit_beam_select", index, logits.data_ptr(), ld, _dtype_code(logits.dtype), scores.data_ptr(), groups, beams, vocab, keep, p,
           p + 4 * groups * keep, p + 8 * groups * keep, workspace.data_ptr(), workspace.numel())
     values, beam, token = packed.unbind(0)
-    return values.view(torch.float32), beam, token
+    return values.view(_F32), beam, token
 
 
 def reorder_slots(buffers: Sequence[torch.Tensor], parents: torch.Tensor, slot0: int = 0, first: int = 0, count: Optional[int] = None) -> None:
     """In every buffer [slots, ...], slot ``slot0 + g * beams + b`` takes what slot ``slot0 + g * beams + parents[g, b]`` held, in place and for any map
     (``onebit_reorder_slots``); ``parents`` int32 [groups, beams] on the device, an entry outside 0 .. beams - 1 leaves its slot as it is.  With ``count``,
     buffers are caches [slots, heads, positions, D] of which positions ``first`` .. ``first + count - 1`` move.  Any dtype; buffers do not overlap."""
-    if parents.dim() != 2 or parents.dtype != torch.int32 or not parents.is_contiguous():
+    if parents.dim() != 2 or parents.dtype is not _I32 or not parents.is_contiguous():
         raise ValueError("reorder_slots: parents must be a contiguous int32 [groups, beams]")
     _require_gpu(parents, "reorder_slots")
     groups, beams = parents.shape

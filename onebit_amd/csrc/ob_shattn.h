@@ -4,10 +4,12 @@
 //   o = sum_j e^{s_j} v_j / sum_j e^{s_j},  s_j = q . k_j / sqrt(D),  j over prefix and own keys together
 // A range of keys leaves a PART: its maximum m, l = sum e^{s - m} and o = sum e^{s - m} v in fp32.  A part is also a state of the running
 // softmax, so parts join by starting from them:  M = max m_p,  l = sum e^{m_p - M} l_p,  o = sum e^{m_p - M} o_p / l.
-//   ob_sh_prefix_kernel / ob_sh_wide_kernel   parts of the prefixes: (kv head) x (block of the group's queries) x (chunk of keys)
-//   ob_sh_own_kernel                          a row's own keys, started from the prefix's parts: the outputs, or, where a row's own keys are
-//                                             split as well, parts again, which ob_sh_join_kernel joins
-// Where a prefix is so short that every row may read it again, the own kernel does, alone.  Parts are joined in their order: deterministic.
+//   ob_sh_one_kernel     few workgroups: parts of the prefixes, (kv head) x (block of the group's queries) x (chunk of keys), and of the rows' own
+//                        keys in one launch; the last workgroup to arrive at a row joins its parts
+//   ob_sh_wide_kernel    many: parts of the prefixes, up to 128 queries of a group at a time, then
+//   ob_sh_own_kernel     the rows' own keys, started from the prefix's parts: the outputs, or, where a row's own keys are split as well, parts
+//                        again, which ob_sh_join_kernel joins.  Where a prefix is so short that every row may read it again, this kernel does, alone
+// Parts are joined in their order, whoever does it: deterministic.
 //
 // Both products are computed transposed, S^T = K Q^T and O^T = V^T P^T (MFMA 16x16x32): a lane holds 4 consecutive keys of one query
 // per 16-key tile, which are, for two tiles, its 8 k elements of the second product; V lies row-major in the LDS and is transposed by
@@ -15,6 +17,7 @@
 // Scores, maxima, sums and outputs are fp32.  The weights e^{s - m} enter the second product as fp16 (relative error 2^-11 each, which the
 // sum averages; the output is rounded to fp16 anyway), the denominator sums the same rounded weights.
 #pragma once
+#include <type_traits>
 #include "ob_common.h"
 
 #define OB_SH_THREADS 256
@@ -36,6 +39,8 @@ struct ObShArgs {
     int pchunk, ochunk, psplits, osplits;             // keys per chunk; parts of a row: psplits of the prefix, then osplits of its own (0: one chunk, no part)
     int own_mb, max_own;                              // query blocks per row and kv head; most own positions
     int inline_prefix;                                // the own kernel reads the prefixes itself
+    int one_items;                                    // ob_sh_one_kernel: items of the prefixes, in front of the rows'
+    int *tickets;                                     // [rows][Hkv] arrivals at a row, zero between launches
     float scale_log2e;                                // log2(e) / sqrt(D)
     int n_groups;
     ObShGroup g[OB_SH_GROUPS];
@@ -87,8 +92,9 @@ struct ObShWave {
         }
     }
 
-    // Weights of 32 keys from key `base` on (kf: their rows); keys from `end` on count for nothing
-    __device__ __forceinline__ void weights(const ob_half8 (&kf)[2][DK], float scale, int base, int end, ob_half8 (&pb)[MT])
+    // Weights of 32 keys (kf: their rows); TAIL: only the first `n` count
+    template <bool TAIL>
+    __device__ __forceinline__ void weights(const ob_half8 (&kf)[2][DK], float scale, int n, ob_half8 (&pb)[MT])
     {
         const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
@@ -100,10 +106,10 @@ struct ObShWave {
 #pragma unroll
                 for (int j = 0; j < DK; ++j) s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[kt][j], qf[mt][j], s[kt], 0, 0, 0);
             }
-            if (base + 32 > end)
+            if (TAIL)
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    if (base + 16 * (e >> 2) + 4 * g + (e & 3) >= end) s[e >> 2][e & 3] = -INFINITY;
+                    if (16 * (e >> 2) + 4 * g + (e & 3) >= n) s[e >> 2][e & 3] = -INFINITY;
             float mx = -INFINITY;
 #pragma unroll
             for (int e = 0; e < 8; ++e) mx = fmaxf(mx, s[e >> 2][e & 3]);
@@ -147,13 +153,14 @@ struct ObShRange { const _Float16 *k, *v; int begin, end; };
 __device__ __forceinline__ int ob_sh_tiles(int n) { return (n + 31) >> 5; }
 
 // A workgroup's four waves over the keys of two ranges one after the other, 32 in turn; each starts from what W holds, the four results are joined in wave 0's W.
+// meanwhile(W) runs while the first loads are on their way.
 // K goes from memory to registers in the layout of its product, V by registers into the wave's own part of the LDS: no barrier in the loop, the
 // next 32 keys and values are on their way while a wave computes.
 template <int DP, int MT, bool EXACT> constexpr int ob_sh_body_floats() { return (4 * 32 * DP * 2 > 2 * MT * 16 * DP * 4 ? 4 * 32 * DP * 2 : 2 * MT * 16 * DP * 4) / 4; }
 template <int DP, int MT, bool EXACT> constexpr int ob_sh_lds_floats() { return ob_sh_body_floats<DP, MT, EXACT>() + 4 * MT * 16 * 2; }
 
-template <int DP, int MT, bool EXACT>
-__device__ __forceinline__ void ob_sh_sweep(const ObShArgs &A, const ObShRange &R0, const ObShRange &R1, ObShWave<DP, MT, EXACT> &W, float *sm)
+template <int DP, int MT, bool EXACT, typename F>
+__device__ __forceinline__ void ob_sh_sweep(const ObShArgs &A, const ObShRange &R0, const ObShRange &R1, ObShWave<DP, MT, EXACT> &W, float *sm, F meanwhile)
 {
     constexpr int DK = DP / 32, DT = DP / 16, PPR = DP / 8, RPL = 64 / PPR, NV = 32 / RPL;       // pieces of 16 bytes per row, rows per load, loads of a V tile
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 15, g = lane >> 4;
@@ -187,6 +194,7 @@ __device__ __forceinline__ void ob_sh_sweep(const ObShArgs &A, const ObShRange &
         }
     };
     if (wave < n) { load_v(wave); load_k(wave); }                      // (values first, as in the loop: what waits for them lets the keys come)
+    meanwhile(W);
     for (int t = wave; t < n; t += 4) {
         const bool one = t < n0;
         const int end = one ? R0.end : R1.end, base = one ? R0.begin + 32 * t : R1.begin + 32 * (t - n0);
@@ -201,7 +209,7 @@ __device__ __forceinline__ void ob_sh_sweep(const ObShArgs &A, const ObShRange &
         __builtin_amdgcn_wave_barrier();
         if (t + 4 < n) load_v(t + 4);
         ob_half8 pb[MT];
-        W.weights(kf, A.scale_log2e, base, end, pb);
+        W.template weights<true>(kf, A.scale_log2e, end - base, pb);
         if (t + 4 < n) load_k(t + 4);
         W.values(vt, pb);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -243,8 +251,8 @@ __device__ __forceinline__ void ob_sh_sweep(const ObShArgs &A, const ObShRange &
         for (int i = 0; i < MT * DT; ++i) W.acc[i / DT][i % DT] += buf[(MT * DT + i) * 64 + lane];
 }
 
-// What W holds of the queries qi0 .. of nq as their part `split`
-template <int DP, int MT, bool EXACT>
+// What W holds of the queries qi0 .. of nq as their part `split`; AGENT: past the XCD's L2, for readers of the same launch
+template <int DP, int MT, bool EXACT, bool AGENT = false>
 __device__ __forceinline__ void ob_sh_store(const ObShArgs &A, const ObShWave<DP, MT, EXACT> &W, int row0, int qi0, int nq, int kvh, int split)
 {
     const int lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4, D = EXACT ? DP : A.D;
@@ -253,10 +261,20 @@ __device__ __forceinline__ void ob_sh_store(const ObShArgs &A, const ObShWave<DP
         const int qi = qi0 + 16 * mt + lr;
         if (qi >= nq) continue;
         const int64_t p = ((int64_t)(row0 + qi / A.rep) * A.H + kvh * A.rep + qi % A.rep) * (A.psplits + A.osplits) + split;
-        if (g == 0) *reinterpret_cast<ob_float2 *>(A.part_ml + 2 * p) = (ob_float2){W.m[mt], W.l[mt][0]};
+        const auto two = [](float *to, float a, float b) {
+            const ob_float2 v = {a, b};
+            if (AGENT) __hip_atomic_store(reinterpret_cast<unsigned long long *>(to), __builtin_bit_cast(unsigned long long, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            else *reinterpret_cast<ob_float2 *>(to) = v;
+        };
+        if (g == 0) two(A.part_ml + 2 * p, W.m[mt], W.l[mt][0]);
 #pragma unroll
-        for (int dt = 0; dt < DP / 16; ++dt)
-            if (EXACT || 16 * dt + 4 * g < D) *reinterpret_cast<ob_float4 *>(A.part_o + p * D + 16 * dt + 4 * g) = W.acc[mt][dt];
+        for (int dt = 0; dt < DP / 16; ++dt) {
+            float *to = A.part_o + p * D + 16 * dt + 4 * g;
+            if (!EXACT && 16 * dt + 4 * g >= D) continue;
+            if (!AGENT) { *reinterpret_cast<ob_float4 *>(to) = W.acc[mt][dt]; continue; }
+            two(to, W.acc[mt][dt][0], W.acc[mt][dt][1]);
+            two(to + 2, W.acc[mt][dt][2], W.acc[mt][dt][3]);
+        }
     }
 }
 
@@ -281,23 +299,10 @@ __device__ __forceinline__ ObShItem ob_sh_item(const ObShArgs &A, int per, ObShG
     return I;
 }
 
-// Up to 32 queries of a group and kv head: the four waves share the keys out.
-template <int DP, int MT, bool EXACT>
-__global__ __launch_bounds__(OB_SH_THREADS, 2) void ob_sh_prefix_kernel(const ObShArgs A)
-{
-    __shared__ __attribute__((aligned(16))) float sm[ob_sh_lds_floats<DP, MT, EXACT>()];
-    ObShGroup G;
-    const ObShItem I = ob_sh_item(A, 16 * MT, G);
-    ObShWave<DP, MT, EXACT> W;
-    W.init(A, G.row0, I.qi0, G.n * A.rep, I.kvh);
-    ob_sh_sweep<DP, MT, EXACT>(A, {I.kb, I.vb, I.k0, I.k1}, {I.kb, I.vb, 0, 0}, W, sm);
-    if (threadIdx.x < 64) ob_sh_store<DP, MT, EXACT>(A, W, G.row0, I.qi0, G.n * A.rep, I.kvh, I.chunk);
-}
-
 // More queries: the four waves share the queries out, 16 MT each, over tiles of 64 keys and values that they read from the LDS together (two tiles there,
 // a third on its way in registers; one barrier a tile).
 template <int DP, int MT, bool EXACT>
-__global__ __launch_bounds__(OB_SH_THREADS, MT < 4 ? 2 : 1) void ob_sh_wide_kernel(const ObShArgs A)
+__global__ __launch_bounds__(OB_SH_THREADS, 2) void ob_sh_wide_kernel(const ObShArgs A)
 {
     constexpr int DK = DP / 32, PPR = DP / 8, NP = 64 * PPR / OB_SH_THREADS, RPL = OB_SH_THREADS / PPR;      // pieces of a thread, rows apart
     __shared__ __attribute__((aligned(16))) _Float16 kv[2][2][64 * DP];
@@ -331,23 +336,25 @@ __global__ __launch_bounds__(OB_SH_THREADS, MT < 4 ? 2 : 1) void ob_sh_wide_kern
     store(I.k0, 0);
     if (I.k0 + 64 < I.k1) load(I.k0 + 64);
     __syncthreads();
-    int b = 0;
-    for (int base = I.k0; base < I.k1; base += 64, b ^= 1) {
+    const auto half = [&](int b, int h, auto tail, int n) {                          // 32 keys of the tile in buffer b
+        ob_half8 kf[2][DK], pb[MT];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int j = 0; j < DK; ++j) kf[kt][j] = *reinterpret_cast<const ob_half8 *>(&kv[b][0][ob_sh_place<DP>(32 * h + 16 * kt + lr, 4 * j + g)]);
+        W.template weights<decltype(tail)::value>(kf, A.scale_log2e, n, pb);
+        W.values(&kv[b][1][32 * h * DP], pb);
+    };
+    int b = 0, base = I.k0;
+    for (; base + 64 <= I.k1; base += 64, b ^= 1) {
         if (base + 64 < I.k1) store(base + 64, b ^ 1);
         if (base + 128 < I.k1) load(base + 128);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if (base + 32 * h >= I.k1) break;
-            ob_half8 kf[2][DK], pb[MT];
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                for (int j = 0; j < DK; ++j) kf[kt][j] = *reinterpret_cast<const ob_half8 *>(&kv[b][0][ob_sh_place<DP>(32 * h + 16 * kt + lr, 4 * j + g)]);
-            W.weights(kf, A.scale_log2e, base + 32 * h, I.k1, pb);
-            W.values(&kv[b][1][32 * h * DP], pb);
-        }
+        half(b, 0, std::false_type(), 32);
+        half(b, 1, std::false_type(), 32);
         __syncthreads();
     }
+#pragma unroll 1
+    for (int h = 0; base + 32 * h < I.k1; ++h) half(b, h, std::true_type(), I.k1 - base - 32 * h);
     ob_sh_store<DP, MT, EXACT>(A, W, G.row0, qi0, nq, I.kvh, I.chunk);
 }
 
@@ -382,25 +389,36 @@ __global__ __launch_bounds__(OB_SH_THREADS, 2) void ob_sh_own_kernel(const ObShA
     W.init(A, r, 16 * mb, A.rep, kvh);
     const int qi = 16 * mb + lr, head = kvh * A.rep + qi;
     const bool mine = qi < A.rep;
-    if (!parts && !A.inline_prefix) {
+    // the prefix's parts, this wave's of them: two at a time
+    const auto start = [&](ObShWave<DP, 1, EXACT> &W) {
+        if (parts || A.inline_prefix) return;
         const int64_t p0 = ((int64_t)r * A.H + (mine ? head : 0)) * A.psplits;
-        for (int s = wave; s < G.chunks; s += 4) {
-            const ob_float2 ml = mine ? *reinterpret_cast<const ob_float2 *>(A.part_ml + 2 * (p0 + s)) : (ob_float2){-INFINITY, 0.f};
-            const float M = fmaxf(W.m[0], ml[0]), f = ob_sh_weight(W.m[0], M), x = ob_sh_weight(ml[0], M);
-            W.m[0] = M;
-            W.l[0] = W.l[0] * f + x * ml[1];
+        for (int s0 = wave; s0 < G.chunks; s0 += 8) {
+            ob_float2 ml[2];
+            ob_float4 o[2][DT];
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                const bool in = mine && (EXACT || 16 * dt + 4 * g < D);
-                const ob_float4 o = in ? *reinterpret_cast<const ob_float4 *>(A.part_o + (p0 + s) * D + 16 * dt + 4 * g) : (ob_float4){0.f, 0.f, 0.f, 0.f};
-                W.acc[0][dt] = W.acc[0][dt] * f + o * x;
+            for (int j = 0; j < 2; ++j) {
+                const bool in = mine && s0 + 4 * j < G.chunks;
+                const int64_t p = p0 + min(s0 + 4 * j, G.chunks - 1);
+                ml[j] = in ? *reinterpret_cast<const ob_float2 *>(A.part_ml + 2 * p) : (ob_float2){-INFINITY, 0.f};
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+                    o[j][dt] = in && (EXACT || 16 * dt + 4 * g < D) ? *reinterpret_cast<const ob_float4 *>(A.part_o + p * D + 16 * dt + 4 * g) : (ob_float4){0.f, 0.f, 0.f, 0.f};
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const float M = fmaxf(W.m[0], ml[j][0]), f = ob_sh_weight(W.m[0], M), x = ob_sh_weight(ml[j][0], M);
+                W.m[0] = M;
+                W.l[0] = W.l[0] * f + x * ml[j][1];
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) W.acc[0][dt] = W.acc[0][dt] * f + o[j][dt] * x;
             }
         }
-    }
+    };
     const int64_t row = ((int64_t)slot * A.Hkv + kvh) * A.max_len * A.D;
     const int64_t prow = A.inline_prefix ? ((int64_t)G.slot * A.Hkv + kvh) * A.p_max_len * A.D : 0;
     const int k0 = first + (parts ? split * A.ochunk : 0), k1 = first + (parts ? min(own, (split + 1) * A.ochunk) : own);
-    ob_sh_sweep<DP, 1, EXACT>(A, {A.pk + prow, A.pv + prow, 0, A.inline_prefix ? G.len : 0}, {A.k + row, A.v + row, k0, k1}, W, sm);
+    ob_sh_sweep<DP, 1, EXACT>(A, {A.pk + prow, A.pv + prow, 0, A.inline_prefix ? G.len : 0}, {A.k + row, A.v + row, k0, k1}, W, sm, start);
     if (wave) return;
     if (parts) {
         ob_sh_store<DP, 1, EXACT>(A, W, r, 16 * mb, A.rep, kvh, A.psplits + split);
@@ -424,19 +442,17 @@ __global__ __launch_bounds__(OB_SH_THREADS, 2) void ob_sh_own_kernel(const ObShA
     }
 }
 
-// A wave per (row, head): its parts in order, two output columns a lane.
-__global__ __launch_bounds__(OB_SH_THREADS) void ob_sh_join_kernel(const ObShArgs A)
+// A wave joins the n parts of (row, head), np of them the prefix's, in order, two output columns a lane
+template <bool AGENT>
+__device__ __forceinline__ void ob_sh_join(const ObShArgs &A, int r, int head, int np, int n)
 {
-    const int w = blockIdx.x * (OB_SH_THREADS / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (w >= A.rows * A.H) return;
-    const int r = A.row_base + w / A.H, head = w % A.H;
-    int gi = 0, slot, own;
-    while (r >= A.g[gi].row0 + A.g[gi].n) ++gi;
-    if (!ob_sh_row(A, r, A.g[gi].first, slot, own)) return;                       // idle: its output stays as it is
-    const int np = A.g[gi].chunks, n = np + (own + A.ochunk - 1) / A.ochunk;
-    const int64_t p0 = ((int64_t)r * A.H + head) * (A.psplits + A.osplits);
-    const int d = 2 * lane;
+    const int lane = threadIdx.x & 63, d = 2 * lane;
     if (d >= A.D) return;
+    const int64_t p0 = ((int64_t)r * A.H + head) * (A.psplits + A.osplits);
+    const auto two = [](const float *p) -> ob_float2 {
+        if (!AGENT) return *reinterpret_cast<const ob_float2 *>(p);
+        return __builtin_bit_cast(ob_float2, __hip_atomic_load(reinterpret_cast<const unsigned long long *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    };
     float M = -INFINITY, l = 0.f;
     ob_float2 o = {0.f, 0.f};
     for (int s0 = 0; s0 < n; s0 += 8) {
@@ -445,8 +461,8 @@ __global__ __launch_bounds__(OB_SH_THREADS) void ob_sh_join_kernel(const ObShArg
         for (int j = 0; j < 8; ++j) {
             const int s = min(s0 + j, n - 1);
             const int64_t p = p0 + (s < np ? s : A.psplits + s - np);
-            ml[j] = *reinterpret_cast<const ob_float2 *>(A.part_ml + 2 * p);
-            po[j] = *reinterpret_cast<const ob_float2 *>(A.part_o + p * A.D + d);
+            ml[j] = two(A.part_ml + 2 * p);
+            po[j] = two(A.part_o + p * A.D + d);
         }
         float mb = M;
 #pragma unroll
@@ -462,8 +478,94 @@ __global__ __launch_bounds__(OB_SH_THREADS) void ob_sh_join_kernel(const ObShArg
             }
     }
     _Float16 *out = A.o + ((int64_t)r * A.H + head) * A.D + d;
-    ob_half2 y = {(_Float16)0, (_Float16)0};                                       // no key at all: zeros
-    if (n) { y[0] = (_Float16)(o[0] / l); y[1] = (_Float16)(o[1] / l); }
+    ob_half2 y = {(_Float16)(o[0] / l), (_Float16)(o[1] / l)};
     if (A.h_next) { y[0] *= A.h_next[head * A.D + d]; y[1] *= A.h_next[head * A.D + d + 1]; }
     *reinterpret_cast<ob_half2 *>(out) = y;
+}
+
+__global__ __launch_bounds__(OB_SH_THREADS) void ob_sh_join_kernel(const ObShArgs A)
+{
+    const int w = blockIdx.x * (OB_SH_THREADS / 64) + (threadIdx.x >> 6);
+    if (w >= A.rows * A.H) return;
+    const int r = A.row_base + w / A.H, head = w % A.H;
+    int gi = 0, slot, own;
+    while (r >= A.g[gi].row0 + A.g[gi].n) ++gi;
+    if (!ob_sh_row(A, r, A.g[gi].first, slot, own)) return;                       // idle: its output stays as it is
+    const int np = A.g[gi].chunks, n = np + (own + A.ochunk - 1) / A.ochunk;
+    if (n) ob_sh_join<false>(A, r, head, np, n);
+    else if (2 * (threadIdx.x & 63) < A.D) *reinterpret_cast<ob_half2 *>(A.o + ((int64_t)r * A.H + head) * A.D + 2 * (threadIdx.x & 63)) = (ob_half2)(_Float16)0;
+}
+
+// One launch: the items of the prefixes (up to 16 MT queries of a group), then those of the rows' own keys.  A workgroup publishes its part WRITE-THROUGH
+// (agent-scope stores), waits until it has left, and takes a ticket of every row that it holds queries of; the last one at a row joins the row's parts and
+// sets the ticket back to zero.  Every row has own items, an empty one if it has no key of its own.
+template <int DP, int MT, bool EXACT>
+__global__ __launch_bounds__(OB_SH_THREADS, 2) void ob_sh_one_kernel(const ObShArgs A)
+{
+    __shared__ __attribute__((aligned(16))) float sm[ob_sh_lds_floats<DP, MT, EXACT>()];
+    __shared__ int last_s[64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int row0, r_lo, r_hi, kvh, chunks, per, first, n_query;              // rows that this workgroup holds queries of
+    if ((int)blockIdx.x < A.one_items * A.Hkv) {
+        ObShGroup G;
+        const ObShItem I = ob_sh_item(A, 16 * MT, G);
+        ObShWave<DP, MT, EXACT> W;
+        n_query = G.n * A.rep;
+        W.init(A, G.row0, I.qi0, n_query, I.kvh);
+        ob_sh_sweep<DP, MT, EXACT>(A, {I.kb, I.vb, I.k0, I.k1}, {I.kb, I.vb, 0, 0}, W, sm, [](auto &) {});
+        if (wave == 0) ob_sh_store<DP, MT, EXACT, true>(A, W, G.row0, I.qi0, n_query, I.kvh, I.chunk);
+        row0 = G.row0; kvh = I.kvh; chunks = G.chunks; first = G.first;
+        r_lo = G.row0 + I.qi0 / A.rep;
+        r_hi = G.row0 + (min(I.qi0 + 16 * MT, n_query) - 1) / A.rep;
+    } else {
+        const int at0 = blockIdx.x - A.one_items * A.Hkv, item = at0 / A.Hkv;
+        kvh = at0 - item * A.Hkv;
+        const int at = item / A.rows, r = A.row_base + item - at * A.rows, split = at / A.own_mb, mb = at - split * A.own_mb;
+        int gi = 0, slot, own;
+        while (r >= A.g[gi].row0 + A.g[gi].n) ++gi;
+        const ObShGroup &G = A.g[gi];
+        first = G.first;
+        if (!ob_sh_row(A, r, first, slot, own)) return;                          // idle: its output stays as it is
+        if (split && split * A.ochunk >= own) return;
+        const int64_t row = ((int64_t)slot * A.Hkv + kvh) * A.max_len * A.D;
+        ObShWave<DP, 1, EXACT> W;
+        W.init(A, r, 16 * mb, A.rep, kvh);
+        ob_sh_sweep<DP, 1, EXACT>(A, {A.k + row, A.v + row, first + split * A.ochunk, first + min(own, (split + 1) * A.ochunk)}, {A.k + row, A.v + row, 0, 0}, W, sm,
+                                  [](auto &) {});
+        if (wave == 0) ob_sh_store<DP, 1, EXACT, true>(A, W, r, 16 * mb, A.rep, kvh, A.psplits + split);
+        row0 = G.row0; chunks = G.chunks; n_query = G.n * A.rep;
+        r_lo = r_hi = r;
+    }
+    per = 16 * MT;
+    if (wave == 0) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                         // the part has left
+        for (int r = r_lo + lane; r <= r_hi; r += 64) {                          // (at most 16 MT rows: one turn)
+            int slot, own, last = 0;
+            if (ob_sh_row(A, r, first, slot, own)) {
+                const int q = (r - row0) * A.rep, blocks = (q + A.rep - 1) / per - q / per + 1;
+                const int all = chunks * blocks + A.own_mb * max(1, (own + A.ochunk - 1) / A.ochunk);
+                int *t = A.tickets + (int64_t)r * A.Hkv + kvh;
+                last = __hip_atomic_fetch_add(t, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == all - 1;
+                if (last) __hip_atomic_store(t, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (last) last = chunks + max(1, (own + A.ochunk - 1) / A.ochunk);      // its parts
+            }
+            last_s[r - r_lo] = last;
+        }
+    }
+    __syncthreads();
+    const int pairs = (r_hi - r_lo + 1) * A.rep;
+    for (int i = wave; i < pairs; i += 4) {
+        const int r = i / A.rep, n = last_s[r];
+        if (!n) continue;
+        const int head = kvh * A.rep + i - r * A.rep;
+        if (chunks == 0 && n == 1) {                                             // perhaps without any key: zeros
+            int slot, own;
+            ob_sh_row(A, r_lo + r, first, slot, own);
+            if (own == 0) {
+                if (2 * lane < A.D) *reinterpret_cast<ob_half2 *>(A.o + ((int64_t)(r_lo + r) * A.H + head) * A.D + 2 * lane) = (ob_half2)(_Float16)0;
+                continue;
+            }
+        }
+        ob_sh_join<true>(A, r_lo + r, head, chunks, n);
+    }
 }

@@ -17,8 +17,10 @@ static const int64_t OB_MAX_WGS = 0xffffff;            // workgroups of 256 thre
 static const int64_t OB_SH_MAX_LEN = 1 << 30;         // (positions and their chunks are counted in 32 bits)
 
 // ------------------------------------------------------------------------------------------- attention over a shared prefix --
-// form: 0, 1: ob_sh_prefix_kernel of 16, 32 queries; 2, 3, 4: ob_sh_wide_kernel of 64, 128, 256; osplits 0: a row's own keys are one chunk
-struct ObShPlan { int form, per, pchunk, ochunk, psplits, osplits, own_mb, inline_prefix; };
+// form: ob_sh_one_kernel; ob_sh_wide_kernel of 64 / 128 queries and ob_sh_own_kernel; the latter alone.  osplits 0: a row's own keys are one chunk, no part
+enum { OB_SH_INLINE, OB_SH_ONE, OB_SH_WIDE64, OB_SH_WIDE128 };
+struct ObShPlan { int form, per, pchunk, ochunk, psplits, osplits, own_mb; };
+#define OB_SH_TICKETS 16384                           // their place in front of the scratch memory does not depend on a call's sizes
 
 static ObShPlan ob_sh_plan(const onebit_prefix_t *groups, int32_t n_groups, int64_t rows, int32_t n_heads, int32_t n_kv_heads, int64_t max_own)
 {
@@ -32,17 +34,20 @@ static ObShPlan ob_sh_plan(const onebit_prefix_t *groups, int32_t n_groups, int6
     }
     p.own_mb = (int)ob_up(rep, 16);
     const int64_t own = rows * n_kv_heads * p.own_mb;                    // workgroups of one chunk per row
-    if (own < 256 && max_own > 512) {
-        p.ochunk = (int)(128 * std::max<int64_t>(2, ob_up(own * max_own, 512 * 128)));
-        p.osplits = (int)ob_up(max_own, p.ochunk);
+    p.ochunk = (int)(128 * std::max<int64_t>(1, ob_up(max_own, 128)));
+    if (own < 256 && max_own > 512) p.ochunk = (int)(128 * std::max<int64_t>(2, ob_up(own * max_own, 512 * 128)));
+    p.osplits = (int)ob_up(max_own, p.ochunk);
+    if (p.osplits <= 1 && longest <= 256 && again * n_kv_heads * p.own_mb <= 64 * 1024) {
+        p.form = OB_SH_INLINE;
+        p.osplits = 0;
+        return p;
     }
-    if (p.osplits <= 1) { p.osplits = 0; p.ochunk = 1; }
-    p.inline_prefix = p.osplits == 0 && longest <= 256 && again * n_kv_heads * p.own_mb <= 64 * 1024;
-    if (p.inline_prefix) return p;
-    p.form = most <= 16 ? 0 : most <= 32 ? 1 : most <= 64 ? 2 : most <= 128 ? 3 : 4;
-    p.per = 16 << p.form;
+    p.form = most <= 16 && rows * n_kv_heads <= OB_SH_TICKETS && own <= 1024 ? OB_SH_ONE : most <= 64 ? OB_SH_WIDE64 : OB_SH_WIDE128;
+    p.per = p.form == OB_SH_ONE ? 16 : p.form == OB_SH_WIDE64 ? 64 : 128;
+    if (p.form == OB_SH_ONE) p.osplits = std::max(p.osplits, 1);
+    else if (p.osplits <= 1) p.osplits = 0;
     for (int i = 0; i < n_groups; ++i) work += ob_up(groups[i].n * rep, p.per) * groups[i].len * n_kv_heads;
-    p.pchunk = (int)(128 * std::max<int64_t>(1, ob_up(work, (p.form == 4 ? 256 : 512) * 128)));
+    p.pchunk = (int)(128 * std::max<int64_t>(1, ob_up(work, 512 * 128)));
     p.psplits = (int)ob_up(longest, p.pchunk);
     return p;
 }
@@ -71,21 +76,22 @@ extern "C" size_t onebit_attention_shared_scratch_bytes(const onebit_prefix_t *g
 {
     if (rows <= 0 || ob_sh_check(groups, n_groups, rows, n_heads, n_kv_heads, head_dim, max_own)) return 0;
     const ObShPlan p = ob_sh_plan(groups, n_groups, rows, n_heads, n_kv_heads, max_own);
-    return (size_t)rows * n_heads * (p.psplits + p.osplits) * (head_dim + 2) * 4 + 16;
+    return OB_SH_TICKETS * 4 + (size_t)rows * n_heads * (p.psplits + p.osplits) * (head_dim + 2) * 4;
 }
 
 template <int DP, bool EXACT>
 static void ob_sh_launch(const ObShArgs &a, int form, int64_t prefix_items, int64_t own_items, hipStream_t s)
 {
-    const dim3 block(OB_SH_THREADS), pg((unsigned)(prefix_items * a.Hkv)), og((unsigned)(own_items * a.Hkv));
-    if (prefix_items > 0) {
-        if (form == 0) hipLaunchKernelGGL((ob_sh_prefix_kernel<DP, 1, EXACT>), pg, block, 0, s, a);
-        else if (form == 1) hipLaunchKernelGGL((ob_sh_prefix_kernel<DP, 2, EXACT>), pg, block, 0, s, a);
-        else if (form == 2) hipLaunchKernelGGL((ob_sh_wide_kernel<DP, 1, EXACT>), pg, block, 0, s, a);
-        else if (form == 3) hipLaunchKernelGGL((ob_sh_wide_kernel<DP, 2, EXACT>), pg, block, 0, s, a);
-        else hipLaunchKernelGGL((ob_sh_wide_kernel<DP, 4, EXACT>), pg, block, 0, s, a);
+    const dim3 block(OB_SH_THREADS), pg((unsigned)(prefix_items * a.Hkv)), og((unsigned)(own_items * a.Hkv)), all(pg.x + og.x);
+    if (form == OB_SH_ONE) hipLaunchKernelGGL((ob_sh_one_kernel<DP, 1, EXACT>), all, block, 0, s, a);
+    else {
+        if (prefix_items > 0) {
+            if (form == OB_SH_WIDE64) hipLaunchKernelGGL((ob_sh_wide_kernel<DP, 1, EXACT>), pg, block, 0, s, a);
+            else hipLaunchKernelGGL((ob_sh_wide_kernel<DP, 2, EXACT>), pg, block, 0, s, a);
+        }
+        hipLaunchKernelGGL((ob_sh_own_kernel<DP, EXACT>), og, block, 0, s, a);
+        if (a.osplits) hipLaunchKernelGGL(ob_sh_join_kernel, dim3((unsigned)ob_up((int64_t)a.rows * a.H, OB_SH_THREADS / 64)), block, 0, s, a);
     }
-    hipLaunchKernelGGL((ob_sh_own_kernel<DP, EXACT>), og, block, 0, s, a);
 }
 
 extern "C" int onebit_attention_shared_rows(const void *q, const void *prefix_k, const void *prefix_v, const void *k_cache, const void *v_cache, void *o,
@@ -112,7 +118,7 @@ extern "C" int onebit_attention_shared_rows(const void *q, const void *prefix_k,
         (prefixes && (!ob_aligned(prefix_k, 16) || !ob_aligned(prefix_v, 16))))
         return ob_fail(ONEBIT_E_ALIGN, "attention_shared_rows: q and the caches must be 16-byte aligned");
     const size_t need = onebit_attention_shared_scratch_bytes(groups, n_groups, rows, n_heads, n_kv_heads, head_dim, max_own);
-    if (!scratch || scratch_bytes < need || !ob_aligned(scratch, 16)) return ob_fail(ONEBIT_E_WSPACE, "attention_shared_rows: needs %zu bytes of 16-byte aligned scratch", need);
+    if (!scratch || scratch_bytes < need || !ob_aligned(scratch, 16)) return ob_fail(ONEBIT_E_WSPACE, "attention_shared_rows: needs %zu bytes of zero-initialised, 16-byte aligned scratch", need);
     const ObShPlan p = ob_sh_plan(groups, n_groups, rows, n_heads, n_kv_heads, max_own);
     const int64_t rep = n_heads / n_kv_heads;
     ObShArgs a = {};
@@ -120,10 +126,11 @@ extern "C" int onebit_attention_shared_rows(const void *q, const void *prefix_k,
     a.o = (_Float16 *)o; a.h_next = (const _Float16 *)h_next; a.row_slot = row_slot; a.row_pos = row_pos;
     a.p_max_len = prefix_max_len; a.max_len = max_len; a.H = n_heads; a.Hkv = n_kv_heads; a.rep = (int)rep; a.D = head_dim; a.n_slots = (int)n_slots;
     a.pchunk = p.pchunk; a.ochunk = p.ochunk; a.psplits = p.psplits; a.osplits = p.osplits; a.own_mb = p.own_mb; a.max_own = (int)max_own;
-    a.inline_prefix = p.inline_prefix;
+    a.inline_prefix = p.form == OB_SH_INLINE;
     a.scale_log2e = 1.4426950408889634f / sqrtf((float)head_dim);
     const size_t parts = (size_t)rows * n_heads * (p.psplits + p.osplits);
-    a.part_o = (float *)scratch;
+    a.tickets = (int *)scratch;
+    a.part_o = (float *)scratch + OB_SH_TICKETS;
     a.part_ml = a.part_o + parts * head_dim;
     for (int g0 = 0; g0 < n_groups; g0 += OB_SH_GROUPS) {
         a.n_groups = std::min(n_groups - g0, OB_SH_GROUPS);
@@ -131,20 +138,19 @@ extern "C" int onebit_attention_shared_rows(const void *q, const void *prefix_k,
         int64_t items = 0;
         for (int i = 0; i < a.n_groups; ++i) {
             const onebit_prefix_t &g = groups[g0 + i];
-            const int64_t chunks = p.inline_prefix ? 0 : ob_up(g.len, p.pchunk);
+            const int64_t chunks = a.inline_prefix ? 0 : ob_up(g.len, p.pchunk);
             items += chunks ? chunks * ob_up(g.n * rep, p.per) : 0;
             a.g[i] = {g.row0, g.n, g.slot, g.len, g.first, (int)chunks, (int)items};
             a.rows += g.n;
         }
         const int64_t own_items = (int64_t)a.rows * p.own_mb * std::max(p.osplits, 1);
-        if (items * n_kv_heads > OB_MAX_WGS || own_items * n_kv_heads > OB_MAX_WGS) return ob_fail(ONEBIT_E_ARG, "attention_shared_rows: too many workgroups");
+        a.one_items = (int)items;
+        if ((items + own_items) * n_kv_heads > OB_MAX_WGS) return ob_fail(ONEBIT_E_ARG, "attention_shared_rows: too many workgroups");
         hipStream_t s = (hipStream_t)stream;
         if (head_dim == 128) ob_sh_launch<128, true>(a, p.form, items, own_items, s);
         else if (head_dim == 64) ob_sh_launch<64, true>(a, p.form, items, own_items, s);
         else if (head_dim > 64) ob_sh_launch<128, false>(a, p.form, items, own_items, s);
         else ob_sh_launch<64, false>(a, p.form, items, own_items, s);
-        if (p.osplits)
-            hipLaunchKernelGGL(ob_sh_join_kernel, dim3((unsigned)ob_up((int64_t)a.rows * n_heads, OB_SH_THREADS / 64)), dim3(OB_SH_THREADS), 0, s, a);
         const int rc2 = ob_launch_status("attention_shared_rows");
         if (rc2) return rc2;
     }

@@ -741,6 +741,6 @@ class MixedStep:
         c = self.cfg
         nb = shared_prefix_workspace(groups, row, c.num_attention_heads, c.num_key_value_heads, c.head_dim, most, "meta").numel()
         if self._shared_ws is None or self._shared_ws.numel() < nb:
-            self._shared_ws = torch.empty(2 * nb, dtype=torch.uint8, device=self.dev)
+            self._shared_ws = torch.zeros(2 * nb, dtype=torch.uint8, device=self.dev)
         return self.lib.onebit_mixed_step_shared(ctypes.byref(self._model), ctypes.byref(state), _prefixes(groups), len(groups), most,
                                                  self._shared_ws.data_ptr(), self._shared_ws.numel(), stream)
