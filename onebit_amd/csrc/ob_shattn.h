@@ -58,7 +58,8 @@ __device__ __forceinline__ float ob_sh_rows_max(float v)
     auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
-__device__ __forceinline__ float ob_sh_weight(float m, float M) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M); }
+#define OB_SH_NONE -3e38f                // the maximum of no key (finite: differences of two stay numbers)
+__device__ __forceinline__ float ob_sh_weight(float m, float M) { return __builtin_amdgcn_exp2f(m - M); }
 
 // LDS place (halves) of 16-byte piece p of row r of a tile of DP columns: pairs of pieces swizzled by the row
 template <int DP> __device__ __forceinline__ int ob_sh_place(int r, int p) { return r * DP + 8 * (2 * ((p >> 1) ^ (r & (DP / 16 - 1))) + (p & 1)); }
@@ -85,7 +86,7 @@ struct ObShWave {
                 const int d = 32 * j + 8 * g;
                 qf[mt][j] = EXACT || d < D ? *reinterpret_cast<const ob_half8 *>(qr + d) : (ob_half8)(_Float16)0;
             }
-            m[mt] = -INFINITY;
+            m[mt] = OB_SH_NONE;
             l[mt] = (ob_float4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) acc[mt][dt] = (ob_float4){0.f, 0.f, 0.f, 0.f};
@@ -110,21 +111,27 @@ struct ObShWave {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                     if (16 * (e >> 2) + 4 * g + (e & 3) >= n) s[e >> 2][e & 3] = -INFINITY;
-            float mx = -INFINITY;
+            // the running maximum moves only where a weight exceeds 2^8 (the first ones do): the weights stay far inside fp16, and neither the tile's maximum nor a
+            // rescaled output is needed otherwise.  Weights are not negative, so their bits order like whole numbers.
+            const auto exponentials = [&]() {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, s[e >> 2][e & 3]);
-            mx = ob_sh_rows_max(mx) * scale;
-            // the running maximum moves only where a tile exceeds it by 2^8: the weights stay far inside fp16, the output is rescaled seldom
-            if (__any(mx > m[mt] + 8.f)) {
-                const float mn = fmaxf(m[mt], mx), f = ob_sh_weight(m[mt], mn);
+                for (int e = 0; e < 8; ++e) pb[mt][e] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 2][e & 3], scale, -m[mt]));
+            };
+            exponentials();
+            const ob_u32x4 bits = __builtin_bit_cast(ob_u32x4, pb[mt]);
+            const auto pair = [](uint32_t v) { return __builtin_bit_cast(ob_u16x2, v); };
+            const ob_u16x2 most = __builtin_elementwise_max(__builtin_elementwise_max(pair(bits[0]), pair(bits[1])), __builtin_elementwise_max(pair(bits[2]), pair(bits[3])));
+            if (__any(__builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(most, (ob_u16x2)(unsigned short)0x5c00)) != 0)) {
+                float mx = s[0][0];
+#pragma unroll
+                for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[e >> 2][e & 3]);
+                const float mn = fmaxf(m[mt], ob_sh_rows_max(mx) * scale), f = ob_sh_weight(m[mt], mn);
                 l[mt] *= f;
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) acc[mt][dt] *= f;
                 m[mt] = mn;
+                exponentials();
             }
-            const float mu = m[mt] == -INFINITY ? 0.f : m[mt];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) pb[mt][e] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 2][e & 3], scale, -mu));
         }
     }
 
@@ -400,7 +407,7 @@ __global__ __launch_bounds__(OB_SH_THREADS, 2) void ob_sh_own_kernel(const ObShA
             for (int j = 0; j < 2; ++j) {
                 const bool in = mine && s0 + 4 * j < G.chunks;
                 const int64_t p = p0 + min(s0 + 4 * j, G.chunks - 1);
-                ml[j] = in ? *reinterpret_cast<const ob_float2 *>(A.part_ml + 2 * p) : (ob_float2){-INFINITY, 0.f};
+                ml[j] = in ? *reinterpret_cast<const ob_float2 *>(A.part_ml + 2 * p) : (ob_float2){OB_SH_NONE, 0.f};
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt)
                     o[j][dt] = in && (EXACT || 16 * dt + 4 * g < D) ? *reinterpret_cast<const ob_float4 *>(A.part_o + p * D + 16 * dt + 4 * g) : (ob_float4){0.f, 0.f, 0.f, 0.f};
@@ -453,7 +460,7 @@ __device__ __forceinline__ void ob_sh_join(const ObShArgs &A, int r, int head, i
         if (!AGENT) return *reinterpret_cast<const ob_float2 *>(p);
         return __builtin_bit_cast(ob_float2, __hip_atomic_load(reinterpret_cast<const unsigned long long *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
     };
-    float M = -INFINITY, l = 0.f;
+    float M = OB_SH_NONE, l = 0.f;
     ob_float2 o = {0.f, 0.f};
     for (int s0 = 0; s0 < n; s0 += 8) {
         ob_float2 ml[8], po[8];

@@ -47,7 +47,7 @@ static ObShPlan ob_sh_plan(const onebit_prefix_t *groups, int32_t n_groups, int6
     if (p.form == OB_SH_ONE) p.osplits = std::max(p.osplits, 1);
     else if (p.osplits <= 1) p.osplits = 0;
     for (int i = 0; i < n_groups; ++i) work += ob_up(groups[i].n * rep, p.per) * groups[i].len * n_kv_heads;
-    p.pchunk = (int)(128 * std::max<int64_t>(1, ob_up(work, 512 * 128)));
+    p.pchunk = (int)(128 * std::max<int64_t>(p.form == OB_SH_ONE ? 1 : 2, ob_up(work, (p.form == OB_SH_ONE ? 256 : 512) * 128)));
     p.psplits = (int)ob_up(longest, p.pchunk);
     return p;
 }
