@@ -7,14 +7,13 @@
 // Both find the best by a threshold instead of one after the other: every wave publishes the largest of its lanes' largest values, its share of `keep` and
 // two more; at least `keep` candidates reach the keep-th of all published, and few more do; those are listed (the scan) or ranked by counting (the
 // pick).  Where too many reach it (rows of equal logits), the best are taken one after the other.
-// The logits are read once.  e^x: the product x log2 e is carried in two parts, so a term is off by 2^-23 at most however far x lies below the
-// maximum; terms are added in 64 bits.  A row's elements belong to threads by their index alone, not by the row's alignment: equal rows have equal
-// sums, bit for bit.
+// The logits are read once.  A term e^{x - max} is off by |x - max| 2^-24 of itself (the rounded product with log2 e), so by less than 2^-25 of the largest
+// term, with either sign; terms are added in 64 bits.  A row's elements belong to threads by their index alone, not by the row's alignment: equal rows
+// have equal sums, bit for bit.
 #pragma once
 #include "ob_common.h"
 
 #define OB_BS_THREADS 256
-#define OB_BS_PICK 1024                            // threads of the pick
 #define OB_BS_MAX_KEEP 64
 #define OB_BS_MAX_BEAMS 32
 #define OB_BS_RANKED 1024                          // candidates that the pick ranks by counting
@@ -33,14 +32,6 @@ struct ObBsArgs {
     int *list_t;
     float *out_scores; int *out_beams, *out_tokens;      // [groups][keep]
 };
-
-__device__ __forceinline__ float ob_bs_exp(float d)              // e^d, d <= 0
-{
-    d = d < -1000.f ? -1000.f : d;                               // (-inf has no two parts; NaN stays)
-    const float hi = d * 1.44269502162933349609375f;             // log2 e = 1.44269502... + 1.925963033e-8
-    const float lo = __builtin_fmaf(d, 1.44269502162933349609375f, -hi) + d * 1.925963033500011e-8f;
-    return __builtin_amdgcn_exp2f(hi) * __builtin_fmaf(lo, 0.693147180559945f, 1.f);
-}
 
 __device__ __forceinline__ double ob_bs_wave_sum(double v)
 {
@@ -71,7 +62,7 @@ __device__ __forceinline__ bool ob_bs_is_kth(const float *pub, int n, int keep, 
 
 // NV: pieces of 8 elements of a thread, OB_BS_THREADS apart
 template <typename T, int NV>
-__global__ __launch_bounds__(OB_BS_THREADS) void ob_bs_scan_kernel(const ObBsArgs A)
+__global__ __launch_bounds__(OB_BS_THREADS, NV == 1 ? 8 : 7) void ob_bs_scan_kernel(const ObBsArgs A)
 {
     __shared__ float red_m[4], pub[4 * (OB_BS_MAX_KEEP + 2)], t_s;
     __shared__ double red_s[4];
@@ -112,22 +103,29 @@ __global__ __launch_bounds__(OB_BS_THREADS) void ob_bs_scan_kernel(const ObBsArg
     const int64_t list = (int64_t)row * A.chunks + chunk;
     float *lx = A.list_x + list * room;
     int *lt = A.list_t + list * room;
-    if (best >= t && best > -INFINITY) {
+    const float least = fmaxf(t, -3.402823466e38f);                             // (-inf is no candidate)
+    if (best >= least) {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (x[j][e] >= t && x[j][e] > -INFINITY) {
+                if (x[j][e] >= least) {
                     const int at = atomicAdd(&n_s, 1);
                     if (at < room) { lx[at] = x[j][e]; lt[at] = c0 + 8 * (tid + OB_BS_THREADS * j) + e; }
                 }
     }
-    double s = 0.;
+    double s = 0.;                                                              // (a NaN makes the row's sum NaN, +inf as well)
+    if (m > -INFINITY) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+        for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            s += (double)(m == -INFINITY ? (x[j][e] == -INFINITY ? 0.f : x[j][e]) : ob_bs_exp(x[j][e] - m));        // (a NaN makes the row's sum NaN, +inf as well)
+            for (int e = 0; e < 8; ++e) s += (double)__builtin_amdgcn_exp2f((x[j][e] - m) * 1.44269504f);
+    } else {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s += x[j][e] == -INFINITY ? 0. : (double)x[j][e];
+    }
     s = ob_bs_wave_sum(s);
     if (lane == 0) red_s[wave] = s;
     __syncthreads();
@@ -178,9 +176,13 @@ __device__ __forceinline__ bool ob_bs_before(const ObBsCand &a, const ObBsCand &
     return a.x != b.x ? a.x > b.x : a.tok < b.tok;
 }
 
-__global__ __launch_bounds__(OB_BS_PICK) void ob_bs_pick_kernel(const ObBsArgs A)
+#define OB_BS_PLACES 8                                                            // candidate places of a thread of the pick that stay in registers
+
+// THREADS: 256 or 1024
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void ob_bs_pick_kernel(const ObBsArgs A)
 {
-    constexpr int WAVES = OB_BS_PICK / 64, NS = 8;                                // candidate places of a thread that stay in registers
+    constexpr int WAVES = THREADS / 64, NS = OB_BS_PLACES;
     __shared__ double row_v[OB_BS_MAX_BEAMS], cand_v[OB_BS_RANKED];               // lse of a beam; NaN: it offers nothing
     __shared__ float pub[WAVES * (OB_BS_MAX_KEEP + 2)], t_s;
     __shared__ ObBsCand cand[OB_BS_RANKED];
@@ -206,7 +208,7 @@ __global__ __launch_bounds__(OB_BS_PICK) void ob_bs_pick_kernel(const ObBsArgs A
     Place place[NS];
 #pragma unroll
     for (int k = 0; k < NS; ++k)
-        if (OB_BS_PICK * k < total) fetch(tid + OB_BS_PICK * k, place[k]);
+        if (THREADS * k < total) fetch(tid + THREADS * k, place[k]);
         else place[k] = {0.f, 0.f, 0, 0, 0, 0};
     for (int b = wave; b < A.beams; b += WAVES) {
         const double *sm = A.sums + (list0 + (int64_t)b * A.chunks) * 2;
@@ -225,7 +227,7 @@ __global__ __launch_bounds__(OB_BS_PICK) void ob_bs_pick_kernel(const ObBsArgs A
 #pragma unroll
         for (int k = 0; k < NS; ++k)
             if (value(place[k], c)) f(c);
-        for (int i = tid + OB_BS_PICK * NS; i < total; i += OB_BS_PICK) {
+        for (int i = tid + THREADS * NS; i < total; i += THREADS) {
             Place p;
             fetch(i, p);
             if (value(p, c)) f(c);
@@ -251,14 +253,14 @@ __global__ __launch_bounds__(OB_BS_PICK) void ob_bs_pick_kernel(const ObBsArgs A
     const int64_t out = (int64_t)group * A.keep;
     const auto put = [&](int k, const ObBsCand &c) { A.out_scores[out + k] = (float)c.v; A.out_beams[out + k] = c.beam; A.out_tokens[out + k] = c.tok; };
     if (n <= OB_BS_RANKED) {
-        if (tid < n) {
-            const ObBsCand c = cand[tid];
+        for (int i = tid; i < n; i += THREADS) {
+            const ObBsCand c = cand[i];
             int rank = 0;
 #pragma unroll 4
             for (int k = 0; k < n; ++k) {
                 const double v = cand_v[k];
                 rank += v > c.v;
-                if (v == c.v && k != tid) rank += ob_bs_before(cand[k], c);
+                if (v == c.v && k != i) rank += ob_bs_before(cand[k], c);
             }
             if (rank < A.keep) put(rank, c);
         }
@@ -270,7 +272,7 @@ __global__ __launch_bounds__(OB_BS_PICK) void ob_bs_pick_kernel(const ObBsArgs A
             __syncthreads();
             cand[tid] = b;
             __syncthreads();
-            for (int h = OB_BS_PICK / 2; h; h >>= 1) {
+            for (int h = THREADS / 2; h; h >>= 1) {
                 if (tid < h && ob_bs_before(cand[tid + h], cand[tid])) cand[tid] = cand[tid + h];
                 __syncthreads();
             }

@@ -217,7 +217,8 @@ extern "C" int onebit_beam_select(const void *logits, int64_t ld, int dtype, con
         if (p.nv == 1) hipLaunchKernelGGL((ob_bs_scan_kernel<float, 1>), grid, block, 0, s, a);
         else hipLaunchKernelGGL((ob_bs_scan_kernel<float, 4>), grid, block, 0, s, a);
     }
-    hipLaunchKernelGGL(ob_bs_pick_kernel, dim3((unsigned)groups), dim3(OB_BS_PICK), 0, s, a);
+    if ((int64_t)beams * p.chunks * ob_bs_list(keep) <= 256 * OB_BS_PLACES) hipLaunchKernelGGL((ob_bs_pick_kernel<256>), dim3((unsigned)groups), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((ob_bs_pick_kernel<1024>), dim3((unsigned)groups), dim3(1024), 0, s, a);
     return ob_launch_status("beam_select");
 }
 
