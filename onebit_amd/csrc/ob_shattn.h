@@ -8,7 +8,8 @@
 //                        keys in one launch; the last workgroup to arrive at a row joins its parts
 //   ob_sh_wide_kernel    many: parts of the prefixes, up to 128 queries of a group at a time, then
 //   ob_sh_own_kernel     the rows' own keys, started from the prefix's parts: the outputs, or, where a row's own keys are split as well, parts
-//                        again, which ob_sh_join_kernel joins.  Where a prefix is so short that every row may read it again, this kernel does, alone
+//                        again, which ob_sh_join_kernel joins.  Where a prefix is so short that every row may read it again, this kernel does, alone.
+//                        Where the rows' own keys are the larger share, their workgroups run among the wide kernel's and leave parts
 // Parts are joined in their order, whoever does it: deterministic.
 //
 // Both products are computed transposed, S^T = K Q^T and O^T = V^T P^T (MFMA 16x16x32): a lane holds 4 consecutive keys of one query
@@ -40,6 +41,7 @@ struct ObShArgs {
     int own_mb, max_own;                              // query blocks per row and kv head; most own positions
     int inline_prefix;                                // the own kernel reads the prefixes itself
     int one_items;                                    // ob_sh_one_kernel: items of the prefixes, in front of the rows'
+    int own_blocks;                                   // ob_sh_wide_kernel: workgroups of the rows' own keys among its others
     int *tickets;                                     // [rows][Hkv] arrivals at a row, zero between launches
     float scale_log2e;                                // log2(e) / sqrt(D)
     int n_groups;
@@ -285,13 +287,23 @@ __device__ __forceinline__ void ob_sh_store(const ObShArgs &A, const ObShWave<DP
     }
 }
 
+// own keys of a row (0: none), false for an idle row
+__device__ __forceinline__ bool ob_sh_row(const ObShArgs &A, int row, int first, int &slot, int &own)
+{
+    slot = A.row_slot ? A.row_slot[row] : row;
+    const int pos = A.row_pos[row];
+    if (slot < 0 || slot >= A.n_slots || pos < 0 || pos >= A.max_len) return false;
+    own = max(0, min(pos + 1 - first, A.max_own));
+    return true;
+}
+
 // a prefix item: kv head kvh, keys k0 .. k1 - 1 of the group's prefix (rows from kb, vb on), chunk and block of `per` queries
 struct ObShItem { int kvh, chunk, qi0, k0, k1; const _Float16 *kb, *vb; };
-__device__ __forceinline__ ObShItem ob_sh_item(const ObShArgs &A, int per, ObShGroup &G)
+__device__ __forceinline__ ObShItem ob_sh_item(const ObShArgs &A, int block, int per, ObShGroup &G)
 {
     ObShItem I;
-    const int item = blockIdx.x / A.Hkv;
-    I.kvh = blockIdx.x - item * A.Hkv;
+    const int item = block / A.Hkv;
+    I.kvh = block - item * A.Hkv;
     int gi = 0;
     while (item >= A.g[gi].item_end) ++gi;
     G = A.g[gi];
@@ -309,12 +321,9 @@ __device__ __forceinline__ ObShItem ob_sh_item(const ObShArgs &A, int per, ObShG
 // More queries: the four waves share the queries out, 16 MT each, over tiles of 64 keys and values that they read from the LDS together (two tiles there,
 // a third on its way in registers; one barrier a tile).
 template <int DP, int MT, bool EXACT>
-__global__ __launch_bounds__(OB_SH_THREADS, 2) void ob_sh_wide_kernel(const ObShArgs A)
+__device__ __forceinline__ void ob_sh_wide(const ObShArgs &A, const ObShItem &I, const ObShGroup &G, _Float16 (*kv)[2][64 * DP])
 {
     constexpr int DK = DP / 32, PPR = DP / 8, NP = 64 * PPR / OB_SH_THREADS, RPL = OB_SH_THREADS / PPR;      // pieces of a thread, rows apart
-    __shared__ __attribute__((aligned(16))) _Float16 kv[2][2][64 * DP];
-    ObShGroup G;
-    const ObShItem I = ob_sh_item(A, 64 * MT, G);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, g = lane >> 4;
     const int D = EXACT ? DP : A.D, qi0 = I.qi0 + 16 * MT * wave, nq = G.n * A.rep;
     ObShWave<DP, MT, EXACT> W;
@@ -365,14 +374,29 @@ __global__ __launch_bounds__(OB_SH_THREADS, 2) void ob_sh_wide_kernel(const ObSh
     ob_sh_store<DP, MT, EXACT>(A, W, G.row0, qi0, nq, I.kvh, I.chunk);
 }
 
-// own keys of a row (0: none), false for an idle row
-__device__ __forceinline__ bool ob_sh_row(const ObShArgs &A, int row, int first, int &slot, int &own)
+template <int DP, int MT, bool EXACT>
+__global__ __launch_bounds__(OB_SH_THREADS, 2) void ob_sh_wide_kernel(const ObShArgs A)
 {
-    slot = A.row_slot ? A.row_slot[row] : row;
-    const int pos = A.row_pos[row];
-    if (slot < 0 || slot >= A.n_slots || pos < 0 || pos >= A.max_len) return false;
-    own = max(0, min(pos + 1 - first, A.max_own));
-    return true;
+    __shared__ __attribute__((aligned(16))) _Float16 kv[2][2][64 * DP];
+    const int before = (int)((long long)blockIdx.x * A.own_blocks / gridDim.x);
+    if ((int)((long long)(blockIdx.x + 1) * A.own_blocks / gridDim.x) == before) {
+        ObShGroup G;
+        const ObShItem I = ob_sh_item(A, blockIdx.x - before, 64 * MT, G);
+        ob_sh_wide<DP, MT, EXACT>(A, I, G, kv);
+        return;
+    }
+    const int item = before / A.Hkv, kvh = before - item * A.Hkv;
+    const int at = item / A.rows, r = A.row_base + item - at * A.rows, split = at / A.own_mb, mb = at - split * A.own_mb;
+    int gi = 0, slot, own;
+    while (r >= A.g[gi].row0 + A.g[gi].n) ++gi;
+    const int first = A.g[gi].first;
+    if (!ob_sh_row(A, r, first, slot, own) || split * A.ochunk >= own) return;
+    const int64_t row = ((int64_t)slot * A.Hkv + kvh) * A.max_len * A.D;
+    ObShWave<DP, 1, EXACT> W;
+    W.init(A, r, 16 * mb, A.rep, kvh);
+    ob_sh_sweep<DP, 1, EXACT>(A, {A.k + row, A.v + row, first + split * A.ochunk, first + min(own, (split + 1) * A.ochunk)}, {A.k + row, A.v + row, 0, 0}, W,
+                              reinterpret_cast<float *>(kv), [](auto &) {});
+    if (threadIdx.x < 64) ob_sh_store<DP, 1, EXACT>(A, W, r, 16 * mb, A.rep, kvh, A.psplits + split);
 }
 
 // One row's queries of a kv head (16 of them: block mb) over its own keys.  osplits 0: all of them, started from the prefix's parts (the waves take
@@ -515,7 +539,7 @@ __global__ __launch_bounds__(OB_SH_THREADS, 2) void ob_sh_one_kernel(const ObShA
     int row0, r_lo, r_hi, kvh, chunks, per, first, n_query;              // rows that this workgroup holds queries of
     if ((int)blockIdx.x < A.one_items * A.Hkv) {
         ObShGroup G;
-        const ObShItem I = ob_sh_item(A, 16 * MT, G);
+        const ObShItem I = ob_sh_item(A, blockIdx.x, 16 * MT, G);
         ObShWave<DP, MT, EXACT> W;
         n_query = G.n * A.rep;
         W.init(A, G.row0, I.qi0, n_query, I.kvh);

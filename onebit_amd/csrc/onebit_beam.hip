@@ -19,7 +19,7 @@ static const int64_t OB_SH_MAX_LEN = 1 << 30;         // (positions and their ch
 // ------------------------------------------------------------------------------------------- attention over a shared prefix --
 // form: ob_sh_one_kernel; ob_sh_wide_kernel of 64 / 128 queries and ob_sh_own_kernel; the latter alone.  osplits 0: a row's own keys are one chunk, no part
 enum { OB_SH_INLINE, OB_SH_ONE, OB_SH_WIDE64, OB_SH_WIDE128 };
-struct ObShPlan { int form, per, pchunk, ochunk, psplits, osplits, own_mb; };
+struct ObShPlan { int form, per, pchunk, ochunk, psplits, osplits, own_mb; bool among; };
 #define OB_SH_TICKETS 16384                           // their place in front of the scratch memory does not depend on a call's sizes
 
 static ObShPlan ob_sh_plan(const onebit_prefix_t *groups, int32_t n_groups, int64_t rows, int32_t n_heads, int32_t n_kv_heads, int64_t max_own)
@@ -44,9 +44,10 @@ static ObShPlan ob_sh_plan(const onebit_prefix_t *groups, int32_t n_groups, int6
     }
     p.form = most <= 16 && rows * n_kv_heads <= OB_SH_TICKETS && own <= 1024 ? OB_SH_ONE : most <= 64 ? OB_SH_WIDE64 : OB_SH_WIDE128;
     p.per = p.form == OB_SH_ONE ? 16 : p.form == OB_SH_WIDE64 ? 64 : 128;
-    if (p.form == OB_SH_ONE) p.osplits = std::max(p.osplits, 1);
-    else if (p.osplits <= 1) p.osplits = 0;
     for (int i = 0; i < n_groups; ++i) work += ob_up(groups[i].n * rep, p.per) * groups[i].len * n_kv_heads;
+    p.among = p.form != OB_SH_ONE && own * max_own >= work;
+    if (p.form == OB_SH_ONE || p.among) p.osplits = std::max(p.osplits, 1);
+    else if (p.osplits <= 1) p.osplits = 0;
     p.pchunk = (int)(128 * std::max<int64_t>(p.form == OB_SH_ONE ? 1 : 2, ob_up(work, (p.form == OB_SH_ONE ? 256 : 512) * 128)));
     p.psplits = (int)ob_up(longest, p.pchunk);
     return p;
@@ -80,18 +81,21 @@ extern "C" size_t onebit_attention_shared_scratch_bytes(const onebit_prefix_t *g
 }
 
 template <int DP, bool EXACT>
-static void ob_sh_launch(const ObShArgs &a, int form, int64_t prefix_items, int64_t own_items, hipStream_t s)
+static void ob_sh_launch(ObShArgs &a, const ObShPlan &p, int64_t prefix_items, int64_t own_items, hipStream_t s)
 {
-    const dim3 block(OB_SH_THREADS), pg((unsigned)(prefix_items * a.Hkv)), og((unsigned)(own_items * a.Hkv)), all(pg.x + og.x);
-    if (form == OB_SH_ONE) hipLaunchKernelGGL((ob_sh_one_kernel<DP, 1, EXACT>), all, block, 0, s, a);
-    else {
-        if (prefix_items > 0) {
-            if (form == OB_SH_WIDE64) hipLaunchKernelGGL((ob_sh_wide_kernel<DP, 1, EXACT>), pg, block, 0, s, a);
-            else hipLaunchKernelGGL((ob_sh_wide_kernel<DP, 2, EXACT>), pg, block, 0, s, a);
-        }
-        hipLaunchKernelGGL((ob_sh_own_kernel<DP, EXACT>), og, block, 0, s, a);
-        if (a.osplits) hipLaunchKernelGGL(ob_sh_join_kernel, dim3((unsigned)ob_up((int64_t)a.rows * a.H, OB_SH_THREADS / 64)), block, 0, s, a);
+    const dim3 block(OB_SH_THREADS), own((unsigned)(own_items * a.Hkv)), all((unsigned)((prefix_items + own_items) * a.Hkv));
+    if (p.form == OB_SH_ONE) {
+        hipLaunchKernelGGL((ob_sh_one_kernel<DP, 1, EXACT>), all, block, 0, s, a);
+        return;
     }
+    a.own_blocks = p.among ? (int)own.x : 0;
+    const dim3 wide(p.among ? all.x : all.x - own.x);
+    if (wide.x > 0) {
+        if (p.form == OB_SH_WIDE64) hipLaunchKernelGGL((ob_sh_wide_kernel<DP, 1, EXACT>), wide, block, 0, s, a);
+        else if (p.form == OB_SH_WIDE128) hipLaunchKernelGGL((ob_sh_wide_kernel<DP, 2, EXACT>), wide, block, 0, s, a);
+    }
+    if (!p.among) hipLaunchKernelGGL((ob_sh_own_kernel<DP, EXACT>), own, block, 0, s, a);
+    if (a.osplits) hipLaunchKernelGGL(ob_sh_join_kernel, dim3((unsigned)ob_up((int64_t)a.rows * a.H, OB_SH_THREADS / 64)), block, 0, s, a);
 }
 
 extern "C" int onebit_attention_shared_rows(const void *q, const void *prefix_k, const void *prefix_v, const void *k_cache, const void *v_cache, void *o,
@@ -147,10 +151,10 @@ extern "C" int onebit_attention_shared_rows(const void *q, const void *prefix_k,
         a.one_items = (int)items;
         if ((items + own_items) * n_kv_heads > OB_MAX_WGS) return ob_fail(ONEBIT_E_ARG, "attention_shared_rows: too many workgroups");
         hipStream_t s = (hipStream_t)stream;
-        if (head_dim == 128) ob_sh_launch<128, true>(a, p.form, items, own_items, s);
-        else if (head_dim == 64) ob_sh_launch<64, true>(a, p.form, items, own_items, s);
-        else if (head_dim > 64) ob_sh_launch<128, false>(a, p.form, items, own_items, s);
-        else ob_sh_launch<64, false>(a, p.form, items, own_items, s);
+        if (head_dim == 128) ob_sh_launch<128, true>(a, p, items, own_items, s);
+        else if (head_dim == 64) ob_sh_launch<64, true>(a, p, items, own_items, s);
+        else if (head_dim > 64) ob_sh_launch<128, false>(a, p, items, own_items, s);
+        else ob_sh_launch<64, false>(a, p, items, own_items, s);
         const int rc2 = ob_launch_status("attention_shared_rows");
         if (rc2) return rc2;
     }

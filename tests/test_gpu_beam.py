@@ -111,6 +111,15 @@ def test_own_positions(own):
     _check(c := _case([50, 0], [2, 2], [own, max(own - 1, 0), own, 3], 4, 4, 128, seed=own), _call(c, max_own=max(own, 3)))
 
 
+@pytest.mark.parametrize("H, hkv, rows, length, own", [(8, 8, 40, 100, 300), (16, 2, 20, 200, 300), (16, 2, 5, 300, 900), (16, 2, 5, 5000, 900), (64, 2, 9, 700, 1),
+                                                       (4, 4, 64, 3000, 20), (24, 1, 7, 2100, 130), (2, 2, 64, 0, 200), (8, 1, 3, 4000, 600)])
+def test_many_queries_and_long_own_positions(H, hkv, rows, length, own):
+    """16, 64 and 128 queries a workgroup; own positions that outweigh the prefix, that are split, that are few."""
+    lens, n = [length, length // 3], [rows - 1, 1]
+    own = [1 + (own * ((7 * r) % rows)) // rows for r in range(rows - 1)] + [own]
+    _check(c := _case(lens, n, own, H, hkv, 128 if H != 24 else 72, seed=rows, idle=(1,)), _call(c))
+
+
 @pytest.mark.parametrize("one_cache", [False, True])
 def test_ragged_groups_and_idle_rows(one_cache):
     lens, rows = [515, 64, 0, 1, 130], [5, 1, 3, 2, 4]
@@ -161,6 +170,9 @@ def test_output_scaling():
     c = _case([70], [3], [5, 1, 20], 4, 4, 64, seed=9)
     h = torch.rand(4 * 64, device="cuda").to(F16) + 0.5
     assert torch.equal(_call(c, h_next=h), _call(c) * h.view(4, 64))
+    for rows, length, own in ((3, 500, 20), (40, 500, 20), (40, 50, 200), (40, 5000, 600)):          # every form writes its outputs itself
+        c = _case([length], [rows], [own] * rows, 4, 4, 64, seed=rows)
+        assert torch.equal(_call(c, h_next=h), _call(c) * h.view(4, 64))
 
 
 def test_large_scores_and_one_far_maximum():
