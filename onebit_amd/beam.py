@@ -138,8 +138,8 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: Optional[torch.Tensor], p
 
 
 def beam_select_workspace(rows: int, vocab: int, keep: int, device="cuda") -> torch.Tensor:
-    """Scratch memory for ``beam_select`` calls of these sizes."""
-    return torch.empty(max(int(_lib.load().onebit_beam_select_scratch_bytes(rows, vocab, keep)), 1), dtype=torch.uint8, device=device)
+    """Scratch memory for ``beam_select`` calls of these sizes and smaller ones: zero-filled once, every call leaves its counters at zero."""
+    return torch.zeros(max(int(_lib.load().onebit_beam_select_scratch_bytes(rows, vocab, keep)), 1), dtype=torch.uint8, device=device)
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, keep: int,

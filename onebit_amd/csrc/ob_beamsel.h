@@ -3,7 +3,8 @@
 // continuations are wanted in the order (v descending, beam, x descending, token).  v is a sum in 64 bits: two beams' values often lie closer
 // than fp32 resolves, while within a row the logits themselves order.
 //   ob_bs_scan_kernel   (row, chunk of the vocabulary): max and sum e^{x - max} of the chunk, and a list of candidates that holds its `keep` best
-//   ob_bs_pick_kernel   (group): the rows' sums joined, then the `keep` best of the lists
+//   ob_bs_pick          (group): the rows' sums joined, then the `keep` best of the lists; a launch of its own, or, where the scan is small, by the scan's
+//                       last workgroup to arrive at the group
 // Both find the best by a threshold instead of one after the other: every wave publishes the largest of its lanes' largest values, its share of `keep` and
 // two more; at least `keep` candidates reach the keep-th of all published, and few more do; those are listed (the scan) or ranked by counting (the
 // pick).  Where too many reach it (rows of equal logits), the best are taken one after the other.
@@ -11,12 +12,13 @@
 // term, with either sign; terms are added in 64 bits.  A row's elements belong to threads by their index alone, not by the row's alignment: equal rows
 // have equal sums, bit for bit.
 #pragma once
+#include <type_traits>
 #include "ob_common.h"
 
 #define OB_BS_THREADS 256
 #define OB_BS_MAX_KEEP 64
 #define OB_BS_MAX_BEAMS 32
-#define OB_BS_RANKED 1024                          // candidates that the pick ranks by counting
+#define OB_BS_TICKETS 4096                         // groups whose pick may be the scan's: counters in front of the scratch memory, zero between launches
 
 // room for the candidates of a chunk
 static inline __host__ __device__ int ob_bs_list(int keep) { return keep + keep / 2 + 16; }
@@ -31,13 +33,46 @@ struct ObBsArgs {
     float *list_x;                   // [rows][chunks][ob_bs_list(keep)]
     int *list_t;
     float *out_scores; int *out_beams, *out_tokens;      // [groups][keep]
+    int *tickets;
 };
 
+// what a later launch reads, or (AGENT) another workgroup of this one: past the XCD's L2
+template <bool AGENT, typename V> __device__ __forceinline__ void ob_bs_put(V *p, V v)
+{
+    if (AGENT) __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    else *p = v;
+}
+template <bool AGENT, typename V> __device__ __forceinline__ V ob_bs_get(const V *p) { return AGENT ? __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : *p; }
+
+template <int CTRL, int ROWS> __device__ __forceinline__ double ob_bs_dpp(double v)
+{
+    const ob_u32x2 u = __builtin_bit_cast(ob_u32x2, v);
+    const ob_u32x2 o = {(uint32_t)__builtin_amdgcn_update_dpp(0, (int)u[0], CTRL, ROWS, 0xF, false), (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u[1], CTRL, ROWS, 0xF, false)};
+    return __builtin_bit_cast(double, o);
+}
+// sums over 16 lanes, in every one of them, and over the wave, on the DPP network (as ob_wave_sum)
+__device__ __forceinline__ double ob_bs_row_sum(double v)
+{
+    v += ob_bs_dpp<0xB1, 0xF>(v);
+    v += ob_bs_dpp<0x4E, 0xF>(v);
+    v += ob_bs_dpp<0x141, 0xF>(v);
+    return v + ob_bs_dpp<0x140, 0xF>(v);
+}
 __device__ __forceinline__ double ob_bs_wave_sum(double v)
 {
-#pragma unroll
-    for (int k = 32; k; k >>= 1) v += __shfl_xor(v, k, 64);
-    return v;
+    v = ob_bs_row_sum(v);
+    v += ob_bs_dpp<0x142, 0xA>(v);
+    v += ob_bs_dpp<0x143, 0xC>(v);
+    const ob_u32x2 u = __builtin_bit_cast(ob_u32x2, v);
+    const ob_u32x2 t = {(uint32_t)__builtin_amdgcn_readlane((int)u[0], 63), (uint32_t)__builtin_amdgcn_readlane((int)u[1], 63)};
+    return __builtin_bit_cast(double, t);
+}
+__device__ __forceinline__ float ob_bs_row_max(float v)
+{
+    v = fmaxf(v, OB_DPP_F(v, 0xB1, 0xF));
+    v = fmaxf(v, OB_DPP_F(v, 0x4E, 0xF));
+    v = fmaxf(v, OB_DPP_F(v, 0x141, 0xF));
+    return fmaxf(v, OB_DPP_F(v, 0x140, 0xF));
 }
 
 // the k largest of the lanes' values (equal ones one by one; -inf where there are fewer), in order, to out
@@ -60,9 +95,142 @@ __device__ __forceinline__ bool ob_bs_is_kth(const float *pub, int n, int keep, 
     return rank == keep - 1;
 }
 
-// NV: pieces of 8 elements of a thread, OB_BS_THREADS apart
-template <typename T, int NV>
-__global__ __launch_bounds__(OB_BS_THREADS, NV == 1 ? 8 : 7) void ob_bs_scan_kernel(const ObBsArgs A)
+// candidate a in front of candidate b?  (value, beam, logit, token)
+struct ObBsCand { double v; float x; int beam, tok; };
+__device__ __forceinline__ bool ob_bs_before(const ObBsCand &a, const ObBsCand &b)
+{
+    if (a.v != b.v) return a.v > b.v;
+    if (a.beam != b.beam) return a.beam < b.beam;
+    return a.x != b.x ? a.x > b.x : a.tok < b.tok;
+}
+
+#define OB_BS_PLACES 8                                                            // candidate places of a thread of the pick that stay in registers
+
+// THREADS: 256 or 1024
+template <int THREADS, bool AGENT>
+__device__ __forceinline__ void ob_bs_pick(const ObBsArgs &A, int group)
+{
+    constexpr int WAVES = THREADS / 64, NS = OB_BS_PLACES, RANKED = THREADS;       // candidates that are ranked by counting
+    __shared__ double row_v[OB_BS_MAX_BEAMS], cand_v[RANKED];                     // lse of a beam; NaN: it offers nothing
+    __shared__ float pub[WAVES * (OB_BS_MAX_KEEP + 2)], t_s;
+    __shared__ ObBsCand cand[RANKED];
+    __shared__ int n_s;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int room = ob_bs_list(A.keep), total = A.beams * A.chunks * room;
+    const int64_t list0 = (int64_t)group * A.beams * A.chunks;
+    if (tid == 0) { n_s = 0; t_s = -INFINITY; }
+    struct Place { float x, score; int tok, n, beam, e; };
+    const auto fetch = [&](int i, Place &p) {                                    // (all of it at once: what lies behind a list's end is memory of the list, not used)
+        const int l = min(i, total - 1) / room;
+        p.e = i < total ? i - l * room : 0x7fffffff;
+        p.beam = l / A.chunks;
+        p.n = ob_bs_get<AGENT>(A.counts + list0 + l);
+        p.x = ob_bs_get<AGENT>(A.list_x + list0 * room + min(i, total - 1));
+        p.tok = ob_bs_get<AGENT>(A.list_t + list0 * room + min(i, total - 1));
+        p.score = A.scores[group * A.beams + p.beam];
+    };
+    const auto value = [&](const Place &p, ObBsCand &c) -> bool {                // false where there is no candidate
+        c = {(double)p.score + ((double)p.x - row_v[p.beam]), p.x, p.beam, p.tok};
+        return p.e < p.n && c.v > -INFINITY;                                     // (NaN: none)
+    };
+    Place place[NS];
+#pragma unroll
+    for (int k = 0; k < NS; ++k)
+        if (THREADS * k < total) fetch(tid + THREADS * k, place[k]);
+        else place[k] = {0.f, 0.f, 0, 0, 0, 0};
+    // a chunk's sum in terms of the row's largest logit
+    const auto term = [](double m, double part, float M) { return m == -INFINITY ? part : part * exp(m - (double)M); };
+    if (A.chunks <= 16)                                                          // a row of 16 lanes for a beam
+        for (int b0 = 4 * wave; b0 < A.beams; b0 += 4 * WAVES) {
+            const int b = b0 + (lane >> 4), c = lane & 15;
+            const bool in = b < A.beams && c < A.chunks;
+            const double *sm = A.sums + (list0 + (int64_t)min(b, A.beams - 1) * A.chunks + min(c, A.chunks - 1)) * 2;
+            const double m = ob_bs_get<AGENT>(sm), part = ob_bs_get<AGENT>(sm + 1);
+            const float M = ob_bs_row_max(in ? (float)m : -INFINITY);
+            const double s = ob_bs_row_sum(in ? term(m, part, M) : 0.);
+            if (b < A.beams && c == 0) row_v[b] = (double)M + log(s);
+        }
+    else
+        for (int b = wave; b < A.beams; b += WAVES) {
+            const double *sm = A.sums + (list0 + (int64_t)b * A.chunks) * 2;
+            float M = -INFINITY;                                                 // (a logit)
+            for (int c = lane; c < A.chunks; c += 64) M = fmaxf(M, (float)ob_bs_get<AGENT>(sm + 2 * c));
+            M = ob_wave_max(M);
+            double s = 0.;
+            for (int c = lane; c < A.chunks; c += 64) s += term(ob_bs_get<AGENT>(sm + 2 * c), ob_bs_get<AGENT>(sm + 2 * c + 1), M);
+            s = ob_bs_wave_sum(s);
+            if (lane == 0) row_v[b] = (double)M + log(s);
+        }
+    __syncthreads();
+    // f over all candidate places of this thread
+    const auto each = [&](auto f) {
+        ObBsCand c;
+#pragma unroll
+        for (int k = 0; k < NS; ++k)
+            if (value(place[k], c)) f(c);
+        for (int i = tid + THREADS * NS; i < total; i += THREADS) {
+            Place p;
+            fetch(i, p);
+            if (value(p, c)) f(c);
+        }
+    };
+    float best = -INFINITY;
+    each([&](const ObBsCand &c) { best = fmaxf(best, __double2float_rd(c.v)); });      // (rounded down: what reaches the threshold reaches it in 64 bits, too)
+    const int waves = min(WAVES, (total + 63) / 64), share = min(64, (A.keep + waves - 1) / waves + 2);
+    if (wave < waves) ob_bs_publish(best, share, pub + wave * share);
+    __syncthreads();
+    if (ob_bs_is_kth(pub, waves * share, A.keep, tid)) t_s = pub[tid];
+    __syncthreads();
+    const double t = t_s;
+    if (best >= t_s)
+        each([&](const ObBsCand &c) {
+            if (c.v >= t) {
+                const int k = atomicAdd(&n_s, 1);
+                if (k < RANKED) { cand_v[k] = c.v; cand[k] = c; }
+            }
+        });
+    __syncthreads();
+    int n = n_s;
+    const int64_t out = (int64_t)group * A.keep;
+    const auto put = [&](int k, const ObBsCand &c) { A.out_scores[out + k] = (float)c.v; A.out_beams[out + k] = c.beam; A.out_tokens[out + k] = c.tok; };
+    if (n <= RANKED) {
+        for (int i = tid; i < n; i += THREADS) {
+            const ObBsCand c = cand[i];
+            int rank = 0;
+#pragma unroll 4
+            for (int k = 0; k < n; ++k) {
+                const double v = cand_v[k];
+                rank += v > c.v;
+                if (v == c.v && k != i) rank += ob_bs_before(cand[k], c);
+            }
+            if (rank < A.keep) put(rank, c);
+        }
+    } else {                                                                     // one after the other: the best behind the last one
+        ObBsCand last = {INFINITY, INFINITY, -1, -1};
+        for (n = 0; n < A.keep; ++n) {
+            ObBsCand b = {-INFINITY, -INFINITY, 0x7fffffff, 0x7fffffff};
+            each([&](const ObBsCand &c) { if (ob_bs_before(last, c) && ob_bs_before(c, b)) b = c; });
+            __syncthreads();
+            cand[tid] = b;
+            __syncthreads();
+            for (int h = THREADS / 2; h; h >>= 1) {
+                if (tid < h && ob_bs_before(cand[tid + h], cand[tid])) cand[tid] = cand[tid + h];
+                __syncthreads();
+            }
+            last = cand[0];
+            if (last.v == -INFINITY) break;
+            if (tid == 0) put(n, last);
+        }
+    }
+    if (tid >= n && tid < A.keep) put(tid, {-INFINITY, 0.f, -1, -1});
+}
+
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void ob_bs_pick_kernel(const ObBsArgs A) { ob_bs_pick<THREADS, false>(A, blockIdx.x); }
+
+// NV: pieces of 8 elements of a thread, OB_BS_THREADS apart.  PICK: the last workgroup of a group picks
+template <typename T, int NV, bool PICK>
+__global__ __launch_bounds__(OB_BS_THREADS, PICK ? 4 : NV == 1 ? 8 : 7) void ob_bs_scan_kernel(const ObBsArgs A)
 {
     __shared__ float red_m[4], pub[4 * (OB_BS_MAX_KEEP + 2)], t_s;
     __shared__ double red_s[4];
@@ -111,7 +279,7 @@ __global__ __launch_bounds__(OB_BS_THREADS, NV == 1 ? 8 : 7) void ob_bs_scan_ker
             for (int e = 0; e < 8; ++e)
                 if (x[j][e] >= least) {
                     const int at = atomicAdd(&n_s, 1);
-                    if (at < room) { lx[at] = x[j][e]; lt[at] = c0 + 8 * (tid + OB_BS_THREADS * j) + e; }
+                    if (at < room) { ob_bs_put<PICK>(lx + at, x[j][e]); ob_bs_put<PICK>(lt + at, c0 + 8 * (tid + OB_BS_THREADS * j) + e); }
                 }
     }
     double s = 0.;                                                              // (a NaN makes the row's sum NaN, +inf as well)
@@ -131,6 +299,7 @@ __global__ __launch_bounds__(OB_BS_THREADS, NV == 1 ? 8 : 7) void ob_bs_scan_ker
     __syncthreads();
     int n = n_s;
     if (n > room) {                                                             // too many reach the threshold: one after the other
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                         // (over what is listed already)
         float px = INFINITY;
         int pt = -1;
         for (n = 0; n < A.keep; ++n) {
@@ -157,129 +326,24 @@ __global__ __launch_bounds__(OB_BS_THREADS, NV == 1 ? 8 : 7) void ob_bs_scan_ker
             for (int w2 = 0; w2 < 4; ++w2)
                 if (red_m[w2] == px) pt = min(pt, red_i[w2]);
             if (px == -INFINITY) break;
-            if (tid == 0) { lx[n] = px; lt[n] = pt; }
+            if (tid == 0) { ob_bs_put<PICK>(lx + n, px); ob_bs_put<PICK>(lt + n, pt); }
         }
     }
     if (tid == 0) {
-        A.sums[2 * list] = (double)m;
-        A.sums[2 * list + 1] = (red_s[0] + red_s[1]) + (red_s[2] + red_s[3]);
-        A.counts[list] = n;
+        ob_bs_put<PICK>(A.sums + 2 * list, (double)m);
+        ob_bs_put<PICK>(A.sums + 2 * list + 1, (red_s[0] + red_s[1]) + (red_s[2] + red_s[3]));
+        ob_bs_put<PICK>(A.counts + list, n);
     }
-}
-
-// candidate a in front of candidate b?  (value, beam, logit, token)
-struct ObBsCand { double v; float x; int beam, tok; };
-__device__ __forceinline__ bool ob_bs_before(const ObBsCand &a, const ObBsCand &b)
-{
-    if (a.v != b.v) return a.v > b.v;
-    if (a.beam != b.beam) return a.beam < b.beam;
-    return a.x != b.x ? a.x > b.x : a.tok < b.tok;
-}
-
-#define OB_BS_PLACES 8                                                            // candidate places of a thread of the pick that stay in registers
-
-// THREADS: 256 or 1024
-template <int THREADS>
-__global__ __launch_bounds__(THREADS) void ob_bs_pick_kernel(const ObBsArgs A)
-{
-    constexpr int WAVES = THREADS / 64, NS = OB_BS_PLACES;
-    __shared__ double row_v[OB_BS_MAX_BEAMS], cand_v[OB_BS_RANKED];               // lse of a beam; NaN: it offers nothing
-    __shared__ float pub[WAVES * (OB_BS_MAX_KEEP + 2)], t_s;
-    __shared__ ObBsCand cand[OB_BS_RANKED];
-    __shared__ int n_s;
-    const int group = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int room = ob_bs_list(A.keep), total = A.beams * A.chunks * room;
-    const int64_t list0 = (int64_t)group * A.beams * A.chunks;
-    if (tid == 0) { n_s = 0; t_s = -INFINITY; }
-    struct Place { float x, score; int tok, n, beam, e; };
-    const auto fetch = [&](int i, Place &p) {                                    // (all of it at once: what lies behind a list's end is memory of the list, not used)
-        const int l = min(i, total - 1) / room;
-        p.e = i < total ? i - l * room : 0x7fffffff;
-        p.beam = l / A.chunks;
-        p.n = A.counts[list0 + l];
-        p.x = A.list_x[list0 * room + min(i, total - 1)];
-        p.tok = A.list_t[list0 * room + min(i, total - 1)];
-        p.score = A.scores[group * A.beams + p.beam];
-    };
-    const auto value = [&](const Place &p, ObBsCand &c) -> bool {                // false where there is no candidate
-        c = {(double)p.score + ((double)p.x - row_v[p.beam]), p.x, p.beam, p.tok};
-        return p.e < p.n && c.v > -INFINITY;                                     // (NaN: none)
-    };
-    Place place[NS];
-#pragma unroll
-    for (int k = 0; k < NS; ++k)
-        if (THREADS * k < total) fetch(tid + THREADS * k, place[k]);
-        else place[k] = {0.f, 0.f, 0, 0, 0, 0};
-    for (int b = wave; b < A.beams; b += WAVES) {
-        const double *sm = A.sums + (list0 + (int64_t)b * A.chunks) * 2;
-        double M = -INFINITY, s = 0.;
-        for (int c = lane; c < A.chunks; c += 64) M = fmax(M, sm[2 * c]);
-#pragma unroll
-        for (int k = 32; k; k >>= 1) M = fmax(M, __shfl_xor(M, k, 64));
-        for (int c = lane; c < A.chunks; c += 64) s += sm[2 * c] == -INFINITY ? sm[2 * c + 1] : sm[2 * c + 1] * exp(sm[2 * c] - M);
-        s = ob_bs_wave_sum(s);
-        if (lane == 0) row_v[b] = M + log(s);
+    if constexpr (PICK) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                         // every wave: what it wrote has left
+        __syncthreads();
+        const int group = row / A.beams;
+        if (tid == 0) {
+            const int all = A.beams * A.chunks, last = __hip_atomic_fetch_add(A.tickets + group, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == all - 1;
+            if (last) __hip_atomic_store(A.tickets + group, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            n_s = last;
+        }
+        __syncthreads();
+        if (n_s) ob_bs_pick<OB_BS_THREADS, true>(A, group);
     }
-    __syncthreads();
-    // f over all candidate places of this thread
-    const auto each = [&](auto f) {
-        ObBsCand c;
-#pragma unroll
-        for (int k = 0; k < NS; ++k)
-            if (value(place[k], c)) f(c);
-        for (int i = tid + THREADS * NS; i < total; i += THREADS) {
-            Place p;
-            fetch(i, p);
-            if (value(p, c)) f(c);
-        }
-    };
-    float best = -INFINITY;
-    each([&](const ObBsCand &c) { best = fmaxf(best, __double2float_rd(c.v)); });      // (rounded down: what reaches the threshold reaches it in 64 bits, too)
-    const int waves = min(WAVES, (total + 63) / 64), share = min(64, (A.keep + waves - 1) / waves + 2);
-    if (wave < waves) ob_bs_publish(best, share, pub + wave * share);
-    __syncthreads();
-    if (ob_bs_is_kth(pub, waves * share, A.keep, tid)) t_s = pub[tid];
-    __syncthreads();
-    const double t = t_s;
-    if (best >= t_s)
-        each([&](const ObBsCand &c) {
-            if (c.v >= t) {
-                const int k = atomicAdd(&n_s, 1);
-                if (k < OB_BS_RANKED) { cand_v[k] = c.v; cand[k] = c; }
-            }
-        });
-    __syncthreads();
-    int n = n_s;
-    const int64_t out = (int64_t)group * A.keep;
-    const auto put = [&](int k, const ObBsCand &c) { A.out_scores[out + k] = (float)c.v; A.out_beams[out + k] = c.beam; A.out_tokens[out + k] = c.tok; };
-    if (n <= OB_BS_RANKED) {
-        for (int i = tid; i < n; i += THREADS) {
-            const ObBsCand c = cand[i];
-            int rank = 0;
-#pragma unroll 4
-            for (int k = 0; k < n; ++k) {
-                const double v = cand_v[k];
-                rank += v > c.v;
-                if (v == c.v && k != i) rank += ob_bs_before(cand[k], c);
-            }
-            if (rank < A.keep) put(rank, c);
-        }
-    } else {                                                                     // one after the other: the best behind the last one
-        ObBsCand last = {INFINITY, INFINITY, -1, -1};
-        for (n = 0; n < A.keep; ++n) {
-            ObBsCand b = {-INFINITY, -INFINITY, 0x7fffffff, 0x7fffffff};
-            each([&](const ObBsCand &c) { if (ob_bs_before(last, c) && ob_bs_before(c, b)) b = c; });
-            __syncthreads();
-            cand[tid] = b;
-            __syncthreads();
-            for (int h = THREADS / 2; h; h >>= 1) {
-                if (tid < h && ob_bs_before(cand[tid + h], cand[tid])) cand[tid] = cand[tid + h];
-                __syncthreads();
-            }
-            last = cand[0];
-            if (last.v == -INFINITY) break;
-            if (tid == 0) put(n, last);
-        }
-    }
-    if (tid >= n && tid < A.keep) put(tid, {-INFINITY, 0.f, -1, -1});
 }

@@ -171,22 +171,33 @@ static int ob_bs_check(int64_t groups, int32_t beams, int64_t vocab, int32_t kee
     return 0;
 }
 
-// pieces of 8 elements per thread, chunks of a row and pieces of a chunk (as even as they go)
-struct ObBsPlan { int nv, chunks, vecs; };
-static ObBsPlan ob_bs_plan(int64_t rows, int64_t vocab)
+// pieces of 8 elements per thread, chunks of a row and pieces of a chunk (as even as they go); fused: the scan's last workgroups pick
+struct ObBsPlan { int nv, chunks, vecs; bool fused; };
+static ObBsPlan ob_bs_plan(int64_t groups, int32_t beams, int64_t vocab, int32_t keep)
 {
-    const int64_t all = ob_up(vocab, 8);
+    const int64_t all = ob_up(vocab, 8), one = ob_up(all, OB_BS_THREADS), few = 256 * OB_BS_PLACES;
     ObBsPlan p;
-    p.nv = rows * ob_up(all, OB_BS_THREADS) > 2048 ? 4 : 1;
+    p.nv = groups * beams * one > 2048 || beams * one * ob_bs_list(keep) > few ? 4 : 1;
     p.chunks = (int)ob_up(all, p.nv * OB_BS_THREADS);
     p.vecs = (int)ob_up(all, p.chunks);
+    p.fused = groups <= OB_BS_TICKETS && groups * beams * p.chunks <= 1024 && (int64_t)beams * p.chunks * ob_bs_list(keep) <= few;
     return p;
 }
 
 extern "C" size_t onebit_beam_select_scratch_bytes(int64_t rows, int64_t vocab, int32_t keep)
 {
     if (rows <= 0 || vocab <= 0 || keep <= 0 || rows > 65535 || vocab > (1 << 20) || keep > OB_BS_MAX_KEEP) return 0;
-    return (size_t)rows * ob_bs_plan(rows, vocab).chunks * (16 + 4 + 8 * (size_t)ob_bs_list(keep)) + 256;
+    return OB_BS_TICKETS * 4 + (size_t)rows * ob_up(vocab, 8 * OB_BS_THREADS) * (16 + 4 + 8 * (size_t)ob_bs_list(keep));
+}
+
+template <typename T>
+static void ob_bs_scan(const ObBsArgs &a, const ObBsPlan &p, const dim3 &grid, const dim3 &block, hipStream_t s)
+{
+    if (p.fused) {
+        if (p.nv == 1) hipLaunchKernelGGL((ob_bs_scan_kernel<T, 1, true>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((ob_bs_scan_kernel<T, 4, true>), grid, block, 0, s, a);
+    } else if (p.nv == 1) hipLaunchKernelGGL((ob_bs_scan_kernel<T, 1, false>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((ob_bs_scan_kernel<T, 4, false>), grid, block, 0, s, a);
 }
 
 extern "C" int onebit_beam_select(const void *logits, int64_t ld, int dtype, const float *scores, int64_t groups, int32_t beams, int64_t vocab, int32_t keep,
@@ -202,27 +213,24 @@ extern "C" int onebit_beam_select(const void *logits, int64_t ld, int dtype, con
         return ob_fail(ONEBIT_E_ALIGN, "beam_select: misaligned pointer");
     const int64_t rows = groups * beams;
     const size_t need = onebit_beam_select_scratch_bytes(rows, vocab, keep);
-    if (!scratch || scratch_bytes < need || !ob_aligned(scratch, 16)) return ob_fail(ONEBIT_E_WSPACE, "beam_select: needs %zu bytes of 16-byte aligned scratch", need);
+    if (!scratch || scratch_bytes < need || !ob_aligned(scratch, 16)) return ob_fail(ONEBIT_E_WSPACE, "beam_select: needs %zu bytes of zero-initialised, 16-byte aligned scratch", need);
     ObBsArgs a = {};
-    const ObBsPlan p = ob_bs_plan(rows, vocab);
+    const ObBsPlan p = ob_bs_plan(groups, beams, vocab, keep);
     a.logits = logits; a.ld = ld; a.scores = scores; a.beams = beams; a.keep = keep; a.vocab = (int)vocab; a.chunks = p.chunks; a.vecs = p.vecs;
     const size_t lists = (size_t)rows * p.chunks;
-    a.sums = (double *)scratch;
+    a.tickets = (int *)scratch;
+    a.sums = (double *)(a.tickets + OB_BS_TICKETS);
     a.counts = (int *)(a.sums + 2 * lists);
     a.list_x = (float *)(a.counts + lists);
     a.list_t = (int *)(a.list_x + lists * ob_bs_list(keep));
     a.out_scores = out_scores; a.out_beams = out_beams; a.out_tokens = out_tokens;
     hipStream_t s = (hipStream_t)stream;
     const dim3 grid((unsigned)a.chunks, (unsigned)rows), block(OB_BS_THREADS);
-    if (dtype == ONEBIT_F16) {
-        if (p.nv == 1) hipLaunchKernelGGL((ob_bs_scan_kernel<_Float16, 1>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((ob_bs_scan_kernel<_Float16, 4>), grid, block, 0, s, a);
-    } else {
-        if (p.nv == 1) hipLaunchKernelGGL((ob_bs_scan_kernel<float, 1>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((ob_bs_scan_kernel<float, 4>), grid, block, 0, s, a);
-    }
-    if ((int64_t)beams * p.chunks * ob_bs_list(keep) <= 256 * OB_BS_PLACES) hipLaunchKernelGGL((ob_bs_pick_kernel<256>), dim3((unsigned)groups), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((ob_bs_pick_kernel<1024>), dim3((unsigned)groups), dim3(1024), 0, s, a);
+    if (dtype == ONEBIT_F16) ob_bs_scan<_Float16>(a, p, grid, block, s);
+    else ob_bs_scan<float>(a, p, grid, block, s);
+    const bool few = (int64_t)beams * p.chunks * ob_bs_list(keep) <= 256 * OB_BS_PLACES;
+    if (!p.fused && few) hipLaunchKernelGGL((ob_bs_pick_kernel<256>), dim3((unsigned)groups), dim3(256), 0, s, a);
+    else if (!p.fused) hipLaunchKernelGGL((ob_bs_pick_kernel<1024>), dim3((unsigned)groups), dim3(1024), 0, s, a);
     return ob_launch_status("beam_select");
 }
 

@@ -12,7 +12,7 @@ from typing import Dict, List, Optional, Sequence, Set, Tuple
 
 import torch
 
-from .beam import MAX_BEAMS, MAX_KEEP, beam_select, reorder_slots
+from .beam import MAX_BEAMS, MAX_KEEP, beam_select, beam_select_workspace, reorder_slots
 
 _PRIME_ROWS = 8192          # prompt tokens of one step, unless a single prompt has more
 
@@ -155,12 +155,13 @@ def beam_search(engine, prompts: Sequence[Sequence[int]], max_new_tokens: int, e
         raise ValueError("beam_search: prompt + max_new_tokens exceeds the engine's slots")
     lengths = [len(p) for p in prompts]
     keep = min(MAX_KEEP, (1 + max(1, len(eos or ()))) * W)
+    workspace = beam_select_workspace(B * W, engine.vocab, keep, engine.device)
     logits = engine.prime(prompts)
     engine.spread(lengths)
     states = [_Prompt(W, length_penalty, early_stopping) for _ in prompts]
     live, scores, per = list(range(B)), torch.zeros(B, device=engine.device), 1
     for step in range(max_new_tokens):
-        v, b, t = (x.tolist() for x in beam_select(logits, scores, per, keep))
+        v, b, t = (x.tolist() for x in beam_select(logits, scores, per, keep, workspace=workspace))
         moves, moved = [list(range(W)) for _ in range(B)], False
         for g, i in enumerate(live):
             moves[i] = states[i].take(list(zip(v[g], b[g], t[g])), eos)
