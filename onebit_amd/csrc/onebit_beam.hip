@@ -239,7 +239,6 @@ template <typename U>
 static void ob_re_launch(const ObReArgs &a, const dim3 &grid, hipStream_t s)
 {
     if (a.beams <= 4) hipLaunchKernelGGL((ob_re_kernel<4, U>), grid, dim3(OB_RE_THREADS), 0, s, a);
-    else if (a.beams <= 8) hipLaunchKernelGGL((ob_re_kernel<8, U>), grid, dim3(OB_RE_THREADS), 0, s, a);
     else if (a.beams <= 16) hipLaunchKernelGGL((ob_re_kernel<16, U>), grid, dim3(OB_RE_THREADS), 0, s, a);
     else hipLaunchKernelGGL((ob_re_kernel<32, U>), grid, dim3(OB_RE_THREADS), 0, s, a);
 }
