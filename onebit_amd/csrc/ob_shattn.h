@@ -473,11 +473,11 @@ __global__ __launch_bounds__(OB_SH_THREADS, 2) void ob_sh_own_kernel(const ObShA
     }
 }
 
-// A wave joins the n parts of (row, head), np of them the prefix's, in order, two output columns a lane
+// Half a wave joins the n parts of (row, head), np of them the prefix's, in order, four output columns a lane (n = 0: zeros)
 template <bool AGENT>
 __device__ __forceinline__ void ob_sh_join(const ObShArgs &A, int r, int head, int np, int n)
 {
-    const int lane = threadIdx.x & 63, d = 2 * lane;
+    const int d = 4 * (threadIdx.x & 31);
     if (d >= A.D) return;
     const int64_t p0 = ((int64_t)r * A.H + head) * (A.psplits + A.osplits);
     const auto two = [](const float *p) -> ob_float2 {
@@ -485,15 +485,16 @@ __device__ __forceinline__ void ob_sh_join(const ObShArgs &A, int r, int head, i
         return __builtin_bit_cast(ob_float2, __hip_atomic_load(reinterpret_cast<const unsigned long long *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
     };
     float M = OB_SH_NONE, l = 0.f;
-    ob_float2 o = {0.f, 0.f};
+    ob_float4 o = {0.f, 0.f, 0.f, 0.f};
     for (int s0 = 0; s0 < n; s0 += 8) {
-        ob_float2 ml[8], po[8];
+        ob_float2 ml[8], po[8][2];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int s = min(s0 + j, n - 1);
             const int64_t p = p0 + (s < np ? s : A.psplits + s - np);
             ml[j] = two(A.part_ml + 2 * p);
-            po[j] = two(A.part_o + p * A.D + d);
+            po[j][0] = two(A.part_o + p * A.D + d);
+            po[j][1] = two(A.part_o + p * A.D + d + 2);
         }
         float mb = M;
 #pragma unroll
@@ -505,26 +506,28 @@ __device__ __forceinline__ void ob_sh_join(const ObShArgs &A, int r, int head, i
             if (s0 + j < n) {
                 const float x = ob_sh_weight(ml[j][0], M);
                 l += x * ml[j][1];
-                o += x * po[j];
+                o += x * (ob_float4){po[j][0][0], po[j][0][1], po[j][1][0], po[j][1][1]};
             }
     }
-    _Float16 *out = A.o + ((int64_t)r * A.H + head) * A.D + d;
-    ob_half2 y = {(_Float16)(o[0] / l), (_Float16)(o[1] / l)};
-    if (A.h_next) { y[0] *= A.h_next[head * A.D + d]; y[1] *= A.h_next[head * A.D + d + 1]; }
-    *reinterpret_cast<ob_half2 *>(out) = y;
+    ob_half4 y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        y[i] = n ? (_Float16)(o[i] / l) : (_Float16)0;
+        if (A.h_next) y[i] *= A.h_next[head * A.D + d + i];
+    }
+    *reinterpret_cast<ob_half4 *>(A.o + ((int64_t)r * A.H + head) * A.D + d) = y;
 }
 
 __global__ __launch_bounds__(OB_SH_THREADS) void ob_sh_join_kernel(const ObShArgs A)
 {
-    const int w = blockIdx.x * (OB_SH_THREADS / 64) + (threadIdx.x >> 6);
+    const int w = blockIdx.x * (OB_SH_THREADS / 32) + (threadIdx.x >> 5);
     if (w >= A.rows * A.H) return;
     const int r = A.row_base + w / A.H, head = w % A.H;
     int gi = 0, slot, own;
     while (r >= A.g[gi].row0 + A.g[gi].n) ++gi;
     if (!ob_sh_row(A, r, A.g[gi].first, slot, own)) return;                       // idle: its output stays as it is
-    const int np = A.g[gi].chunks, n = np + (own + A.ochunk - 1) / A.ochunk;
-    if (n) ob_sh_join<false>(A, r, head, np, n);
-    else if (2 * (threadIdx.x & 63) < A.D) *reinterpret_cast<ob_half2 *>(A.o + ((int64_t)r * A.H + head) * A.D + 2 * (threadIdx.x & 63)) = (ob_half2)(_Float16)0;
+    const int np = A.g[gi].chunks;
+    ob_sh_join<false>(A, r, head, np, np + (own + A.ochunk - 1) / A.ochunk);
 }
 
 // One launch: the items of the prefixes (up to 16 MT queries of a group), then those of the rows' own keys.  A workgroup publishes its part WRITE-THROUGH
@@ -578,25 +581,15 @@ __global__ __launch_bounds__(OB_SH_THREADS, 2) void ob_sh_one_kernel(const ObShA
                 int *t = A.tickets + (int64_t)r * A.Hkv + kvh;
                 last = __hip_atomic_fetch_add(t, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == all - 1;
                 if (last) __hip_atomic_store(t, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                if (last) last = chunks + max(1, (own + A.ochunk - 1) / A.ochunk);      // its parts
-            }
+                last = last ? chunks + (own + A.ochunk - 1) / A.ochunk : -1;      // its parts
+            } else last = -1;
             last_s[r - r_lo] = last;
         }
     }
     __syncthreads();
     const int pairs = (r_hi - r_lo + 1) * A.rep;
-    for (int i = wave; i < pairs; i += 4) {
+    for (int i = tid >> 5; i < pairs; i += OB_SH_THREADS / 32) {
         const int r = i / A.rep, n = last_s[r];
-        if (!n) continue;
-        const int head = kvh * A.rep + i - r * A.rep;
-        if (chunks == 0 && n == 1) {                                             // perhaps without any key: zeros
-            int slot, own;
-            ob_sh_row(A, r_lo + r, first, slot, own);
-            if (own == 0) {
-                if (2 * lane < A.D) *reinterpret_cast<ob_half2 *>(A.o + ((int64_t)(r_lo + r) * A.H + head) * A.D + 2 * lane) = (ob_half2)(_Float16)0;
-                continue;
-            }
-        }
-        ob_sh_join<true>(A, r_lo + r, head, chunks, n);
+        if (n >= 0) ob_sh_join<true>(A, r_lo + r, kvh * A.rep + i - r * A.rep, chunks, n);
     }
 }

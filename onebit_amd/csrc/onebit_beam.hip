@@ -26,29 +26,44 @@ static ObShPlan ob_sh_plan(const onebit_prefix_t *groups, int32_t n_groups, int6
 {
     ObShPlan p = {};
     const int64_t rep = n_heads / n_kv_heads;
-    int64_t most = 1, longest = 0, again = 0, work = 0;
+    int64_t most = 1, longest = 0, again = 0;
     for (int i = 0; i < n_groups; ++i) {
         if (groups[i].len > 0) most = std::max<int64_t>(most, groups[i].n * rep);
         longest = std::max<int64_t>(longest, groups[i].len);
         again += (int64_t)groups[i].n * groups[i].len;
     }
+    // (us of kernels at D = 128, rows x heads / kv heads; the other side in brackets)
     p.own_mb = (int)ob_up(rep, 16);
     const int64_t own = rows * n_kv_heads * p.own_mb;                    // workgroups of one chunk per row
     p.ochunk = (int)(128 * std::max<int64_t>(1, ob_up(max_own, 128)));
+    // a row's own keys in chunks where the rows are few: 8 x 8 / 8 with 1000 own keys each 10.8 (in one chunk 17.3), 16 x 8 / 8 with 600 12.4 (14.2), 30 x 8 / 8 18.7 (18.7)
     if (own < 256 && max_own > 512) p.ochunk = (int)(128 * std::max<int64_t>(2, ob_up(own * max_own, 512 * 128)));
     p.osplits = (int)ob_up(max_own, p.ochunk);
-    if (p.osplits <= 1 && longest <= 256 && again * n_kv_heads * p.own_mb <= 64 * 1024) {
+    // one launch that reads short prefixes once a row: 4 x 8 / 8 sharing 96 5.8 (ob_sh_one_kernel 7.2), 8 x 32 / 32 sharing 256 8.4 (8.8), 64 x 64 / 8 sharing 200 11.0
+    // (16.1); behind the bound 8 x 32 / 32 sharing 500 11.0 (9.6), 32 x 32 / 32 sharing 256 19.4 (16.6), 64 x 32 / 32 sharing 128 26.4 (wide 22.5)
+    if (p.osplits <= 1 && longest <= 256 && again * n_kv_heads * p.own_mb <= 128 * 1024) {
         p.form = OB_SH_INLINE;
         p.osplits = 0;
         return p;
     }
-    p.form = most <= 16 && rows * n_kv_heads <= OB_SH_TICKETS && own <= 1024 ? OB_SH_ONE : most <= 64 ? OB_SH_WIDE64 : OB_SH_WIDE128;
+    const auto tiles = [&](int per) {                                    // keys of all workgroups of `per` queries together
+        int64_t n = 0;
+        for (int i = 0; i < n_groups; ++i) n += ob_up(groups[i].n * rep, per) * groups[i].len * n_kv_heads;
+        return n;
+    };
+    // up to 32 queries of a group and kv head in blocks of 16, one launch: 17 x 32 / 32 sharing 1000 14.3 (blocks of 64 16.8), 32 x 32 / 32 sharing 4000 31.7 (34.1), 4 rows x
+    // 8 groups x 40 / 40 up to 2000 38.1 (47.0); more: 64 x 32 / 32 sharing 8000 54.0 (49.9), 48 x 32 / 8 sharing 2000 23.9 (17.7).
+    // Blocks of 128 where 512 workgroups of them have 512 keys and more: 64 x 64 / 8 sharing 32768 107 (of 64 139), sharing 8000 44.6 (45.3), 48 x 32 / 8 sharing 2000 20.4 (17.7)
+    p.form = most <= 32 && rows * n_kv_heads <= OB_SH_TICKETS ? OB_SH_ONE : most > 64 && tiles(128) >= 512 * 512 ? OB_SH_WIDE128 : OB_SH_WIDE64;
     p.per = p.form == OB_SH_ONE ? 16 : p.form == OB_SH_WIDE64 ? 64 : 128;
-    for (int i = 0; i < n_groups; ++i) work += ob_up(groups[i].n * rep, p.per) * groups[i].len * n_kv_heads;
-    p.among = p.form != OB_SH_ONE && own * max_own >= work;
+    // own keys' workgroups among the prefix's and a launch that joins: 64 x 40 / 40 sharing 2000 with 20 own 37.5 (after them, started from their parts, 44.5), 64 x 32 / 32
+    // sharing 8000 49.9 (57.8); with more queries of a row per kv head, whose parts fill the lanes that fetch them, 64 x 64 / 8 sharing 2000 30.7 (23.9)
+    p.among = p.form == OB_SH_WIDE64 && rep <= 2;
     if (p.form == OB_SH_ONE || p.among) p.osplits = std::max(p.osplits, 1);
     else if (p.osplits <= 1) p.osplits = 0;
-    p.pchunk = (int)(128 * std::max<int64_t>(p.form == OB_SH_ONE ? 1 : 2, ob_up(work, (p.form == OB_SH_ONE ? 256 : 512) * 128)));
+    // chunks for 256 workgroups where a row's last one joins them (1 x 32 / 32 of 8192 26.8, for 512 29.0; 16 x 32 / 32 of 4000 23.7 and 26.4), for 512 else (64 x 64 / 8
+    // sharing 32768 101 of the prefix, for 256 149), no fewer than 256 keys (32 x 32 / 8 sharing 8192 28.7, from 128 on 35.0)
+    p.pchunk = (int)(128 * std::max<int64_t>(p.form == OB_SH_ONE ? 1 : 2, ob_up(tiles(p.per), (p.form == OB_SH_ONE ? 256 : 512) * 128)));
     p.psplits = (int)ob_up(longest, p.pchunk);
     return p;
 }
@@ -95,7 +110,7 @@ static void ob_sh_launch(ObShArgs &a, const ObShPlan &p, int64_t prefix_items, i
         else if (p.form == OB_SH_WIDE128) hipLaunchKernelGGL((ob_sh_wide_kernel<DP, 2, EXACT>), wide, block, 0, s, a);
     }
     if (!p.among) hipLaunchKernelGGL((ob_sh_own_kernel<DP, EXACT>), own, block, 0, s, a);
-    if (a.osplits) hipLaunchKernelGGL(ob_sh_join_kernel, dim3((unsigned)ob_up((int64_t)a.rows * a.H, OB_SH_THREADS / 64)), block, 0, s, a);
+    if (a.osplits) hipLaunchKernelGGL(ob_sh_join_kernel, dim3((unsigned)ob_up((int64_t)a.rows * a.H, OB_SH_THREADS / 32)), block, 0, s, a);
 }
 
 extern "C" int onebit_attention_shared_rows(const void *q, const void *prefix_k, const void *prefix_v, const void *k_cache, const void *v_cache, void *o,
