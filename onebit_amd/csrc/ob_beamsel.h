@@ -18,6 +18,7 @@
 #define OB_BS_THREADS 256
 #define OB_BS_MAX_KEEP 64
 #define OB_BS_MAX_BEAMS 32
+#define OB_BS_LISTS 2048                           // lists of a group that the pick can choose from first
 #define OB_BS_TICKETS 4096                         // groups whose pick may be the scan's: counters in front of the scratch memory, zero between launches
 
 // room for the candidates of a chunk
@@ -114,19 +115,22 @@ __device__ __forceinline__ void ob_bs_pick(const ObBsArgs &A, int group)
     __shared__ double row_v[OB_BS_MAX_BEAMS], cand_v[RANKED];                     // lse of a beam; NaN: it offers nothing
     __shared__ float pub[WAVES * (OB_BS_MAX_KEEP + 2)], t_s;
     __shared__ ObBsCand cand[RANKED];
-    __shared__ int n_s;
+    __shared__ int n_s, lists_s;
+    __shared__ unsigned short live[OB_BS_LISTS];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int room = ob_bs_list(A.keep), total = A.beams * A.chunks * room;
+    const int room = ob_bs_list(A.keep), lists = A.beams * A.chunks, total = lists * room;
+    // more places than registers, in many lists: a threshold from the lists' largest logits first, then the lists that reach it alone (32 rows of 128256, 64 kept: 84 ->
+    // 42 us of both kernels)
+    const bool by_lists = total > THREADS * NS && lists <= OB_BS_LISTS && lists >= 2 * A.keep;
     const int64_t list0 = (int64_t)group * A.beams * A.chunks;
-    if (tid == 0) { n_s = 0; t_s = -INFINITY; }
+    if (tid == 0) { n_s = 0; lists_s = 0; t_s = -INFINITY; }
     struct Place { float x, score; int tok, n, beam, e; };
-    const auto fetch = [&](int i, Place &p) {                                    // (all of it at once: what lies behind a list's end is memory of the list, not used)
-        const int l = min(i, total - 1) / room;
-        p.e = i < total ? i - l * room : 0x7fffffff;
+    const auto fetch = [&](int l, int e, Place &p) {                             // (all of it at once: what lies behind a list's end is memory of the list, not used)
+        p.e = e;
         p.beam = l / A.chunks;
         p.n = ob_bs_get<AGENT>(A.counts + list0 + l);
-        p.x = ob_bs_get<AGENT>(A.list_x + list0 * room + min(i, total - 1));
-        p.tok = ob_bs_get<AGENT>(A.list_t + list0 * room + min(i, total - 1));
+        p.x = ob_bs_get<AGENT>(A.list_x + (list0 + l) * room + e);
+        p.tok = ob_bs_get<AGENT>(A.list_t + (list0 + l) * room + e);
         p.score = A.scores[group * A.beams + p.beam];
     };
     const auto value = [&](const Place &p, ObBsCand &c) -> bool {                // false where there is no candidate
@@ -135,9 +139,11 @@ __device__ __forceinline__ void ob_bs_pick(const ObBsArgs &A, int group)
     };
     Place place[NS];
 #pragma unroll
-    for (int k = 0; k < NS; ++k)
-        if (THREADS * k < total) fetch(tid + THREADS * k, place[k]);
-        else place[k] = {0.f, 0.f, 0, 0, 0, 0};
+    for (int k = 0; k < NS; ++k) {
+        const int i = tid + THREADS * k, l = i / room;
+        place[k] = {0.f, 0.f, 0, 0, 0, 0};                                       // (none)
+        if (!by_lists && i < total) fetch(l, i - l * room, place[k]);
+    }
     // a chunk's sum in terms of the row's largest logit
     const auto term = [](double m, double part, float M) { return m == -INFINITY ? part : part * exp(m - (double)M); };
     if (A.chunks <= 16)                                                          // a row of 16 lanes for a beam
@@ -168,27 +174,55 @@ __device__ __forceinline__ void ob_bs_pick(const ObBsArgs &A, int group)
 #pragma unroll
         for (int k = 0; k < NS; ++k)
             if (value(place[k], c)) f(c);
-        for (int i = tid + THREADS * NS; i < total; i += THREADS) {
+        for (int i = tid + (by_lists ? 0 : THREADS * NS); i < total; i += THREADS) {
             Place p;
-            fetch(i, p);
+            const int l = i / room;
+            fetch(l, i - l * room, p);
             if (value(p, c)) f(c);
         }
     };
+    const auto keep_it = [&](const ObBsCand &c) {
+        const int k = atomicAdd(&n_s, 1);
+        if (k < RANKED) { cand_v[k] = c.v; cand[k] = c; }
+    };
     float best = -INFINITY;
-    each([&](const ObBsCand &c) { best = fmaxf(best, __double2float_rd(c.v)); });      // (rounded down: what reaches the threshold reaches it in 64 bits, too)
-    const int waves = min(WAVES, (total + 63) / 64), share = min(64, (A.keep + waves - 1) / waves + 2);
-    if (wave < waves) ob_bs_publish(best, share, pub + wave * share);
-    __syncthreads();
-    if (ob_bs_is_kth(pub, waves * share, A.keep, tid)) t_s = pub[tid];
-    __syncthreads();
-    const double t = t_s;
-    if (best >= t_s)
-        each([&](const ObBsCand &c) {
-            if (c.v >= t) {
-                const int k = atomicAdd(&n_s, 1);
-                if (k < RANKED) { cand_v[k] = c.v; cand[k] = c; }
-            }
-        });
+    if (by_lists) {
+        constexpr int NL = OB_BS_LISTS / THREADS;
+        float top[NL];
+#pragma unroll
+        for (int k = 0; k < NL; ++k) {
+            const int l = min(tid + THREADS * k, lists - 1), beam = l / A.chunks;
+            const double v = (double)A.scores[group * A.beams + beam] + (ob_bs_get<AGENT>(A.sums + 2 * (list0 + l)) - row_v[beam]);
+            top[k] = tid + THREADS * k < lists && v > -INFINITY ? __double2float_rd(v) : -INFINITY;
+            best = fmaxf(best, top[k]);
+        }
+        const int waves = min(WAVES, (lists + 63) / 64), share = min(64, (A.keep + waves - 1) / waves + 2);
+        if (wave < waves) ob_bs_publish(best, share, pub + wave * share);
+        __syncthreads();
+        if (ob_bs_is_kth(pub, waves * share, A.keep, tid)) t_s = pub[tid];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < NL; ++k)
+            if (top[k] >= t_s && top[k] > -INFINITY) live[atomicAdd(&lists_s, 1)] = (unsigned short)(tid + THREADS * k);
+        __syncthreads();
+        const double t = t_s;
+        for (int i = tid; i < lists_s * room; i += THREADS) {
+            Place p;
+            ObBsCand c;
+            const int at = i / room;
+            fetch(live[at], i - at * room, p);
+            if (value(p, c) && c.v >= t) keep_it(c);
+        }
+    } else {
+        each([&](const ObBsCand &c) { best = fmaxf(best, __double2float_rd(c.v)); });      // (rounded down: what reaches the threshold reaches it in 64 bits, too)
+        const int waves = min(WAVES, (total + 63) / 64), share = min(64, (A.keep + waves - 1) / waves + 2);
+        if (wave < waves) ob_bs_publish(best, share, pub + wave * share);
+        __syncthreads();
+        if (ob_bs_is_kth(pub, waves * share, A.keep, tid)) t_s = pub[tid];
+        __syncthreads();
+        const double t = t_s;
+        if (best >= t_s) each([&](const ObBsCand &c) { if (c.v >= t) keep_it(c); });
+    }
     __syncthreads();
     int n = n_s;
     const int64_t out = (int64_t)group * A.keep;
@@ -234,7 +268,7 @@ __global__ __launch_bounds__(OB_BS_THREADS, PICK ? 4 : NV == 1 ? 8 : 7) void ob_
 {
     __shared__ float red_m[4], pub[4 * (OB_BS_MAX_KEEP + 2)], t_s;
     __shared__ double red_s[4];
-    __shared__ int n_s, red_i[4];
+    __shared__ int n_s, red_i[8];
     const int chunk = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const T *x_row = (const T *)A.logits + (int64_t)row * A.ld;
     const int c0 = chunk * A.vecs * 8, c1 = min(A.vocab, c0 + A.vecs * 8);
@@ -298,36 +332,59 @@ __global__ __launch_bounds__(OB_BS_THREADS, PICK ? 4 : NV == 1 ? 8 : 7) void ob_
     if (lane == 0) red_s[wave] = s;
     __syncthreads();
     int n = n_s;
-    if (n > room) {                                                             // too many reach the threshold: one after the other
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                         // (over what is listed already)
-        float px = INFINITY;
-        int pt = -1;
-        for (n = 0; n < A.keep; ++n) {
-            float bx = -INFINITY;
-            int bt = 0x7fffffff;
+    if (n > room) {
+        // too many reach the threshold: a search for one that `keep` reach and the list has room for, bit by bit (x as whole numbers of its order; NaN the lowest), and,
+        // where that is one of too many equal logits, for the last index that is taken
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                         // (what is listed already is written over)
+        int turn = 0;
+        const auto count = [&](auto in) -> int {                                 // elements that `in` holds for, over the workgroup
+            int c = 0;
 #pragma unroll
             for (int j = 0; j < NV; ++j)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int tok = c0 + 8 * (tid + OB_BS_THREADS * j) + e;
-                    const float v = x[j][e];
-                    if ((v < px || (v == px && tok > pt)) && v > bx) { bx = v; bt = tok; }       // (a thread's tokens ascend)
-                }
-            const float w = ob_wave_max(bx);
-            int wt2 = bx == w ? bt : 0x7fffffff;
-#pragma unroll
-            for (int k = 32; k; k >>= 1) wt2 = min(wt2, __shfl_xor(wt2, k, 64));
+                for (int e = 0; e < 8; ++e) c += __popcll(__ballot(in(__float_as_uint(x[j][e]), 8 * (tid + OB_BS_THREADS * j) + e)));
+            int *to = red_i + 4 * turn;
+            turn ^= 1;
+            if (lane == 0) to[wave] = c;
             __syncthreads();
-            if (lane == 0) { red_m[wave] = w; red_i[wave] = wt2; }
-            __syncthreads();
-            px = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3]));
-            pt = 0x7fffffff;
+            return (to[0] + to[1]) + (to[2] + to[3]);
+        };
 #pragma unroll
-            for (int w2 = 0; w2 < 4; ++w2)
-                if (red_m[w2] == px) pt = min(pt, red_i[w2]);
-            if (px == -INFINITY) break;
-            if (tid == 0) { ob_bs_put<PICK>(lx + n, px); ob_bs_put<PICK>(lt + n, pt); }
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t u = __float_as_uint(x[j][e] + 0.f);               // (-0 is 0)
+                x[j][e] = __uint_as_float(x[j][e] != x[j][e] ? 0u : u & 0x80000000u ? ~u : u | 0x80000000u);
+            }
+        uint32_t kth = 0;
+        int reach = n;
+        for (uint32_t bit = 0x80000000u; bit && reach > room; bit >>= 1) {
+            const uint32_t k = kth | bit;
+            const int c = count([&](uint32_t u, int) { return u >= k; });
+            if (c >= A.keep) { kth = k; reach = c; }
         }
+        int last = 8 * OB_BS_THREADS * NV;
+        if (reach > room) {
+            const int want = A.keep - count([&](uint32_t u, int) { return u > kth; });
+            last = 0;
+            for (int bit = 4 * OB_BS_THREADS * NV; bit; bit >>= 1)
+                if (count([&](uint32_t u, int at) { return u == kth && at < (last | bit); }) < want) last |= bit;
+        }
+        if (tid == 0) n_s = 0;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t u = __float_as_uint(x[j][e]);
+                const int at0 = 8 * (tid + OB_BS_THREADS * j) + e;
+                if (u > kth || (u == kth && at0 <= last)) {
+                    const int at = atomicAdd(&n_s, 1);
+                    if (at < room) { ob_bs_put<PICK>(lx + at, __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u)); ob_bs_put<PICK>(lt + at, c0 + at0); }
+                }
+            }
+        __syncthreads();
+        n = min(n_s, room);
     }
     if (tid == 0) {
         ob_bs_put<PICK>(A.sums + 2 * list, (double)m);

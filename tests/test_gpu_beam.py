@@ -254,7 +254,7 @@ def _best(logits, scores, beams, keep):
         v = torch.where(torch.isnan(v), -math.inf, v)
         cand = []
         for b in range(beams):
-            order = torch.sort(x[g * beams + b].nan_to_num(nan=-math.inf), descending=True, stable=True).indices[:keep + 1].tolist()
+            order = torch.sort(x[g * beams + b].nan_to_num(nan=-math.inf) + 0.0, descending=True, stable=True).indices[:keep + 1].tolist()
             cand += [(-v[b, t].item(), b, i, t) for i, t in enumerate(order) if v[b, t] > -math.inf]
         cand = sorted(cand)[:keep]
         cand += [(math.inf, -1, 0, -1)] * (keep - len(cand))
@@ -292,6 +292,21 @@ def test_ties_go_to_the_lowest_beam_and_token(dtype, keep):
     logits = row.repeat(6, 1)                                       # equal hypotheses: every value occurs in each of them, many times
     _check_select(logits, torch.full((6,), -3.0, device="cuda"), 3, keep)
     _check_select(torch.zeros(4, 5001, dtype=dtype, device="cuda"), torch.zeros(4, device="cuda"), 4, keep)
+
+
+@pytest.mark.parametrize("vocab, beams, keep, banned", [(512, 32, 64, 0), (512, 32, 64, 300), (32000, 32, 64, 10666), (9001, 2, 64, 0), (50257, 32, 64, 0), (520, 3, 64, 500)])
+@pytest.mark.parametrize("values", ["many", "few"])
+def test_more_candidates_than_a_list_holds(vocab, beams, keep, banned, values):
+    """Many kept next to a chunk's lanes, few distinct values, banned tokens in runs: the search for a threshold, lists that the pick chooses from first."""
+    g = torch.Generator(device="cuda").manual_seed(vocab + keep)
+    x = 2 * torch.randn(2 * beams, vocab, generator=g, device="cuda")
+    if values == "few":
+        x = (x * 2).round() / 2
+        x[:, ::7] *= -0.0                                            # zeros of both signs are equal logits
+    x[:, vocab // 3:vocab // 3 + banned] = -math.inf
+    scores = -10 - 2 * torch.rand(2 * beams, generator=g, device="cuda")
+    _check_select(x.half(), scores, beams, keep)
+    _check_select(x, scores, beams, keep)
 
 
 def test_equal_rows_at_every_alignment_have_equal_values():
