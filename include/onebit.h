@@ -523,7 +523,7 @@ size_t onebit_mixed_workspace_bytes(const onebit_model_t *model, int64_t max_row
 int onebit_mixed_step(const onebit_model_t *model, const onebit_mixed_state_t *state, void *stream);
 /* The same step where the single-token rows share prefixes (onebit_attention_shared_rows, with the model's caches as both of its caches):
  * `groups` tile rows 0 .. n_dec - 1; group g's rows attend to the first g.len positions of slot g.slot, and from position g.first on to their own
- * slot.  attn_chunk / dec_ctx are not used.  scratch: onebit_attention_shared_scratch_bytes(groups, n_groups, n_dec, .., max_own). */
+ * slot.  attn_chunk / dec_ctx are not used.  scratch: onebit_attention_shared_scratch_bytes(groups, n_groups, n_dec, .., max_own) bytes, zero-filled once. */
 struct onebit_prefix;
 int onebit_mixed_step_shared(const onebit_model_t *model, const onebit_mixed_state_t *state, const struct onebit_prefix *groups, int32_t n_groups,
                              int64_t max_own, void *scratch, size_t scratch_bytes, void *stream);
@@ -569,8 +569,9 @@ int onebit_fused_gemv(const onebit_proj_t *projs, void *const *outs, int nproj, 
  *   [n_prefix_slots][n_kv_heads][prefix_max_len][D], own cache [n_slots][n_kv_heads][max_len][D]; D a multiple of 8, at most 128.
  *   max_own: bound on row_pos - g.first + 1 over the rows; positions beyond it are NOT attended.  Scores, statistics and sums fp32, the
  *   weights rounded to fp16 before the value product.  Deterministic.
- *   scratch: onebit_attention_shared_scratch_bytes() of the same groups and sizes, 16-byte aligned, its contents of no account; not shared by
- *   calls that may run at the same time (0 bytes: the arguments are refused). */
+ *   o overlaps no input.  scratch: onebit_attention_shared_scratch_bytes() of the same groups and sizes or more, 16-byte aligned, ZERO-FILLED ONCE: the
+ *   counters in front of it (16384 int32, whatever the sizes) are zero again after every call.  Not shared by calls that may run at the same time
+ *   (the function returns 0 where the arguments are refused). */
 typedef struct onebit_prefix { int32_t row0, n, slot, len, first; } onebit_prefix_t;
 size_t onebit_attention_shared_scratch_bytes(const onebit_prefix_t *groups, int32_t n_groups, int64_t rows, int32_t n_heads, int32_t n_kv_heads,
                                              int32_t head_dim, int64_t max_own);
@@ -584,7 +585,8 @@ int onebit_attention_shared_rows(const void *q, const void *prefix_k, const void
  * best in the order (v descending, beam, logit descending, token) are written to out_scores (v rounded to fp32) / out_beams / out_tokens
  * [groups, keep].  A continuation of v = -inf or NaN (a banned token, a dead hypothesis, a row with a NaN or +inf) is none; places that remain
  * hold -inf, -1, -1.  beams 1 .. 32, keep 1 .. 64, vocab <= 2^20, groups * beams <= 65535.  scratch: onebit_beam_select_scratch_bytes(groups * beams, vocab, keep)
- * bytes, 16-byte aligned, its contents of no account. */
+ * bytes or more, 16-byte aligned, ZERO-FILLED ONCE (4096 int32 in front of it are zero again after every call); not shared by calls that may run at the
+ * same time. */
 size_t onebit_beam_select_scratch_bytes(int64_t rows, int64_t vocab, int32_t keep);
 int onebit_beam_select(const void *logits, int64_t ld, int dtype, const float *scores, int64_t groups, int32_t beams, int64_t vocab, int32_t keep,
                        float *out_scores, int32_t *out_beams, int32_t *out_tokens, void *scratch, size_t scratch_bytes, void *stream);

@@ -3,7 +3,7 @@ hypotheses from their logits, and their states brought to the slots that go on w
 
 All three enqueue on the current stream of their tensors' device and never synchronise; they can be captured into a HIP graph (host
 arguments -- the groups, lengths, positions -- are fixed by the capture, device tensors are read by every replay).  A workspace may be kept
-between calls of the same sizes; calls that may run at the same time need one each.  There is no CPU fallback."""
+between calls; calls that may run at the same time (other streams, graphs replayed next to each other) need one each.  There is no CPU fallback."""
 from __future__ import annotations
 
 import ctypes
@@ -121,8 +121,8 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: Optional[torch.Tensor], p
         scale = h_next.data_ptr()
     if out is None:
         out = torch.zeros_like(q)
-    elif out.shape != shape or out.dtype is not _F16 or not out.is_contiguous():
-        raise ValueError(f"{what}: out must be like q")
+    elif out.shape != shape or out.dtype is not _F16 or not out.is_contiguous() or out.data_ptr() == q.data_ptr() != 0:
+        raise ValueError(f"{what}: out must be like q and not q")
     arr = _prefixes(groups)
     if max_own is None:
         max_own = max([0] + [max_len - int(g[4]) for g in groups])

@@ -262,7 +262,8 @@ __device__ __forceinline__ void ob_bs_pick(const ObBsArgs &A, int group)
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void ob_bs_pick_kernel(const ObBsArgs A) { ob_bs_pick<THREADS, false>(A, blockIdx.x); }
 
-// NV: pieces of 8 elements of a thread, OB_BS_THREADS apart.  PICK: the last workgroup of a group picks
+// NV: pieces of 8 elements of a thread, OB_BS_THREADS apart.  PICK: the last workgroup of a group picks.
+// 256 rows of 50257 fp16 12 us (2.1 TB/s; NV = 4 in 72 registers, so that the 1792 workgroups run in one round: 85 registers 13.6), 8 rows of 32000 with the pick 15.5.
 template <typename T, int NV, bool PICK>
 __global__ __launch_bounds__(OB_BS_THREADS, PICK ? 4 : NV == 1 ? 8 : 7) void ob_bs_scan_kernel(const ObBsArgs A)
 {

@@ -192,10 +192,14 @@ static ObBsPlan ob_bs_plan(int64_t groups, int32_t beams, int64_t vocab, int32_t
 {
     const int64_t all = ob_up(vocab, 8), one = ob_up(all, OB_BS_THREADS), few = 256 * OB_BS_PLACES;
     ObBsPlan p;
-    p.nv = groups * beams * one > 2048 || beams * one * ob_bs_list(keep) > few ? 4 : 1;
+    // (us of both halves, groups x beams, vocabulary 32000 if not said otherwise; the other side in brackets)
+    // four pieces a thread: 1 x 4 12.4 (one piece 13.7), 16 x 1 11.0 (12.1), 16 x 4 13.0 (15.1), 64 x 4 16.1 (22.1), 64 x 4 of 50257 18.4 (26.7); one: 1 x 1 9.6 (four 9.9), 64 x 4 of 512
+    // 13.4 (15.4)
+    p.nv = one >= 4 && (beams * one >= 64 || groups * beams * one > 128) ? 4 : 1;
     p.chunks = (int)ob_up(all, p.nv * OB_BS_THREADS);
     p.vecs = (int)ob_up(all, p.chunks);
-    p.fused = groups <= OB_BS_TICKETS && groups * beams * p.chunks <= 1024 && (int64_t)beams * p.chunks * ob_bs_list(keep) <= few;
+    // one launch: 1 x 4 12.4 (two 12.1), 2 x 8 16.0 (15.7), 4 x 4 12.8 (12.8), and 4 less on the host; 16 x 4, 256 workgroups, 15.1 (13.0), 64 x 4, 1024, 18.6 (16.1)
+    p.fused = groups <= OB_BS_TICKETS && groups * beams * p.chunks <= 128 && (int64_t)beams * p.chunks * ob_bs_list(keep) <= few;
     return p;
 }
 

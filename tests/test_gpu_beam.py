@@ -236,7 +236,7 @@ def test_attention_python_refusals():
     for b in bad:
         with pytest.raises(ValueError):
             _call({**c, **b})
-    for b in (dict(out=c["q"].float()), dict(h_next=c["q"][0, 0]), dict(workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))):
+    for b in (dict(out=c["q"]), dict(out=c["q"].float()), dict(h_next=c["q"][0, 0]), dict(workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))):
         with pytest.raises(ValueError):
             _call(c, **b)
 
