@@ -229,6 +229,69 @@ def test_one_workspace_for_calls_of_many_sizes_in_turn():
         assert torch.equal(y, _call(c))
 
 
+def test_scratch_contents_are_of_no_account_but_for_the_counters():
+    for rows, length, own in ((4, 900, 20), (40, 900, 300), (6, 5000, 900)):
+        c = _case([length], [rows], [own] * rows, 4, 4, 128, seed=rows)
+        ws = shared_prefix_workspace(c["groups"], rows, 4, 4, 128, own)
+        y = _call(c, workspace=ws)
+        ws[4 * 16384:] = 255                                        # NaN, as floats
+        z = _call(c, workspace=ws)
+        assert torch.equal(y, z) and not ws[:4 * 16384].any()
+        _check(c, z)
+
+
+def test_the_same_bits_every_time():
+    for rows, H, hkv, length, own in ((5, 8, 8, 3000, 100), (24, 8, 2, 2000, 700), (64, 8, 8, 900, 60)):
+        c = _case([length, length // 2], [rows - 2, 2], [1 + (own * ((7 * r) % rows)) // rows for r in range(rows)], H, hkv, 64, seed=rows)
+        ws = shared_prefix_workspace(c["groups"], rows, H, hkv, 64, own)
+        y = _call(c, workspace=ws)
+        _check(c, y)
+        assert all(torch.equal(_call(c, workspace=ws), y) for _ in range(50))
+
+
+def test_streams_at_the_same_time():
+    """Calls on two streams, each with a workspace of its own."""
+    cases = [_case([1500], [6], [40 + i] * 6, 8, 8, 128, seed=i) for i in range(2)]
+    want = [_call(c) for c in cases]
+    ws = [shared_prefix_workspace(c["groups"], 6, 8, 8, 128, max(c["own"])) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(_call(cases[i], workspace=ws[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, w) for ys, w in zip(got, want) for y in ys)
+
+
+def test_two_graphs_with_one_workspace_replayed_in_turn():
+    cases = [_case([700 + 900 * i], [3 + 4 * i], [50] * (3 + 4 * i), 4, 4, 64, seed=i) for i in range(2)]
+    ws = shared_prefix_workspace(cases[1]["groups"], 7, 4, 4, 64, 50)
+    outs, graphs = [torch.zeros_like(c["q"]) for c in cases], []
+    for c, o in zip(cases, outs):
+        _call(c, out=o, workspace=ws)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            _call(c, out=o, workspace=ws)
+    for _ in range(3):
+        for c, o, g in zip(cases, outs, graphs):
+            o.zero_()
+            g.replay()
+        torch.cuda.synchronize()
+        for c, o in zip(cases, outs):
+            _check(c, o)
+
+
+def test_thousands_of_rows():
+    """More rows than the counters count: the launches for many."""
+    lens, rows = [(53 * i) % 400 for i in range(600)], [1 + i % 9 for i in range(600)]
+    own = [1 + (13 * r) % 40 for r in range(sum(rows))]
+    assert sum(rows) * 8 > 16384
+    _check(c := _case(lens, rows, own, 8, 8, 40, seed=8), _call(c))
+
+
 def test_attention_python_refusals():
     c = _case([700], [3], [5, 1, 20], 4, 4, 64)
     bad = [dict(q=c["q"].float()), dict(q=c["q"][:, :, :32]), dict(k=c["k"].float()), dict(pk=None), dict(row_pos=c["row_pos"].long()), dict(row_pos=c["row_pos"][:2]),
@@ -360,6 +423,28 @@ def test_select_in_a_graph_and_with_a_kept_workspace():
         rv, rb, rt = _best(logits, scores, 4, 8)
         assert torch.equal(out[1].cpu(), rb) and torch.equal(out[2].cpu(), rt)
         _check_select(logits, scores, 2, 5, workspace=ws)           # the workspace serves another call in between
+
+
+def test_select_gives_the_same_bits_every_time_on_any_stream():
+    g = torch.Generator(device="cuda").manual_seed(5)
+    inputs = [(torch.randn(b * n, v, generator=g, device="cuda"), -torch.rand(b * n, generator=g, device="cuda"), b) for n, b, v in ((1, 4, 32000), (2, 8, 9001), (64, 4, 3000))]
+    ws = [beam_select_workspace(x.shape[0], x.shape[1], 2 * b) for x, _, b in inputs]
+    want = [[t.clone() for t in beam_select(x, s, b, 2 * b)] for x, s, b in inputs]
+    streams = [torch.cuda.Stream() for _ in inputs]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        for i, (x, s, b) in enumerate(inputs):
+            with torch.cuda.stream(streams[i]):
+                got.append((i, beam_select(x, s, b, 2 * b, workspace=ws[i])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for i, y in got for a, b in zip(y, want[i]))
+    assert not any(w[:4 * 4096].any() for w in ws)
+
+
+def test_select_many_groups():
+    g = torch.Generator(device="cuda").manual_seed(6)
+    _check_select(torch.randn(5000, 33, generator=g, device="cuda"), -torch.rand(5000, generator=g, device="cuda"), 1, 3)
 
 
 def test_select_python_refusals():
