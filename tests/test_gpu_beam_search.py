@@ -229,3 +229,45 @@ def test_hybrid_generate():
     out = model.generate(ids, 8, num_beams=3)
     assert out.shape == (3, 19) and torch.equal(out[:, :11], ids)
     assert torch.equal(out, model.generate_native(ids, 8, num_beams=3))
+
+
+def test_command_line(tmp_path, capsys):
+    from onebit_amd.checkpoint import write_safetensors
+    from onebit_amd.cli import main
+    from onebit_amd.lebepel import LebepelConfig, synthetic_weights
+    from onebit_amd.registry import load_model
+    import json
+    raw = {"architecture": "Lebepel", "vocab": 50, "width": 64, "norm": {"eps": 1e-5}, "residual_mult": 0.5, "logit_softcap": 20.0, "max_positions": 128,
+           "layers": [{"type": "mamba2", "mixer": dict(heads=4, groups=2, state=16, vdim=24, conv=4, norm_groups=2), "mlp": {"kind": "dense", "ff": 72}},
+                      {"type": "attention", "mixer": dict(heads=4, kv_heads=2, dim=24, vdim=32, scale=0.2), "mlp": {"kind": "dense", "ff": 72}}]}
+    (tmp_path / "config.json").write_text(json.dumps(raw))
+    write_safetensors(str(tmp_path / "model.safetensors"), synthetic_weights(LebepelConfig.from_dict(raw), 6))
+    prompts = [[3, 4, 9, 30, 7], [8]]
+    run = lambda *extra: main(["generate", "--model", str(tmp_path), "--dtype", "float32", "--max-new-tokens", "5", *extra] + [x for p in prompts for x in ("--prompt", ",".join(map(str, p)))])
+    assert run("--num-beams", "3") == 0
+    rows = [json.loads(l)["tokens"] for l in capsys.readouterr().out.splitlines() if l.startswith("{")]
+    model = load_model(str(tmp_path), dtype=torch.float32)
+    for p, row in zip(prompts, rows):
+        assert row == list(reference(lambda t: model.forward(torch.tensor([t], device="cuda"))[0, -1].cpu(), p, 3, 5)[0][1])
+    end = rows[0][1]
+    assert run("--num-beams", "2", "--eos", str(end), "--length-penalty", "0.5") == 0
+    ended = [json.loads(l)["tokens"] for l in capsys.readouterr().out.splitlines() if l.startswith("{")]
+    for p, row in zip(prompts, ended):
+        assert row == list(reference(lambda t: model.forward(torch.tensor([t], device="cuda"))[0, -1].cpu(), p, 2, 5, frozenset([end]), 0.5)[0][1])
+
+
+def test_shared_rows_next_to_prompts():
+    """A step that carries prompt chunks beside rows that share a prefix gives each what it gives alone."""
+    model = _llama()
+    g = torch.Generator().manual_seed(4)
+    tok = lambda n: torch.randint(0, 96, (n,), generator=g).tolist()
+    base, other, chunk = tok(300), tok(70), tok(40)
+    cache = KVCache(model.config, 8, 400, "cuda", torch.float16)
+    step = MixedStep(model, cache.layers, 8, 400, keep_logits=True)
+    step.launch([(6, 0, base), (5, 0, other)])
+    step.launch([(0, 300, [1]), (7, 0, chunk), (1, 300, [2]), (2, 70, [3])], prefixes=[(2, 6, 300), (1, 5, 70)])
+    got = step.logits[:4].clone()
+    for i, seq in enumerate((base + [1], chunk, base + [2], other + [3])):
+        step.launch([(3, 0, seq)])
+        want = step.logits[0]
+        assert float((got[i].float() - want.float()).norm() / want.float().norm()) < 20 * 2.0 ** -11
