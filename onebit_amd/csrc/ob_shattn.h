@@ -100,40 +100,49 @@ struct ObShWave {
     __device__ __forceinline__ void weights(const ob_half8 (&kf)[2][DK], float scale, int n, ob_half8 (&pb)[MT])
     {
         const int g = (threadIdx.x & 63) >> 4;
+        ob_float4 s[MT][2];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            ob_float4 s[2];
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
-                s[kt] = (ob_float4){0.f, 0.f, 0.f, 0.f};
+                s[mt][kt] = (ob_float4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int j = 0; j < DK; ++j) s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[kt][j], qf[mt][j], s[kt], 0, 0, 0);
+                for (int j = 0; j < DK; ++j) s[mt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[kt][j], qf[mt][j], s[mt][kt], 0, 0, 0);
             }
-            if (TAIL)
+        if (TAIL)
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (16 * (e >> 2) + 4 * g + (e & 3) >= n) s[e >> 2][e & 3] = -INFINITY;
-            // the running maximum moves only where a weight exceeds 2^8 (the first ones do): the weights stay far inside fp16, and neither the tile's maximum nor a
-            // rescaled output is needed otherwise.  Weights are not negative, so their bits order like whole numbers.
-            const auto exponentials = [&]() {
+            for (int e = 0; e < 8; ++e)
+                if (16 * (e >> 2) + 4 * g + (e & 3) >= n)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) pb[mt][e] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 2][e & 3], scale, -m[mt]));
-            };
-            exponentials();
-            const ob_u32x4 bits = __builtin_bit_cast(ob_u32x4, pb[mt]);
-            const auto pair = [](uint32_t v) { return __builtin_bit_cast(ob_u16x2, v); };
-            const ob_u16x2 most = __builtin_elementwise_max(__builtin_elementwise_max(pair(bits[0]), pair(bits[1])), __builtin_elementwise_max(pair(bits[2]), pair(bits[3])));
-            if (__any(__builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(most, (ob_u16x2)(unsigned short)0x5c00)) != 0)) {
-                float mx = s[0][0];
+                    for (int mt = 0; mt < MT; ++mt) s[mt][e >> 2][e & 3] = -INFINITY;
+        // the running maximum moves only where a weight exceeds 2^15 (the first ones do), to where the largest is 2^7: the weights stay inside fp16, those of 2^-21 of the
+        // largest and more as normal numbers, and neither the tile's maximum nor a rescaled output is needed otherwise.  Weights are not negative, so their bits order
+        // like whole numbers.
+        const auto exponentials = [&]() {
+            ob_u16x2 most = {0, 0};
 #pragma unroll
-                for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[e >> 2][e & 3]);
-                const float mn = fmaxf(m[mt], ob_sh_rows_max(mx) * scale), f = ob_sh_weight(m[mt], mn);
+            for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) pb[mt][e] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][e >> 2][e & 3], scale, -m[mt]));
+                const ob_u32x4 bits = __builtin_bit_cast(ob_u32x4, pb[mt]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(ob_u16x2, bits[i]));
+            }
+            return __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(most, (ob_u16x2)(unsigned short)0x7800)) != 0;
+        };
+        if (__any(exponentials())) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                float mx = s[mt][0][0];
+#pragma unroll
+                for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[mt][e >> 2][e & 3]);
+                const float mn = fmaxf(m[mt], __builtin_fmaf(ob_sh_rows_max(mx), scale, -7.f)), f = ob_sh_weight(m[mt], mn);
                 l[mt] *= f;
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) acc[mt][dt] *= f;
                 m[mt] = mn;
-                exponentials();
             }
+            exponentials();
         }
     }
 
@@ -319,7 +328,7 @@ __device__ __forceinline__ ObShItem ob_sh_item(const ObShArgs &A, int block, int
 }
 
 // More queries: the four waves share the queries out, 16 MT each, over tiles of 64 keys and values that they read from the LDS together (two tiles there,
-// a third on its way in registers; one barrier a tile).  MT = 2: 64 rows of 64 / 8 heads over 32768 keys 90 us, 0.76 PFLOP/s, bound by products and exponentials in turn (no
+// a third on its way in registers; one barrier a tile).  MT = 2: 64 rows of 64 / 8 heads over 32768 keys 87 us, 0.79 PFLOP/s, bound by products and exponentials in turn (no
 // LDS bank conflict; MT = 4 140 us: 490 registers, one wave a SIMD).
 template <int DP, int MT, bool EXACT>
 __device__ __forceinline__ void ob_sh_wide(const ObShArgs &A, const ObShItem &I, const ObShGroup &G, _Float16 (*kv)[2][64 * DP])
