@@ -95,12 +95,11 @@ struct ObShWave {
         }
     }
 
-    // Weights of 32 keys (kf: their rows); TAIL: only the first `n` count
+    // Scores of 32 keys (kf: their rows); TAIL: only the first `n` count
     template <bool TAIL>
-    __device__ __forceinline__ void weights(const ob_half8 (&kf)[2][DK], float scale, int n, ob_half8 (&pb)[MT])
+    __device__ __forceinline__ void scores(const ob_half8 (&kf)[2][DK], int n, ob_float4 (&s)[MT][2])
     {
         const int g = (threadIdx.x & 63) >> 4;
-        ob_float4 s[MT][2];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -115,6 +114,11 @@ struct ObShWave {
                 if (16 * (e >> 2) + 4 * g + (e & 3) >= n)
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) s[mt][e >> 2][e & 3] = -INFINITY;
+    }
+
+    // Their weights
+    __device__ __forceinline__ void weights(const ob_float4 (&s)[MT][2], float scale, ob_half8 (&pb)[MT])
+    {
         // the running maximum moves only where a weight exceeds 2^15 (the first ones do), to where the largest is 2^7: the weights stay inside fp16, those of 2^-21 of the
         // largest and more as normal numbers, and neither the tile's maximum nor a rescaled output is needed otherwise.  Weights are not negative, so their bits order
         // like whole numbers.
@@ -146,23 +150,32 @@ struct ObShWave {
         }
     }
 
+    // columns 16 dt .. of the 32 values from vt on, as the second product takes them
+    __device__ __forceinline__ ob_half8 columns(const _Float16 *vt, int dt)
+    {
+        const int lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4;
+        ob_sh_v4s a[2];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+            a[kt] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ob_sh_lds_v4s *)(vt + ob_sh_place<DP>(16 * kt + 4 * g + (lr >> 2), 2 * dt + ((lr & 3) >> 1)) + 4 * (lr & 1)));
+        const ob_sh_v8s av = {a[0][0], a[0][1], a[0][2], a[0][3], a[1][0], a[1][1], a[1][2], a[1][3]};
+        return __builtin_bit_cast(ob_half8, av);
+    }
+
     // acc += weights . values, vt: the 32 keys' rows in the LDS
     __device__ __forceinline__ void values(const _Float16 *vt, const ob_half8 (&pb)[MT])
     {
-        const int lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4;
         const ob_half8 one = (ob_half8)(_Float16)1;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) l[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(one, pb[mt], l[mt], 0, 0, 0);
+        ob_half8 av[DT];
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-            ob_sh_v4s a[2];
+        for (int dt = 0; dt < DT; ++dt) av[dt] = columns(vt, dt);
+        __builtin_amdgcn_sched_barrier(0);                                       // (all of them on their way: left to itself hipcc waits for one after the other)
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
-                a[kt] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ob_sh_lds_v4s *)(vt + ob_sh_place<DP>(16 * kt + 4 * g + (lr >> 2), 2 * dt + ((lr & 3) >> 1)) + 4 * (lr & 1)));
-            const ob_sh_v8s av = {a[0][0], a[0][1], a[0][2], a[0][3], a[1][0], a[1][1], a[1][2], a[1][3]};
+        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) acc[mt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ob_half8, av), pb[mt], acc[mt][dt], 0, 0, 0);
-        }
+            for (int mt = 0; mt < MT; ++mt) acc[mt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[dt], pb[mt], acc[mt][dt], 0, 0, 0);
     }
 };
 
@@ -227,7 +240,9 @@ __device__ __forceinline__ void ob_sh_sweep(const ObShArgs &A, const ObShRange &
         __builtin_amdgcn_wave_barrier();
         if (t + 4 < n) load_v(t + 4);
         ob_half8 pb[MT];
-        W.template weights<true>(kf, A.scale_log2e, end - base, pb);
+        ob_float4 s[MT][2];
+        W.template scores<true>(kf, end - base, s);
+        W.weights(s, A.scale_log2e, pb);
         if (t + 4 < n) load_k(t + 4);
         W.values(vt, pb);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -327,60 +342,73 @@ __device__ __forceinline__ ObShItem ob_sh_item(const ObShArgs &A, int block, int
     return I;
 }
 
-// More queries: the four waves share the queries out, 16 MT each, over tiles of 64 keys and values that they read from the LDS together (two tiles there,
-// a third on its way in registers; one barrier a tile).  MT = 2: 64 rows of 64 / 8 heads over 32768 keys 87 us, 0.79 PFLOP/s, bound by products and exponentials in turn (no
-// LDS bank conflict; MT = 4 140 us: 490 registers, one wave a SIMD).
+// More queries: the four waves share the queries out, 16 MT each, over tiles of 64 keys and values that they read from the LDS together (two tiles
+// there, brought by DMA; one barrier a tile).  The second half's keys are read while the first one's exponentials run.
+// MT = 2: 64 rows of 64 / 8 heads over 32768 keys 77 us, 0.89 PFLOP/s (tiles through registers 87; MT = 4 140: 490 registers, one wave a SIMD): products, exponentials and LDS
+// reads, 32, 40 and 37 us of them each, in turn.
 template <int DP, int MT, bool EXACT>
 __device__ __forceinline__ void ob_sh_wide(const ObShArgs &A, const ObShItem &I, const ObShGroup &G, _Float16 (*kv)[2][64 * DP])
 {
-    constexpr int DK = DP / 32, PPR = DP / 8, NP = 64 * PPR / OB_SH_THREADS, RPL = OB_SH_THREADS / PPR;      // pieces of a thread, rows apart
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, g = lane >> 4;
+    constexpr int DK = DP / 32, PPR = DP / 8, RPL = 64 / PPR, NL = 64 / RPL / 4;      // pieces of 16 bytes per row, rows per DMA, DMAs of a wave
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 15, g = lane >> 4;
     const int D = EXACT ? DP : A.D, qi0 = I.qi0 + 16 * MT * wave, nq = G.n * A.rep;
     ObShWave<DP, MT, EXACT> W;
     W.init(A, G.row0, qi0, nq, I.kvh);
-    ob_half8 kr[NP], vr[NP];
-    const int prow = tid / PPR, ppc = tid % PPR;
-    const bool there = EXACT || 8 * ppc < D;
-    const auto load = [&](int base) {
+    // a lane brings what belongs at its place of RPL rows: row lane / PPR of them (the same of every eight), place lane % PPR
+    const int row = lane / PPR, at = lane % PPR;
+    const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) char *)&kv[0][0][0];
+    const auto load = [&](int base, int b) {
+        const int most = I.k1 - 1 - base;                                        // (rows behind the last one: the last one again, its weights are zero)
+        const char *kb = reinterpret_cast<const char *>(I.kb + (int64_t)base * D), *vb = reinterpret_cast<const char *>(I.vb + (int64_t)base * D);
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            const int64_t at = (int64_t)min(base + prow + RPL * i, I.k1 - 1) * D + 8 * ppc;
-            kr[i] = there ? *reinterpret_cast<const ob_half8 *>(I.kb + at) : (ob_half8)(_Float16)0;
-            vr[i] = there ? *reinterpret_cast<const ob_half8 *>(I.vb + at) : (ob_half8)(_Float16)0;
+        for (int i = 0; i < NL; ++i) {
+            const int r = RPL * (NL * wave + i) + row, p = 2 * ((at >> 1) ^ (r & (DP / 16 - 1))) + (at & 1);
+            const uint32_t off = (uint32_t)(min(r, most) * D + 8 * p) * 2, to = lds0 + (uint32_t)b * (2 * 64 * DP * 2) + (NL * wave + i) * 1024;
+            if (EXACT || 8 * p < D) {
+                ob_dma_1k(kb, off, to);
+                ob_dma_1k(vb, off, to + 64 * DP * 2);
+            }
         }
     };
-    const auto store = [&](int base, int b) {
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            const int row = prow + RPL * i;
-            if (base + 64 > I.k1 && base + row >= I.k1) vr[i] = (ob_half8)(_Float16)0;
-            *reinterpret_cast<ob_half8 *>(&kv[b][0][ob_sh_place<DP>(row, ppc)]) = kr[i];
-            *reinterpret_cast<ob_half8 *>(&kv[b][1][ob_sh_place<DP>(row, ppc)]) = vr[i];
-        }
+    const auto landed = [&]() {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
     };
-    load(I.k0);
-    store(I.k0, 0);
-    if (I.k0 + 64 < I.k1) load(I.k0 + 64);
-    __syncthreads();
-    const auto half = [&](int b, int h, auto tail, int n) {                          // 32 keys of the tile in buffer b
-        ob_half8 kf[2][DK], pb[MT];
+    if (!EXACT) {                                                                // columns from D on are not brought: zeros
+        for (int i = tid; i < 4 * 64 * PPR; i += OB_SH_THREADS) *reinterpret_cast<ob_half8 *>(&kv[0][0][8 * i]) = (ob_half8)(_Float16)0;
+        __syncthreads();
+    }
+    load(I.k0, 0);
+    landed();
+    int b = 0, base = I.k0;
+    const auto keys = [&](int h, ob_half8 (&kf)[2][DK]) {
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
             for (int j = 0; j < DK; ++j) kf[kt][j] = *reinterpret_cast<const ob_half8 *>(&kv[b][0][ob_sh_place<DP>(32 * h + 16 * kt + lr, 4 * j + g)]);
-        W.template weights<decltype(tail)::value>(kf, A.scale_log2e, n, pb);
-        W.values(&kv[b][1][32 * h * DP], pb);
     };
-    int b = 0, base = I.k0;
+    ob_half8 kf[2][DK], pb[MT];
+    ob_float4 s[MT][2];
     for (; base + 64 <= I.k1; base += 64, b ^= 1) {
-        if (base + 64 < I.k1) store(base + 64, b ^ 1);
-        if (base + 128 < I.k1) load(base + 128);
-        half(b, 0, std::false_type(), 32);
-        half(b, 1, std::false_type(), 32);
-        __syncthreads();
+        if (base + 64 < I.k1) load(base + 64, b ^ 1);
+        keys(0, kf);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const _Float16 *vt = &kv[b][1][32 * h * DP];
+            W.template scores<false>(kf, 32, s);
+            if (h == 0) keys(1, kf);
+            W.weights(s, A.scale_log2e, pb);
+            W.values(vt, pb);
+        }
+        landed();
     }
 #pragma unroll 1
-    for (int h = 0; base + 32 * h < I.k1; ++h) half(b, h, std::true_type(), I.k1 - base - 32 * h);
+    for (int h = 0; base + 32 * h < I.k1; ++h) {
+        keys(h, kf);
+        W.template scores<true>(kf, I.k1 - base - 32 * h, s);
+        W.weights(s, A.scale_log2e, pb);
+        W.values(&kv[b][1][32 * h * DP], pb);
+    }
     ob_sh_store<DP, MT, EXACT>(A, W, G.row0, qi0, nq, I.kvh, I.chunk);
 }
 
