@@ -7,6 +7,7 @@ between calls; calls that may run at the same time (other streams, graphs replay
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -21,18 +22,22 @@ class _Prefix(ctypes.Structure):          # onebit_prefix_t
     _fields_ = [("row0", ctypes.c_int32), ("n", ctypes.c_int32), ("slot", ctypes.c_int32), ("len", ctypes.c_int32), ("first", ctypes.c_int32)]
 
 
-_ARRAYS: dict = {}          # ctypes array types by length
+_PACKED: dict = {}          # struct.Struct by number of values
 
 
-def _prefixes(groups):
+def _prefixes(groups) -> bytes:
+    """The groups as an array of onebit_prefix_t."""
     flat = groups[0] if len(groups) == 1 else [v for g in groups for v in g]
     n = len(flat)
     if n != 5 * len(groups) or any(len(g) != 5 for g in groups):
         raise ValueError(f"groups are (first row, rows, prefix slot, prefix length, first own position) each, not {list(groups)!r}")
-    t = _ARRAYS.get(n)
-    if t is None:
-        t = _ARRAYS[n] = ctypes.c_int32 * n
-    return t(*flat)
+    s = _PACKED.get(n)
+    if s is None:
+        s = _PACKED[n] = struct.Struct(f"{n}i")
+    try:
+        return s.pack(*flat)
+    except struct.error as e:
+        raise ValueError(f"groups' entries must be whole numbers of 32 bits: {list(groups)!r}") from e
 
 
 def _call(name: str, index: int, *args):

@@ -47,6 +47,8 @@ def main(argv=None) -> int:
 
     from .registry import load_model
     from .serving import ContinuousBatcher
+    if a.num_beams == 1 and (a.eos or a.length_penalty != 1.0):
+        ap.error("--eos and --length-penalty belong to a beam search: --num-beams")
     model = load_model(a.model, dtype=None if a.dtype is None else getattr(torch, a.dtype))
     prompts = [[int(t) for t in p.replace(",", " ").split()] for p in a.prompt]
     if a.num_beams != 1:

@@ -147,14 +147,19 @@ def beam_search(engine, prompts: Sequence[Sequence[int]], max_new_tokens: int, e
                 early_stopping: bool = False) -> List[List[Tuple[float, List[int]]]]:
     """Per prompt the finished hypotheses, best first, as (score, tokens): the sum of the new tokens' log probabilities over their number to the power
     ``length_penalty``, an end token counted.  A prompt ends when it has ``beams`` finished hypotheses and (``early_stopping`` or) no live one that would
-    beat the worst of them as it stands, or after ``max_new_tokens``, where the live ones count as finished."""
+    beat the worst of them as it stands, or after ``max_new_tokens``, where the live ones count as finished.  A step looks at beams x (1 + end tokens) candidates, so
+    that ``beams`` go on however many of them end; 64 at most."""
     B, W = len(prompts), engine.beams
     if B != engine.batch or any(len(p) < 1 for p in prompts):
         raise ValueError(f"beam_search: {B} prompts of at least one token for an engine of {engine.batch}")
     if max(len(p) for p in prompts) + max_new_tokens > engine.max_len:
         raise ValueError("beam_search: prompt + max_new_tokens exceeds the engine's slots")
     lengths = [len(p) for p in prompts]
-    keep = min(MAX_KEEP, (1 + max(1, len(eos or ()))) * W)
+    keep = (1 + max(1, len(eos or ()))) * W
+    if keep > MAX_KEEP:
+        raise ValueError(f"beam_search: {W} beams with {len(eos)} end tokens look at {keep} candidates a step, at most {MAX_KEEP} are kept")
+    if max_new_tokens < 1:
+        return [[(0.0, [])] for _ in prompts]
     workspace = beam_select_workspace(B * W, engine.vocab, keep, engine.device)
     logits = engine.prime(prompts)
     engine.spread(lengths)

@@ -147,3 +147,37 @@ def test_finished_hypotheses():
     empty = _Slots(2).p
     empty.take([(float("-inf"), -1, -1)] * 4, None)
     assert empty.done and empty.results() == []
+
+
+class _NoEngine:
+    """A search's engine that must not be asked for anything."""
+    batch, beams, max_len, vocab, device = 1, 32, 100, 50, "cpu"
+
+    def prime(self, prompts):
+        raise AssertionError("nothing to prime")
+
+
+def test_search_refuses_more_candidates_than_are_kept():
+    from onebit_amd.search import beam_search
+    with pytest.raises(ValueError, match="96 candidates"):
+        beam_search(_NoEngine(), [[1, 2]], 5, eos={3, 4})
+
+
+def test_search_of_no_token():
+    from onebit_amd.search import beam_search
+    assert beam_search(_NoEngine(), [[1, 2]], 0) == [[(0.0, [])]]
+
+
+def test_groups_beyond_32_bits():
+    with pytest.raises(ValueError, match="32 bits"):
+        shared_prefix_workspace([(0, 2, 0, 1 << 32, 0)], 2, 4, 4, 64, 10, "cpu")
+    with pytest.raises(ValueError, match="32 bits"):
+        shared_prefix_workspace([(0, 2, -(1 << 40), 3, 0)], 2, 4, 4, 64, 10, "cpu")
+
+
+def test_command_line_refuses_a_search_s_options_without_one(capsys):
+    from onebit_amd.cli import main
+    for extra in (["--eos", "3"], ["--length-penalty", "2"]):
+        with pytest.raises(SystemExit):
+            main(["generate", "--model", "none", "--prompt", "1", *extra])
+        assert "--num-beams" in capsys.readouterr().err
