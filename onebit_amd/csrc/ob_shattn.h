@@ -42,6 +42,7 @@ struct ObShArgs {
     int inline_prefix;                                // the own kernel reads the prefixes itself
     int one_items;                                    // ob_sh_one_kernel: items of the prefixes, in front of the rows'
     int own_blocks;                                   // ob_sh_wide_kernel: workgroups of the rows' own keys among its others
+    int own_alone;                                    // their waves each take a row's keys of a kv head
     int *tickets;                                     // [rows][Hkv] arrivals at a row, zero between launches
     float scale_log2e;                                // log2(e) / sqrt(D)
     int n_groups;
@@ -183,14 +184,15 @@ struct ObShWave {
 struct ObShRange { const _Float16 *k, *v; int begin, end; };
 __device__ __forceinline__ int ob_sh_tiles(int n) { return (n + 31) >> 5; }
 
-// A workgroup's four waves over the keys of two ranges one after the other, 32 in turn; each starts from what W holds, the four results are joined in wave 0's W.
+// A workgroup's four waves over the keys of two ranges one after the other, 32 in turn; each starts from what W holds, the four results are joined in wave 0's W.  STEP 1: every
+// wave goes over ranges of its own, alone.
 // meanwhile(W) runs while the first loads are on their way.
 // K goes from memory to registers in the layout of its product, V by registers into the wave's own part of the LDS: no barrier in the loop, the
 // next 32 keys and values are on their way while a wave computes.
 template <int DP, int MT, bool EXACT> constexpr int ob_sh_body_floats() { return (4 * 32 * DP * 2 > 2 * MT * 16 * DP * 4 ? 4 * 32 * DP * 2 : 2 * MT * 16 * DP * 4) / 4; }
 template <int DP, int MT, bool EXACT> constexpr int ob_sh_lds_floats() { return ob_sh_body_floats<DP, MT, EXACT>() + 4 * MT * 16 * 2; }
 
-template <int DP, int MT, bool EXACT, typename F>
+template <int DP, int MT, bool EXACT, int STEP = 4, typename F>
 __device__ __forceinline__ void ob_sh_sweep(const ObShArgs &A, const ObShRange &R0, const ObShRange &R1, ObShWave<DP, MT, EXACT> &W, float *sm, F meanwhile)
 {
     constexpr int DK = DP / 32, DT = DP / 16, PPR = DP / 8, RPL = 64 / PPR, NV = 32 / RPL;       // pieces of 16 bytes per row, rows per load, loads of a V tile
@@ -224,9 +226,10 @@ __device__ __forceinline__ void ob_sh_sweep(const ObShArgs &A, const ObShRange &
             vr[i] = EXACT || 8 * vpc < D ? *reinterpret_cast<const ob_half8 *>(p) : (ob_half8)(_Float16)0;
         }
     };
-    if (wave < n) { load_v(wave); load_k(wave); }                      // (values first, as in the loop: what waits for them lets the keys come)
+    const int t0 = STEP == 4 ? wave : 0;
+    if (t0 < n) { load_v(t0); load_k(t0); }                            // (values first, as in the loop: what waits for them lets the keys come)
     meanwhile(W);
-    for (int t = wave; t < n; t += 4) {
+    for (int t = t0; t < n; t += STEP) {
         const bool one = t < n0;
         const int end = one ? R0.end : R1.end, base = one ? R0.begin + 32 * t : R1.begin + 32 * (t - n0);
         // rows beyond the range as zeros (their weights are zero, their values may be anything)
@@ -238,16 +241,17 @@ __device__ __forceinline__ void ob_sh_sweep(const ObShArgs &A, const ObShRange &
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        if (t + 4 < n) load_v(t + 4);
+        if (t + STEP < n) load_v(t + STEP);
         ob_half8 pb[MT];
         ob_float4 s[MT][2];
         W.template scores<true>(kf, end - base, s);
         W.weights(s, A.scale_log2e, pb);
-        if (t + 4 < n) load_k(t + 4);
+        if (t + STEP < n) load_k(t + STEP);
         W.values(vt, pb);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
+    if (STEP == 1) return;
     // ---- join the four waves: statistics, then the outputs in two steps through two buffers
     float *st = sm + ob_sh_body_floats<DP, MT, EXACT>();               // [4 waves][16 MT][2]
 #pragma unroll
@@ -423,18 +427,25 @@ __global__ __launch_bounds__(OB_SH_THREADS, 2) void ob_sh_wide_kernel(const ObSh
         ob_sh_wide<DP, MT, EXACT>(A, I, G, kv);
         return;
     }
-    const int item = before / A.Hkv, kvh = before - item * A.Hkv;
+    // (a wave of its own for every row and kv head, or four)
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), unit = A.own_alone ? 4 * before + wave : before;
+    const int item = unit / A.Hkv, kvh = unit - item * A.Hkv;
     const int at = item / A.rows, r = A.row_base + item - at * A.rows, split = at / A.own_mb, mb = at - split * A.own_mb;
+    if (split >= A.osplits) return;
     int gi = 0, slot, own;
     while (r >= A.g[gi].row0 + A.g[gi].n) ++gi;
     const int first = A.g[gi].first;
     if (!ob_sh_row(A, r, first, slot, own) || split * A.ochunk >= own) return;
     const int64_t row = ((int64_t)slot * A.Hkv + kvh) * A.max_len * A.D;
+    const ObShRange keys = {A.k + row, A.v + row, first + split * A.ochunk, first + min(own, (split + 1) * A.ochunk)}, none = {A.k + row, A.v + row, 0, 0};
     ObShWave<DP, 1, EXACT> W;
     W.init(A, r, 16 * mb, A.rep, kvh);
-    ob_sh_sweep<DP, 1, EXACT>(A, {A.k + row, A.v + row, first + split * A.ochunk, first + min(own, (split + 1) * A.ochunk)}, {A.k + row, A.v + row, 0, 0}, W,
-                              reinterpret_cast<float *>(kv), [](auto &) {});
-    if (threadIdx.x < 64) ob_sh_store<DP, 1, EXACT>(A, W, r, 16 * mb, A.rep, kvh, A.psplits + split);
+    if (A.own_alone) ob_sh_sweep<DP, 1, EXACT, 1>(A, keys, none, W, reinterpret_cast<float *>(kv), [](auto &) {});
+    else {
+        ob_sh_sweep<DP, 1, EXACT>(A, keys, none, W, reinterpret_cast<float *>(kv), [](auto &) {});
+        if (wave) return;
+    }
+    ob_sh_store<DP, 1, EXACT>(A, W, r, 16 * mb, A.rep, kvh, A.psplits + split);
 }
 
 // Bound by HBM: 8 rows x 32 heads of 1000 own keys each 24.7 us, 5.3 TB/s.

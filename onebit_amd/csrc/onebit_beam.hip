@@ -19,7 +19,7 @@ static const int64_t OB_SH_MAX_LEN = 1 << 30;         // (positions and their ch
 // ------------------------------------------------------------------------------------------- attention over a shared prefix --
 // form: ob_sh_one_kernel; ob_sh_wide_kernel of 64 / 128 queries and ob_sh_own_kernel; the latter alone.  osplits 0: a row's own keys are one chunk, no part
 enum { OB_SH_INLINE, OB_SH_ONE, OB_SH_WIDE64, OB_SH_WIDE128 };
-struct ObShPlan { int form, per, pchunk, ochunk, psplits, osplits, own_mb; bool among; };
+struct ObShPlan { int form, per, pchunk, ochunk, psplits, osplits, own_mb; bool among, alone; };
 #define OB_SH_TICKETS 16384                           // their place in front of the scratch memory does not depend on a call's sizes
 
 static ObShPlan ob_sh_plan(const onebit_prefix_t *groups, int32_t n_groups, int64_t rows, int32_t n_heads, int32_t n_kv_heads, int64_t max_own)
@@ -59,6 +59,13 @@ static ObShPlan ob_sh_plan(const onebit_prefix_t *groups, int32_t n_groups, int6
     // own keys' workgroups among the prefix's and a launch that joins: 64 x 40 / 40 sharing 2000 with 20 own 37.5 (after them, started from their parts, 44.5), 64 x 32 / 32
     // sharing 8000 49.9 (57.8); with more queries of a row per kv head, whose parts fill the lanes that fetch them, 64 x 64 / 8 sharing 2000 30.7 (23.9)
     p.among = p.form == OB_SH_WIDE64 && rep <= 2;
+    // there a wave of its own for 128 of a row's own keys while those are few: 64 x 40 / 40 sharing 2000 with 20 own, not in the caches, 33 (a workgroup for a row's 43), 48 x 40 / 40
+    // sharing 4000 with 100 50 (56), 64 x 32 / 32 sharing 2040 with 200 60 (64), with 300 82 (81); 64 x 40 / 40 sharing 500 with 500 135 (127)
+    p.alone = p.among && max_own <= 384;
+    if (p.alone) {
+        p.ochunk = 128;
+        p.osplits = (int)ob_up(max_own, p.ochunk);
+    }
     if (p.form == OB_SH_ONE || p.among) p.osplits = std::max(p.osplits, 1);
     else if (p.osplits <= 1) p.osplits = 0;
     // chunks for 256 workgroups where a row's last one joins them (1 x 32 / 32 of 8192 26.8, for 512 29.0; 16 x 32 / 32 of 4000 23.7 and 26.4), for 512 else (64 x 64 / 8
@@ -103,8 +110,9 @@ static void ob_sh_launch(ObShArgs &a, const ObShPlan &p, int64_t prefix_items, i
         hipLaunchKernelGGL((ob_sh_one_kernel<DP, 1, EXACT>), all, block, 0, s, a);
         return;
     }
-    a.own_blocks = p.among ? (int)own.x : 0;
-    const dim3 wide(p.among ? all.x : all.x - own.x);
+    a.own_alone = p.alone;
+    a.own_blocks = p.among ? (int)(p.alone ? ob_up(own.x, 4) : own.x) : 0;
+    const dim3 wide(all.x - own.x + a.own_blocks);
     if (wide.x > 0) {
         if (p.form == OB_SH_WIDE64) hipLaunchKernelGGL((ob_sh_wide_kernel<DP, 1, EXACT>), wide, block, 0, s, a);
         else if (p.form == OB_SH_WIDE128) hipLaunchKernelGGL((ob_sh_wide_kernel<DP, 2, EXACT>), wide, block, 0, s, a);
