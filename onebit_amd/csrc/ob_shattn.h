@@ -120,22 +120,21 @@ struct ObShWave {
     // Their weights
     __device__ __forceinline__ void weights(const ob_float4 (&s)[MT][2], float scale, ob_half8 (&pb)[MT])
     {
-        // the running maximum moves only where a weight exceeds 2^15 (the first ones do), to where the largest is 2^7: the weights stay inside fp16, those of 2^-21 of the
-        // largest and more as normal numbers, and neither the tile's maximum nor a rescaled output is needed otherwise.  Weights are not negative, so their bits order
-        // like whole numbers.
-        const auto exponentials = [&]() {
-            ob_u16x2 most = {0, 0};
+        // the running maximum moves only where a weight would exceed 2^15 (the first ones do), to where the largest is 2^7: the weights stay inside fp16, those of 2^-21 of
+        // the largest and more as normal numbers, and neither the tile's maximum nor a rescaled output is needed otherwise
+        float x[MT][8], top = -INFINITY;
+        const auto exponents = [&]() {
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
+            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) pb[mt][e] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][e >> 2][e & 3], scale, -m[mt]));
-                const ob_u32x4 bits = __builtin_bit_cast(ob_u32x4, pb[mt]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(ob_u16x2, bits[i]));
-            }
-            return __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(most, (ob_u16x2)(unsigned short)0x7800)) != 0;
+                for (int e = 0; e < 8; ++e) x[mt][e] = __builtin_fmaf(s[mt][e >> 2][e & 3], scale, -m[mt]);
         };
-        if (__any(exponentials())) {
+        exponents();
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, x[mt][e]);
+        if (__any(top > 15.f)) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 float mx = s[mt][0][0];
@@ -147,8 +146,12 @@ struct ObShWave {
                 for (int dt = 0; dt < DT; ++dt) acc[mt][dt] *= f;
                 m[mt] = mn;
             }
-            exponentials();
+            exponents();
         }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) pb[mt][e] = (_Float16)__builtin_amdgcn_exp2f(x[mt][e]);
     }
 
     // columns 16 dt .. of the 32 values from vt on, as the second product takes them

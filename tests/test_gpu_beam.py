@@ -181,6 +181,29 @@ def test_large_scores_and_one_far_maximum():
     _check(c, _call(c))
 
 
+@pytest.mark.parametrize("H, hkv, rows, length, own", [(4, 4, 8, 1500, 70), (2, 2, 33, 1500, 70), (16, 2, 20, 9000, 70), (4, 4, 8, 200, 70), (2, 2, 33, 0, 700), (16, 2, 40, 0, 1300),
+                                                       (2, 2, 64, 600, 1500), (64, 2, 9, 40000, 40)])
+@pytest.mark.parametrize("high", [11, 17, 40])
+def test_a_maximum_that_moves_late(H, hkv, rows, length, own, high):
+    """Every query's largest score stands at a place of its own behind many small ones, so far above them that the running maximum has to move there: all 32 places of a step
+    of keys, in prefix and own keys, in all forms."""
+    c = _case([length], [rows], [own - (r % 3) for r in range(rows)], H, hkv, 64, seed=high, scale=0.05)
+    n = H // hkv
+    scores = high * math.log(2.0) * 8.0                                 # (times 1 / sqrt(64), log2 e: `high` in powers of two)
+    q = c["q"]
+    for r in range(rows):
+        for h in range(H):
+            q[r, h, (5 * r + h) % 32] = math.sqrt(scores)
+    for i in range(32):
+        if length:
+            c["pk"][0, :, length - 33 * i - 5 if length > 1100 else length - 5 * i - 3, i] = math.sqrt(scores)
+        else:
+            for s in c["slots"]:
+                c["k"][s, :, own - 19 * i - 4, i] = math.sqrt(scores)
+    assert n * hkv == H
+    _check(c, _call(c))
+
+
 def test_offsets_beyond_32_bits():
     """A prefix in the last slot of a cache whose slots hold 2 GiB each, and own positions far inside a slot."""
     long = (1 << 23) + 40
