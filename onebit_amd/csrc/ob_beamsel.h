@@ -35,7 +35,11 @@ struct ObBsArgs {
     int *list_t;
     float *out_scores; int *out_beams, *out_tokens;      // [groups][keep]
     int *tickets;
+    unsigned inv_room, inv_chunks;   // ob_bs_inverse of a list's places, of a row's chunks
 };
+// n / d for n d < 2^31 as one product
+static inline unsigned ob_bs_inverse(int d) { return (unsigned)(((1u << 31) + (unsigned)d - 1) / (unsigned)d); }
+__device__ __forceinline__ int ob_bs_div(int n, unsigned inverse) { return (int)__umulhi(2u * (unsigned)n, inverse); }
 
 // what a later launch reads, or (AGENT) another workgroup of this one: past the XCD's L2
 template <bool AGENT, typename V> __device__ __forceinline__ void ob_bs_put(V *p, V v)
@@ -113,7 +117,7 @@ __device__ __forceinline__ void ob_bs_pick(const ObBsArgs &A, int group)
 {
     constexpr int WAVES = THREADS / 64, NS = OB_BS_PLACES, RANKED = THREADS;       // candidates that are ranked by counting
     __shared__ double row_v[OB_BS_MAX_BEAMS], cand_v[RANKED];                     // lse of a beam; NaN: it offers nothing
-    __shared__ float pub[WAVES * (OB_BS_MAX_KEEP + 2)], t_s;
+    __shared__ float pub[WAVES * (OB_BS_MAX_KEEP + 2)], t_s, row_s[OB_BS_MAX_BEAMS];
     __shared__ ObBsCand cand[RANKED];
     __shared__ int n_s, lists_s;
     __shared__ unsigned short live[OB_BS_LISTS];
@@ -124,25 +128,22 @@ __device__ __forceinline__ void ob_bs_pick(const ObBsArgs &A, int group)
     const bool by_lists = total > THREADS * NS && lists <= OB_BS_LISTS && lists >= 2 * A.keep;
     const int64_t list0 = (int64_t)group * A.beams * A.chunks;
     if (tid == 0) { n_s = 0; lists_s = 0; t_s = -INFINITY; }
-    struct Place { float x, score; int tok, n, beam, e; };
-    const auto fetch = [&](int l, int e, Place &p) {                             // (all of it at once: what lies behind a list's end is memory of the list, not used)
-        p.e = e;
-        p.beam = l / A.chunks;
-        p.n = ob_bs_get<AGENT>(A.counts + list0 + l);
-        p.x = ob_bs_get<AGENT>(A.list_x + (list0 + l) * room + e);
-        p.tok = ob_bs_get<AGENT>(A.list_t + (list0 + l) * room + e);
-        p.score = A.scores[group * A.beams + p.beam];
+    // place e of list l: its logit (NaN behind the list's end) and token
+    const auto fetch = [&](int l, int e, float &x, int &tok) {                   // (all loads at once: what lies behind a list's end is memory of the list, not used)
+        const int n = ob_bs_get<AGENT>(A.counts + list0 + l);
+        x = ob_bs_get<AGENT>(A.list_x + (list0 + l) * room + e);
+        tok = ob_bs_get<AGENT>(A.list_t + (list0 + l) * room + e);
+        if (e >= n) x = NAN;
     };
-    const auto value = [&](const Place &p, ObBsCand &c) -> bool {                // false where there is no candidate
-        c = {(double)p.score + ((double)p.x - row_v[p.beam]), p.x, p.beam, p.tok};
-        return p.e < p.n && c.v > -INFINITY;                                     // (NaN: none)
-    };
-    Place place[NS];
+    const auto beam_of = [&](int l) { return ob_bs_div(l, A.inv_chunks); };
+    const auto value = [&](float x, int beam) { return (double)row_s[beam] + ((double)x - row_v[beam]); };        // (NaN: no candidate)
+    float px[NS];
+    int ptok[NS];
 #pragma unroll
     for (int k = 0; k < NS; ++k) {
-        const int i = tid + THREADS * k, l = i / room;
-        place[k] = {0.f, 0.f, 0, 0, 0, 0};                                       // (none)
-        if (!by_lists && i < total) fetch(l, i - l * room, place[k]);
+        const int i = tid + THREADS * k, l = ob_bs_div(i, A.inv_room);
+        px[k] = NAN; ptok[k] = 0;
+        if (!by_lists && i < total) fetch(l, i - l * room, px[k], ptok[k]);
     }
     // a chunk's sum in terms of the row's largest logit
     const auto term = [](double m, double part, float M) { return m == -INFINITY ? part : part * exp(m - (double)M); };
@@ -154,7 +155,7 @@ __device__ __forceinline__ void ob_bs_pick(const ObBsArgs &A, int group)
             const double m = ob_bs_get<AGENT>(sm), part = ob_bs_get<AGENT>(sm + 1);
             const float M = ob_bs_row_max(in ? (float)m : -INFINITY);
             const double s = ob_bs_row_sum(in ? term(m, part, M) : 0.);
-            if (b < A.beams && c == 0) row_v[b] = (double)M + log(s);
+            if (b < A.beams && c == 0) { row_v[b] = (double)M + log(s); row_s[b] = A.scores[group * A.beams + b]; }
         }
     else
         for (int b = wave; b < A.beams; b += WAVES) {
@@ -165,20 +166,21 @@ __device__ __forceinline__ void ob_bs_pick(const ObBsArgs &A, int group)
             double s = 0.;
             for (int c = lane; c < A.chunks; c += 64) s += term(ob_bs_get<AGENT>(sm + 2 * c), ob_bs_get<AGENT>(sm + 2 * c + 1), M);
             s = ob_bs_wave_sum(s);
-            if (lane == 0) row_v[b] = (double)M + log(s);
+            if (lane == 0) { row_v[b] = (double)M + log(s); row_s[b] = A.scores[group * A.beams + b]; }
         }
     __syncthreads();
-    // f over all candidate places of this thread
-    const auto each = [&](auto f) {
-        ObBsCand c;
+    // their values, in registers; the other places' (where there are more) with every look at them
+    double pv[NS];
 #pragma unroll
-        for (int k = 0; k < NS; ++k)
-            if (value(place[k], c)) f(c);
+    for (int k = 0; k < NS; ++k) pv[k] = value(px[k], min(beam_of(ob_bs_div(tid + THREADS * k, A.inv_room)), A.beams - 1));
+    const auto others = [&](auto f) {
         for (int i = tid + (by_lists ? 0 : THREADS * NS); i < total; i += THREADS) {
-            Place p;
-            const int l = i / room;
-            fetch(l, i - l * room, p);
-            if (value(p, c)) f(c);
+            const int l = ob_bs_div(i, A.inv_room);
+            ObBsCand c;
+            fetch(l, i - l * room, c.x, c.tok);
+            c.beam = beam_of(l);
+            c.v = value(c.x, c.beam);
+            if (c.v > -INFINITY) f(c);
         }
     };
     const auto keep_it = [&](const ObBsCand &c) {
@@ -191,8 +193,8 @@ __device__ __forceinline__ void ob_bs_pick(const ObBsArgs &A, int group)
         float top[NL];
 #pragma unroll
         for (int k = 0; k < NL; ++k) {
-            const int l = min(tid + THREADS * k, lists - 1), beam = l / A.chunks;
-            const double v = (double)A.scores[group * A.beams + beam] + (ob_bs_get<AGENT>(A.sums + 2 * (list0 + l)) - row_v[beam]);
+            const int l = min(tid + THREADS * k, lists - 1), beam = beam_of(l);
+            const double v = (double)row_s[beam] + (ob_bs_get<AGENT>(A.sums + 2 * (list0 + l)) - row_v[beam]);
             top[k] = tid + THREADS * k < lists && v > -INFINITY ? __double2float_rd(v) : -INFINITY;
             best = fmaxf(best, top[k]);
         }
@@ -207,21 +209,39 @@ __device__ __forceinline__ void ob_bs_pick(const ObBsArgs &A, int group)
         __syncthreads();
         const double t = t_s;
         for (int i = tid; i < lists_s * room; i += THREADS) {
-            Place p;
+            const int at = ob_bs_div(i, A.inv_room);
             ObBsCand c;
-            const int at = i / room;
-            fetch(live[at], i - at * room, p);
-            if (value(p, c) && c.v >= t) keep_it(c);
+            fetch(live[at], i - at * room, c.x, c.tok);
+            c.beam = beam_of(live[at]);
+            c.v = value(c.x, c.beam);
+            if (c.v > -INFINITY && c.v >= t) keep_it(c);
         }
     } else {
-        each([&](const ObBsCand &c) { best = fmaxf(best, __double2float_rd(c.v)); });      // (rounded down: what reaches the threshold reaches it in 64 bits, too)
+        double most = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < NS; ++k) most = fmax(most, pv[k]);
+        others([&](const ObBsCand &c) { most = fmax(most, c.v); });
+        best = __double2float_rd(most);                                          // (rounded down: what reaches the threshold reaches it in 64 bits, too)
         const int waves = min(WAVES, (total + 63) / 64), share = min(64, (A.keep + waves - 1) / waves + 2);
         if (wave < waves) ob_bs_publish(best, share, pub + wave * share);
         __syncthreads();
         if (ob_bs_is_kth(pub, waves * share, A.keep, tid)) t_s = pub[tid];
         __syncthreads();
         const double t = t_s;
-        if (best >= t_s) each([&](const ObBsCand &c) { if (c.v >= t) keep_it(c); });
+        if (best >= t_s) {
+            unsigned left = 0;
+#pragma unroll
+            for (int k = 0; k < NS; ++k) left |= pv[k] >= t && pv[k] > -INFINITY ? 1u << k : 0u;
+            for (; left; left &= left - 1) {                                     // (few: one piece of code for all places)
+                const int k = __builtin_ctz(left);
+                ObBsCand c = {pv[0], px[0], beam_of(ob_bs_div(tid + THREADS * k, A.inv_room)), ptok[0]};
+#pragma unroll
+                for (int j = 1; j < NS; ++j)
+                    if (k == j) { c.v = pv[j]; c.x = px[j]; c.tok = ptok[j]; }
+                keep_it(c);
+            }
+            others([&](const ObBsCand &c) { if (c.v >= t) keep_it(c); });
+        }
     }
     __syncthreads();
     int n = n_s;
@@ -243,7 +263,11 @@ __device__ __forceinline__ void ob_bs_pick(const ObBsArgs &A, int group)
         ObBsCand last = {INFINITY, INFINITY, -1, -1};
         for (n = 0; n < A.keep; ++n) {
             ObBsCand b = {-INFINITY, -INFINITY, 0x7fffffff, 0x7fffffff};
-            each([&](const ObBsCand &c) { if (ob_bs_before(last, c) && ob_bs_before(c, b)) b = c; });
+            const auto look = [&](const ObBsCand &c) { if (ob_bs_before(last, c) && ob_bs_before(c, b)) b = c; };
+#pragma unroll
+            for (int k = 0; k < NS; ++k)
+                if (pv[k] > -INFINITY) look({pv[k], px[k], beam_of(ob_bs_div(tid + THREADS * k, A.inv_room)), ptok[k]});
+            others(look);
             __syncthreads();
             cand[tid] = b;
             __syncthreads();
@@ -263,7 +287,8 @@ template <int THREADS>
 __global__ __launch_bounds__(THREADS) void ob_bs_pick_kernel(const ObBsArgs A) { ob_bs_pick<THREADS, false>(A, blockIdx.x); }
 
 // NV: pieces of 8 elements of a thread, OB_BS_THREADS apart.  PICK: the last workgroup of a group picks.
-// 256 rows of 50257 fp16 12 us (2.1 TB/s; NV = 4 in 72 registers, so that the 1792 workgroups run in one round: 85 registers 13.6), 8 rows of 32000 with the pick 15.5.
+// 256 rows of 50257 fp16 12 us (2.1 TB/s; NV = 4 in 72 registers, so that the 1792 workgroups run in one round: 85 registers 13.6), 8 rows of 32000 with the pick 15. What a launch of few workgroups runs is fetched as it goes: pieces of code that few lanes need are there
+// once, not for every element (8 rows of 32000 16.2, 4 rows of 512 11.1, with one for each).
 template <typename T, int NV, bool PICK>
 __global__ __launch_bounds__(OB_BS_THREADS, PICK ? 4 : NV == 1 ? 8 : 7) void ob_bs_scan_kernel(const ObBsArgs A)
 {
@@ -308,14 +333,15 @@ __global__ __launch_bounds__(OB_BS_THREADS, PICK ? 4 : NV == 1 ? 8 : 7) void ob_
     int *lt = A.list_t + list * room;
     const float least = fmaxf(t, -3.402823466e38f);                             // (-inf is no candidate)
     if (best >= least) {
+        unsigned left = 0;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (x[j][e] >= least) {
-                    const int at = atomicAdd(&n_s, 1);
-                    if (at < room) { ob_bs_put<PICK>(lx + at, x[j][e]); ob_bs_put<PICK>(lt + at, c0 + 8 * (tid + OB_BS_THREADS * j) + e); }
-                }
+            for (int e = 0; e < 8; ++e) left |= x[j][e] >= least ? 1u << (8 * j + e) : 0u;
+        for (; left; left &= left - 1) {                                         // (few: one piece of code for all elements, their logits read again)
+            const int k = __builtin_ctz(left), tok = c0 + 8 * (tid + OB_BS_THREADS * (k >> 3)) + (k & 7), at = atomicAdd(&n_s, 1);
+            if (at < room) { ob_bs_put<PICK>(lx + at, (float)x_row[tok]); ob_bs_put<PICK>(lt + at, tok); }
+        }
     }
     double s = 0.;                                                              // (a NaN makes the row's sum NaN, +inf as well)
     if (m > -INFINITY) {

@@ -244,6 +244,7 @@ extern "C" int onebit_beam_select(const void *logits, int64_t ld, int dtype, con
     ObBsArgs a = {};
     const ObBsPlan p = ob_bs_plan(groups, beams, vocab, keep);
     a.logits = logits; a.ld = ld; a.scores = scores; a.beams = beams; a.keep = keep; a.vocab = (int)vocab; a.chunks = p.chunks; a.vecs = p.vecs;
+    a.inv_room = ob_bs_inverse(ob_bs_list(keep)); a.inv_chunks = ob_bs_inverse(p.chunks);
     const size_t lists = (size_t)rows * p.chunks;
     a.tickets = (int *)scratch;
     a.sums = (double *)(a.tickets + OB_BS_TICKETS);
