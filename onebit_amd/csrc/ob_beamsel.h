@@ -287,8 +287,9 @@ template <int THREADS>
 __global__ __launch_bounds__(THREADS) void ob_bs_pick_kernel(const ObBsArgs A) { ob_bs_pick<THREADS, false>(A, blockIdx.x); }
 
 // NV: pieces of 8 elements of a thread, OB_BS_THREADS apart.  PICK: the last workgroup of a group picks.
-// 256 rows of 50257 fp16 12 us (2.1 TB/s; NV = 4 in 72 registers, so that the 1792 workgroups run in one round: 85 registers 13.6), 8 rows of 32000 with the pick 15. What a launch of few workgroups runs is fetched as it goes: pieces of code that few lanes need are there
-// once, not for every element (8 rows of 32000 16.2, 4 rows of 512 11.1, with one for each).
+// 256 rows of 50257 fp16 11.5 us (2.2 TB/s; NV = 4 in 72 registers, so that the 1792 workgroups run in one round: in 85 two us more), 8 rows of 32000 with the pick 15.
+// What a launch of few workgroups runs is fetched as it goes: code that few lanes need is there once, not for every element (8 rows of 32000 16.2, 4 rows of 512 11.1, with
+// one for each).
 template <typename T, int NV, bool PICK>
 __global__ __launch_bounds__(OB_BS_THREADS, PICK ? 4 : NV == 1 ? 8 : 7) void ob_bs_scan_kernel(const ObBsArgs A)
 {

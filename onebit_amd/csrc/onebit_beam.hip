@@ -51,9 +51,9 @@ static ObShPlan ob_sh_plan(const onebit_prefix_t *groups, int32_t n_groups, int6
         for (int i = 0; i < n_groups; ++i) n += ob_up(groups[i].n * rep, per) * groups[i].len * n_kv_heads;
         return n;
     };
-    // up to 32 queries of a group and kv head in blocks of 16, one launch: 17 x 32 / 32 sharing 1000 14.3 (blocks of 64 16.8), 32 x 32 / 32 sharing 4000 31.7 (34.1), 4 rows x
-    // 8 groups x 40 / 40 up to 2000 38.1 (47.0); more: 64 x 32 / 32 sharing 8000 54.0 (49.9), 48 x 32 / 8 sharing 2000 23.9 (17.7).
-    // Blocks of 128 where 512 workgroups of them have 512 keys and more: 64 x 64 / 8 sharing 32768 107 (of 64 139), sharing 8000 44.6 (45.3), 48 x 32 / 8 sharing 2000 20.4 (17.7)
+    // up to 32 queries of a group and kv head in blocks of 16, one launch: 17 x 32 / 32 sharing 1000 15.0 (blocks of 64 16.7), 32 x 32 / 32 sharing 4000 27.8 (31.0), 4 rows x
+    // 8 groups x 40 / 40 of 2000 82 (91); more: 64 x 32 / 32 sharing 8000 56.8 (48.8), 48 x 32 / 8 sharing 2000 23.6 (17.7).
+    // Blocks of 128 where 512 workgroups of them have 512 keys and more: 64 x 64 / 8 sharing 32768 95 (of 64 108), sharing 8000 41 (39), 48 x 32 / 8 sharing 2000 19.8 (17.4)
     p.form = most <= 32 && rows * n_kv_heads <= OB_SH_TICKETS ? OB_SH_ONE : most > 64 && tiles(128) >= 512 * 512 ? OB_SH_WIDE128 : OB_SH_WIDE64;
     p.per = p.form == OB_SH_ONE ? 16 : p.form == OB_SH_WIDE64 ? 64 : 128;
     // own keys' workgroups among the prefix's and a launch that joins: 64 x 40 / 40 sharing 2000 with 20 own 37.5 (after them, started from their parts, 44.5), 64 x 32 / 32
@@ -69,7 +69,7 @@ static ObShPlan ob_sh_plan(const onebit_prefix_t *groups, int32_t n_groups, int6
     if (p.form == OB_SH_ONE || p.among) p.osplits = std::max(p.osplits, 1);
     else if (p.osplits <= 1) p.osplits = 0;
     // chunks for 256 workgroups where a row's last one joins them (1 x 32 / 32 of 8192 26.8, for 512 29.0; 16 x 32 / 32 of 4000 23.7 and 26.4), for 512 else (64 x 64 / 8
-    // sharing 32768 101 of the prefix, for 256 149), no fewer than 256 keys (32 x 32 / 8 sharing 8192 28.7, from 128 on 35.0)
+    // sharing 32768 79 of the prefix, for 256 118), no fewer than 256 keys (32 x 32 / 8 sharing 8192 28.7, from 128 on 35.0)
     p.pchunk = (int)(128 * std::max<int64_t>(p.form == OB_SH_ONE ? 1 : 2, ob_up(tiles(p.per), (p.form == OB_SH_ONE ? 256 : 512) * 128)));
     p.psplits = (int)ob_up(longest, p.pchunk);
     return p;
