@@ -204,6 +204,33 @@ def test_a_maximum_that_moves_late(H, hkv, rows, length, own, high):
     _check(c, _call(c))
 
 
+@pytest.mark.parametrize("D", [128, 64, 80, 40])
+@pytest.mark.parametrize("length", [8192, 8301])
+def test_blocks_of_128_queries(D, length):
+    """Tiles brought by DMA, whole and padded heads, a last tile that is not full, a second group without a prefix."""
+    _check(c := _case([length, 0], [63, 1], [1 + (7 * r) % 40 for r in range(64)], 64, 1, D, seed=D, idle=(5,)), _call(c))
+
+
+@pytest.mark.parametrize("H, hkv, rows, length, own", [(4, 4, 40, 2000, 50), (64, 1, 64, 8200, 20), (4, 4, 40, 2000, 500), (2, 1, 6, 20000, 30)])
+def test_every_replay_of_a_graph_is_the_eager_call(H, hkv, rows, length, own):
+    c = _case([length], [rows], [1 + (own * ((5 * r) % rows)) // rows for r in range(rows)], H, hkv, 128, seed=rows)
+    ws = shared_prefix_workspace(c["groups"], rows, H, hkv, 128, own)
+    out = torch.zeros_like(c["q"])
+    _call(c, out=out, workspace=ws, max_own=own)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _call(c, out=out, workspace=ws, max_own=own)
+    for i in range(3):
+        c["q"].copy_(torch.randn_like(c["q"]))
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        y = out.clone()
+        assert torch.equal(_call(c, max_own=own), y)
+    _check(c, y)
+
+
 def test_offsets_beyond_32_bits():
     """A prefix in the last slot of a cache whose slots hold 2 GiB each, and own positions far inside a slot."""
     long = (1 << 23) + 40
