@@ -22,22 +22,15 @@ class _Prefix(ctypes.Structure):          # onebit_prefix_t
     _fields_ = [("row0", ctypes.c_int32), ("n", ctypes.c_int32), ("slot", ctypes.c_int32), ("len", ctypes.c_int32), ("first", ctypes.c_int32)]
 
 
-_PACKED: dict = {}          # struct.Struct by number of values
+_GROUP = struct.Struct("5i")          # onebit_prefix_t
 
 
 def _prefixes(groups) -> bytes:
     """The groups as an array of onebit_prefix_t."""
-    flat = groups[0] if len(groups) == 1 else [v for g in groups for v in g]
-    n = len(flat)
-    if n != 5 * len(groups) or any(len(g) != 5 for g in groups):
-        raise ValueError(f"groups are (first row, rows, prefix slot, prefix length, first own position) each, not {list(groups)!r}")
-    s = _PACKED.get(n)
-    if s is None:
-        s = _PACKED[n] = struct.Struct(f"{n}i")
     try:
-        return s.pack(*flat)
+        return _GROUP.pack(*groups[0]) if len(groups) == 1 else b"".join([_GROUP.pack(*g) for g in groups])
     except struct.error as e:
-        raise ValueError(f"groups' entries must be whole numbers of 32 bits: {list(groups)!r}") from e
+        raise ValueError(f"groups are (first row, rows, prefix slot, prefix length, first own position) each, whole numbers of 32 bits, not {list(groups)!r}") from e
 
 
 def _call(name: str, index: int, *args):
@@ -117,13 +110,18 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: Optional[torch.Tensor], p
         raise ValueError(f"{what}: prefix keys without values, or values without keys")
     if row_pos is None:
         raise ValueError(f"{what}: row_pos is needed")
-    if not (row_pos.dtype is _I32 and row_pos.shape == (rows,) and row_pos.is_contiguous()) or row_slot is not None:
-        _check_rows(what, rows, row_pos=row_pos, row_slot=row_slot)
-    scale = None
+    if not (row_pos.dtype is _I32 and row_pos.dim() == 1 and row_pos.numel() == rows and row_pos.is_contiguous()):
+        _check_rows(what, rows, row_pos=row_pos)
+    slot, scale, where = None, None, index
+    if row_slot is not None:
+        if not (row_slot.dtype is _I32 and row_slot.dim() == 1 and row_slot.numel() == rows and row_slot.is_contiguous()):
+            _check_rows(what, rows, row_slot=row_slot)
+        slot, where = row_slot.data_ptr(), row_slot.get_device()
     if h_next is not None:
         if h_next.dtype is not _F16 or h_next.numel() != heads * dim or not h_next.is_contiguous():
             raise ValueError(f"{what}: h_next must be contiguous float16 of {heads * dim} entries")
         scale = h_next.data_ptr()
+        where = where if h_next.get_device() == index else -1
     if out is None:
         out = torch.zeros_like(q)
     elif out.shape != shape or out.dtype is not _F16 or not out.is_contiguous() or out.data_ptr() == q.data_ptr() != 0:
@@ -135,10 +133,10 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: Optional[torch.Tensor], p
         workspace = shared_prefix_workspace(groups, rows, heads, kv_heads, dim, max_own, q.device)
     elif workspace.dtype is not _U8 or not workspace.is_contiguous():
         raise ValueError(f"{what}: the workspace must be contiguous uint8")
-    _on(index, what, k_cache, v_cache, row_slot, row_pos, h_next, out, workspace)
+    if not (k_cache.get_device() == index == v_cache.get_device() == row_pos.get_device() == out.get_device() == workspace.get_device()) or where != index:
+        _on(index, what, k_cache, v_cache, row_slot, row_pos, h_next, out, workspace)
     _call("onebit_attention_shared_rows", index, q.data_ptr(), p_k, p_v, k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), scale, arr, len(groups),
-          None if row_slot is None else row_slot.data_ptr(), row_pos.data_ptr(), rows, heads, kv_heads, dim, p_slots, p_len, slots, max_len, max_own,
-          workspace.data_ptr(), workspace.numel())
+          slot, row_pos.data_ptr(), rows, heads, kv_heads, dim, p_slots, p_len, slots, max_len, max_own, workspace.data_ptr(), workspace.numel())
     return out
 
 
@@ -169,9 +167,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, keep: in
     elif workspace.dtype is not _U8 or not workspace.is_contiguous():
         raise ValueError("beam_select: the workspace must be contiguous uint8")
     index = logits.get_device()
-    _on(index, "beam_select", scores, workspace)
+    if not scores.get_device() == index == workspace.get_device():
+        _on(index, "beam_select", scores, workspace)
     groups = rows // beams
-    packed = torch.empty((3, groups, keep), dtype=_I32, device=logits.device)
+    packed = torch.empty_strided((3, groups, keep), (groups * keep, keep, 1), dtype=_I32, device=logits.device)
     p, ld = packed.data_ptr(), logits.stride(0)
     if rows == 1:
         ld = max(ld, vocab)
