@@ -365,7 +365,7 @@ __device__ __forceinline__ void ob_sh_wide(const ObShArgs &A, const ObShItem &I,
     const int row = lane / PPR, at = lane % PPR;
     const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) char *)&kv[0][0][0];
     const auto load = [&](int base, int b) {
-        const int most = I.k1 - 1 - base;                                        // (rows behind the last one: the last one again, its weights are zero)
+        const int most = I.k1 - 1 - base;                                        // (rows behind the last one: the last one again; its scores there are left out, its values written over)
         const char *kb = reinterpret_cast<const char *>(I.kb + (int64_t)base * D), *vb = reinterpret_cast<const char *>(I.vb + (int64_t)base * D);
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
@@ -408,6 +408,10 @@ __device__ __forceinline__ void ob_sh_wide(const ObShArgs &A, const ObShItem &I,
             W.values(vt, pb);
         }
         landed();
+    }
+    if (base < I.k1) {                                                           // a last tile that is not full: weights of zero, and values that no infinity is among
+        for (int i = (I.k1 - base) * PPR + tid; i < 64 * PPR; i += OB_SH_THREADS) *reinterpret_cast<ob_half8 *>(&kv[b][1][8 * i]) = (ob_half8)(_Float16)0;
+        __syncthreads();
     }
 #pragma unroll 1
     for (int h = 0; base + 32 * h < I.k1; ++h) {

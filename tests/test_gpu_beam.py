@@ -204,6 +204,34 @@ def test_a_maximum_that_moves_late(H, hkv, rows, length, own, high):
     _check(c, _call(c))
 
 
+@pytest.mark.parametrize("H, hkv, rows, length, own, D", [(4, 4, 8, 200, 70, 64), (4, 4, 8, 1501, 70, 128), (2, 2, 33, 1509, 70, 64), (2, 2, 33, 1571, 70, 40), (16, 2, 20, 4001, 70, 128),
+                                                          (2, 2, 64, 1541, 1500, 64), (64, 1, 64, 8301, 37, 128), (64, 1, 64, 8193, 37, 80), (16, 2, 40, 0, 1299, 64), (40, 40, 64, 999, 9, 64)])
+def test_infinities_and_nan_in_values(H, hkv, rows, length, own, D):
+    """A value that is infinite or NaN makes that column of its rows infinite or NaN and no other, also in the last row of a prefix or of a row's own positions, in all
+    forms: no place behind a range takes part in the products."""
+    c = _case([length], [rows], [own] * rows, H, hkv, D, seed=length + D, scale=0.5)
+    col = dict(zip((3, 7, 11), (math.inf, -math.inf, math.nan)))
+    for d, bad in col.items():
+        if length:
+            c["pv"][0, :, length - 1, d] = bad
+        c["v"][c["slots"][0], :, own - 1, d + 1] = bad
+    y = _call(c)
+    for d, bad in col.items():
+        same = torch.isnan if math.isnan(bad) else lambda t, bad=bad: t == bad
+        if length:
+            assert same(y[:, :, d]).all(), (d, bad)
+            c["pv"][0, :, length - 1, d] = 0
+        assert same(y[0, :, d + 1]).all(), (d, bad)
+        c["v"][c["slots"][0], :, own - 1, d + 1] = 0
+    clean = _call(c)
+    ref, tol = _reference(c)
+    for d in col:
+        if length:
+            y[:, :, d] = clean[:, :, d]
+        y[0, :, d + 1] = clean[0, :, d + 1]
+    assert torch.isfinite(y).all() and ((y.double() - ref).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("D", [128, 64, 80, 40])
 @pytest.mark.parametrize("length", [8192, 8301])
 def test_blocks_of_128_queries(D, length):
