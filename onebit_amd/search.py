@@ -164,7 +164,7 @@ def beam_search(engine, prompts: Sequence[Sequence[int]], max_new_tokens: int, e
     logits = engine.prime(prompts)
     engine.spread(lengths)
     states = [_Prompt(W, length_penalty, early_stopping) for _ in prompts]
-    live, scores, per = list(range(B)), torch.zeros(B, device=engine.device), 1
+    live, scores, per = list(range(B)), torch.zeros(B, dtype=torch.float32, device=engine.device), 1
     for step in range(max_new_tokens):
         v, b, t = (x.tolist() for x in beam_select(logits, scores, per, keep, workspace=workspace))
         moves, moved = [list(range(W)) for _ in range(B)], False
@@ -184,7 +184,7 @@ def beam_search(engine, prompts: Sequence[Sequence[int]], max_new_tokens: int, e
             flat += [h[0] for h in hyps] + [-math.inf] * len(spare)
         if moved and step:
             engine.move(torch.tensor(moves, dtype=torch.int32).to(engine.device), min(lengths[i] for i in live), max(lengths[i] for i in live) + step)
-        scores, per = torch.tensor(flat).to(engine.device), W
+        scores, per = torch.tensor(flat, dtype=torch.float32).to(engine.device), W
         logits = engine.advance(live, slots, tokens, {i: lengths[i] + step for i in live}, lengths)
     return [s.results() for s in states]
 

@@ -100,6 +100,18 @@ def test_search_on_a_table(batch, beams, vocab, n_new, eos, penalty, early):
     assert eng.moves > 0 or beams == 1 or vocab - len(eos) == 1          # (one token that does not end: one path)
 
 
+@pytest.mark.parametrize("default", [torch.float64, torch.float16])
+def test_search_under_another_default_type(default):
+    """Scores are float32 whatever type new tensors have."""
+    eng = Table(2, 3, 41, seed=5)
+    want = beam_search(eng, [[1], [2, 3]], 6)
+    torch.set_default_dtype(default)
+    try:
+        assert beam_search(eng, [[1], [2, 3]], 6) == want
+    finally:
+        torch.set_default_dtype(torch.float32)
+
+
 def test_search_refusals():
     eng = Table(2, 3, 11, seed=1)
     for prompts, n in (([[1]], 4), ([[1], []], 4), ([[1], [2]], 1000)):
