@@ -569,7 +569,7 @@ int onebit_fused_gemv(const onebit_proj_t *projs, void *const *outs, int nproj, 
  *   [n_prefix_slots][n_kv_heads][prefix_max_len][D], own cache [n_slots][n_kv_heads][max_len][D]; D a multiple of 8, at most 128.
  *   max_own: bound on row_pos - g.first + 1 over the rows; positions beyond it are NOT attended.  Scores, statistics and sums fp32, the
  *   weights rounded to fp16 before the value product.  Deterministic.
- *   o overlaps no input.  scratch: onebit_attention_shared_scratch_bytes() of the same groups and sizes or more, 16-byte aligned, ZERO-FILLED ONCE: the
+ *   o and scratch overlap no input and not each other (refused).  scratch: onebit_attention_shared_scratch_bytes() of the same groups and sizes or more, 16-byte aligned, ZERO-FILLED ONCE: the
  *   counters in front of it (16384 int32, whatever the sizes) are zero again after every call.  Not shared by calls that may run at the same time
  *   (the function returns 0 where the arguments are refused). */
 typedef struct onebit_prefix { int32_t row0, n, slot, len, first; } onebit_prefix_t;

@@ -83,7 +83,7 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: Optional[torch.Tensor], p
     in order; a group's rows attend to positions 0 .. length - 1 of ``slot`` in ``prefix_k`` / ``prefix_v`` [prefix slots, kv heads, prefix positions, D],
     and row r to positions first .. row_pos[r] of slot ``row_slot[r]`` (None: slot r) in ``k_cache`` / ``v_cache`` [slots, kv heads, positions, D].  The two
     pairs may be the same tensors; without any prefix the first may be None.  ``row_slot`` / ``row_pos``: int32 on the device; a row whose slot
-    or position lies outside is idle and keeps what ``out`` holds (zeros without ``out``).  ``max_own``: bound on the rows' own positions, those
+    or position lies outside is idle and keeps what ``out`` holds (zeros without ``out``).  ``out`` overlaps no input.  ``max_own``: bound on the rows' own positions, those
     beyond it are not attended (None: all that fit the cache).  ``h_next`` [heads * D]: the result times this."""
     what = "shared_prefix_attention"
     _require_gpu(q, what)

@@ -16,6 +16,14 @@ static inline int64_t ob_up(int64_t n, int64_t m) { return (n + m - 1) / m; }
 static const int64_t OB_MAX_WGS = 0xffffff;            // workgroups of 256 threads of one launch
 static const int64_t OB_SH_MAX_LEN = 1 << 30;         // (positions and their chunks are counted in 32 bits)
 
+// memory of a call (sizes of products that may pass 64 bits)
+struct ObMem { const void *p; unsigned __int128 n; };
+static inline bool ob_overlap(const ObMem &a, const ObMem &b)
+{
+    const unsigned __int128 x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+    return a.p && b.p && a.n && b.n && x < y + b.n && y < x + a.n;
+}
+
 // ------------------------------------------------------------------------------------------- attention over a shared prefix --
 // form: ob_sh_one_kernel; ob_sh_wide_kernel of 64 / 128 queries and ob_sh_own_kernel; the latter alone.  osplits 0: a row's own keys are one chunk, no part
 enum { OB_SH_INLINE, OB_SH_ONE, OB_SH_WIDE64, OB_SH_WIDE128 };
@@ -146,6 +154,15 @@ extern "C" int onebit_attention_shared_rows(const void *q, const void *prefix_k,
         return ob_fail(ONEBIT_E_ALIGN, "attention_shared_rows: q and the caches must be 16-byte aligned");
     const size_t need = onebit_attention_shared_scratch_bytes(groups, n_groups, rows, n_heads, n_kv_heads, head_dim, max_own);
     if (!scratch || scratch_bytes < need || !ob_aligned(scratch, 16)) return ob_fail(ONEBIT_E_WSPACE, "attention_shared_rows: needs %zu bytes of zero-initialised, 16-byte aligned scratch", need);
+    const auto mem = [](const void *p, int64_t n0, int64_t n1, int64_t n2, int64_t n3) { return ObMem{p, (unsigned __int128)n0 * n1 * n2 * n3}; };
+    const ObMem out = mem(o, rows, n_heads, head_dim, 2), work = {scratch, need};
+    const int64_t pre = prefixes ? prefix_max_len : 0;
+    const ObMem in[] = {mem(q, rows, n_heads, head_dim, 2), mem(k_cache, n_slots, n_kv_heads, max_len, head_dim * 2), mem(v_cache, n_slots, n_kv_heads, max_len, head_dim * 2),
+                        mem(prefix_k, n_prefix_slots, n_kv_heads, pre, head_dim * 2), mem(prefix_v, n_prefix_slots, n_kv_heads, pre, head_dim * 2), mem(h_next, n_heads, head_dim, 2, 1),
+                        mem(row_slot, rows, 4, 1, 1), mem(row_pos, rows, 4, 1, 1)};
+    bool overlap = ob_overlap(out, work);
+    for (const ObMem &m : in) overlap = overlap || ob_overlap(out, m) || ob_overlap(work, m);
+    if (overlap) return ob_fail(ONEBIT_E_ARG, "attention_shared_rows: the output and the scratch memory overlap nothing else");
     const ObShPlan p = ob_sh_plan(groups, n_groups, rows, n_heads, n_kv_heads, max_own);
     const int64_t rep = n_heads / n_kv_heads;
     ObShArgs a = {};

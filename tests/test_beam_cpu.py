@@ -181,3 +181,32 @@ def test_command_line_refuses_a_search_s_options_without_one(capsys):
         with pytest.raises(SystemExit):
             main(["generate", "--model", "none", "--prompt", "1", *extra])
         assert "--num-beams" in capsys.readouterr().err
+
+
+def _pieces():
+    """Addresses in one allocation, 1 MiB apart (never launched on: every call below is refused)."""
+    b = ctypes.create_string_buffer(17 << 20)
+    a = (ctypes.addressof(b) + 255) & ~255
+    return b, [a + (i << 20) for i in range(16)]
+
+
+def test_attention_refuses_overlaps():
+    """q, o [2, 4, 64] 1024 bytes, own caches [2, 2, 16, 64] 8192, prefix caches [1, 2, 10, 64] 2560, row indices 8: one byte into any of them, from either end."""
+    keep, p = _pieces()
+    lib = _lib.load()
+    arr = (_Prefix * 1)(_Prefix(0, 2, 0, 10, 0))
+    size = dict(q=1024, pk=2560, pv=2560, k=8192, v=8192, o=1024, h=512, slot=8, pos=8)
+    size["ws"] = lib.onebit_attention_shared_scratch_bytes(arr, 1, 2, 4, 2, 64, 16)
+    at = dict(zip(size, p))
+
+    def call(**kw):
+        w = {**at, **kw}
+        return lib.onebit_attention_shared_rows(w["q"], w["pk"], w["pv"], w["k"], w["v"], w["o"], w["h"], arr, 1, w["slot"], w["pos"], 2, 4, 2, 64, 1, 10, 2, 16, 16,
+                                                w["ws"], size["ws"], None)
+    for written in ("o", "ws"):
+        step = 8 if written == "o" else 16
+        for other in size:
+            if other == written:
+                continue
+            for where in (at[other], at[other] - size[written] + step, at[other] + (size[other] - 1) // step * step):
+                assert call(**{written: where}) == E_ARG and b"overlap" in lib.onebit_last_error(), (written, other, where - at[other])

@@ -382,6 +382,19 @@ def test_attention_python_refusals():
             _call(c, **b)
 
 
+def test_an_output_beside_its_inputs_but_not_over_them():
+    c = _case([700], [3], [5, 1, 20], 4, 4, 64)
+    want = _call(c)
+    both = torch.zeros(6, 4, 64, dtype=F16, device="cuda")
+    both[:3] = c["q"]
+    c["q"] = both[:3]
+    assert torch.equal(_call(c, out=both[3:]), want) and torch.equal(both[3:], want)
+    for out in (both[1:4], both[2:5], c["k"].view(-1)[40:40 + 768].view(3, 4, 64), c["pv"].view(-1)[-768:].view(3, 4, 64)):
+        with pytest.raises(ValueError, match="overlap"):
+            _call(c, out=out)
+    assert torch.equal(_call(c), want)
+
+
 # ------------------------------------------------------------------------------------------------------- the choice of hypotheses --
 def _best(logits, scores, beams, keep):
     """The definition on the CPU: every continuation of every hypothesis, in the documented order."""
