@@ -176,20 +176,28 @@ extern "C" int onebit_attention_shared_rows(const void *q, const void *prefix_k,
     a.tickets = (int *)scratch;
     a.part_o = (float *)scratch + OB_SH_TICKETS;
     a.part_ml = a.part_o + parts * head_dim;
+    const auto chunks_of = [&](const onebit_prefix_t &g) { return p.form == OB_SH_INLINE ? 0 : ob_up(g.len, p.pchunk); };
+    for (int g0 = 0; g0 < n_groups; g0 += OB_SH_GROUPS) {                        // (all launches are looked at before the first)
+        int64_t items = 0;
+        for (int i = g0; i < std::min(n_groups, g0 + OB_SH_GROUPS); ++i) {
+            const int64_t chunks = chunks_of(groups[i]);
+            items += (chunks ? chunks * ob_up(groups[i].n * rep, p.per) : 0) + (int64_t)groups[i].n * p.own_mb * std::max(p.osplits, 1);
+        }
+        if (items * n_kv_heads > OB_MAX_WGS) return ob_fail(ONEBIT_E_ARG, "attention_shared_rows: too many workgroups");
+    }
     for (int g0 = 0; g0 < n_groups; g0 += OB_SH_GROUPS) {
         a.n_groups = std::min(n_groups - g0, OB_SH_GROUPS);
         a.row_base = groups[g0].row0; a.rows = 0;
         int64_t items = 0;
         for (int i = 0; i < a.n_groups; ++i) {
             const onebit_prefix_t &g = groups[g0 + i];
-            const int64_t chunks = a.inline_prefix ? 0 : ob_up(g.len, p.pchunk);
+            const int64_t chunks = chunks_of(g);
             items += chunks ? chunks * ob_up(g.n * rep, p.per) : 0;
             a.g[i] = {g.row0, g.n, g.slot, g.len, g.first, (int)chunks, (int)items};
             a.rows += g.n;
         }
         const int64_t own_items = (int64_t)a.rows * p.own_mb * std::max(p.osplits, 1);
         a.one_items = (int)items;
-        if ((items + own_items) * n_kv_heads > OB_MAX_WGS) return ob_fail(ONEBIT_E_ARG, "attention_shared_rows: too many workgroups");
         hipStream_t s = (hipStream_t)stream;
         if (head_dim == 128) ob_sh_launch<128, true>(a, p, items, own_items, s);
         else if (head_dim == 64) ob_sh_launch<64, true>(a, p, items, own_items, s);

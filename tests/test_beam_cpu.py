@@ -210,3 +210,13 @@ def test_attention_refuses_overlaps():
                 continue
             for where in (at[other], at[other] - size[written] + step, at[other] + (size[other] - 1) // step * step):
                 assert call(**{written: where}) == E_ARG and b"overlap" in lib.onebit_last_error(), (written, other, where - at[other])
+
+
+def test_attention_refuses_too_many_workgroups_before_the_first_launch():
+    """64 groups of a row, which one launch takes, then 65471 rows of 512 key heads, 2^25 workgroups."""
+    lib = _lib.load()
+    groups = [(r, 1, 0, 0, 0) for r in range(64)] + [(64, 65471, 0, 0, 0)]
+    arr = (_Prefix * 65)(*[_Prefix(*g) for g in groups])
+    at = [(i + 1) << 40 for i in range(6)]
+    rc = lib.onebit_attention_shared_rows(at[0], None, None, at[1], at[2], at[3], None, arr, 65, None, at[4], 65535, 512, 512, 8, 0, 0, 65535, 16, 16, at[5], 1 << 39, None)
+    assert rc == E_ARG and b"too many workgroups" in lib.onebit_last_error()
