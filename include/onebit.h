@@ -594,7 +594,7 @@ int onebit_beam_select(const void *logits, int64_t ld, int dtype, const float *s
  * g * beams + parents[g][b] held, for any map (parents: device int32 [groups, beams]; one outside 0 .. beams - 1 leaves the slot as it is).
  * A slot is slot_bytes apart from the next and has `outer` rows, outer_bytes apart, of which bytes first_byte .. + n_bytes move: with caches
  * [slots][n_kv_heads][max_len][head_dim] the positions that differ between hypotheses.  Whole 16 bytes everywhere (sizes and addresses) run
- * fastest, whole 4 next.  Buffers do not overlap.  beams <= 32. */
+ * fastest, whole 4 next.  Buffers do not overlap each other, nor the parents (refused).  beams <= 32. */
 int onebit_reorder_slots(void *const *buffers, int32_t n_buffers, const int32_t *parents, int64_t groups, int32_t beams, int64_t slot_bytes,
                          int64_t outer, int64_t outer_bytes, int64_t first_byte, int64_t n_bytes, void *stream);
 

@@ -183,7 +183,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, keep: in
 def reorder_slots(buffers: Sequence[torch.Tensor], parents: torch.Tensor, slot0: int = 0, first: int = 0, count: Optional[int] = None) -> None:
     """In every buffer [slots, ...], slot ``slot0 + g * beams + b`` takes what slot ``slot0 + g * beams + parents[g, b]`` held, in place and for any map
     (``onebit_reorder_slots``); ``parents`` int32 [groups, beams] on the device, an entry outside 0 .. beams - 1 leaves its slot as it is.  With ``count``,
-    buffers are caches [slots, heads, positions, D] of which positions ``first`` .. ``first + count - 1`` move.  Any dtype; buffers do not overlap."""
+    buffers are caches [slots, heads, positions, D] of which positions ``first`` .. ``first + count - 1`` move.  Any dtype; buffers overlap neither each other nor ``parents``."""
     if parents.dim() != 2 or parents.dtype is not _I32 or not parents.is_contiguous():
         raise ValueError("reorder_slots: parents must be a contiguous int32 [groups, beams]")
     _require_gpu(parents, "reorder_slots")

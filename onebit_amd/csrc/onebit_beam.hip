@@ -315,6 +315,9 @@ extern "C" int onebit_reorder_slots(void *const *buffers, int32_t n_buffers, con
         if (!buffers[i]) return ob_fail(ONEBIT_E_ARG, "reorder_slots: null buffer %d", i);
         low |= (uint64_t)(uintptr_t)buffers[i];
     }
+    for (int i = 0; i < n_buffers; ++i)                                          // (workgroups that come later would read what others have written)
+        if (ob_overlap({buffers[i], (unsigned __int128)groups * beams * slot_bytes}, {parents, (unsigned __int128)groups * beams * 4}))
+            return ob_fail(ONEBIT_E_ARG, "reorder_slots: the parents overlap buffer %d", i);
     const int unit = low % 16 == 0 ? 16 : low % 4 == 0 ? 4 : 1;
     ObReArgs a = {};
     a.parents = parents; a.slot_bytes = slot_bytes; a.outer_bytes = outer_bytes; a.first_byte = first_byte; a.beams = beams;

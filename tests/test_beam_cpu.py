@@ -220,3 +220,13 @@ def test_attention_refuses_too_many_workgroups_before_the_first_launch():
     at = [(i + 1) << 40 for i in range(6)]
     rc = lib.onebit_attention_shared_rows(at[0], None, None, at[1], at[2], at[3], None, arr, 65, None, at[4], 65535, 512, 512, 8, 0, 0, 65535, 16, 16, at[5], 1 << 39, None)
     assert rc == E_ARG and b"too many workgroups" in lib.onebit_last_error()
+
+
+def test_reorder_refuses_parents_inside_a_buffer():
+    """Two buffers of 4 slots of 256 bytes, parents of 16 bytes: at either end of either buffer."""
+    keep, p = _pieces()
+    lib = _lib.load()
+    for first in (0, 1):
+        bufs = (ctypes.c_void_p * 2)(p[first], p[1 - first])
+        for at in (p[0] - 12, p[0], p[0] + 1020):
+            assert lib.onebit_reorder_slots(bufs, 2, at, 1, 4, 256, 2, 128, 0, 128, None) == E_ARG and b"overlap" in lib.onebit_last_error()

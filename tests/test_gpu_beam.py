@@ -637,3 +637,14 @@ def test_reorder_refusals():
     whole = torch.zeros(16, 4, 64, device="cuda")
     with pytest.raises(ValueError, match="overlap"):
         reorder_slots([whole, whole[4:]], p)
+
+
+def test_reorder_refuses_parents_inside_a_buffer():
+    t = torch.zeros(4, 2, 16, 64, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="overlap"):
+        reorder_slots([torch.zeros_like(t), t], t[3, 0, 0, :4].view(1, 4))
+    both = torch.zeros(4 * 64 + 4, dtype=torch.int32, device="cuda")                        # (beside it they are fine)
+    both[:256] = torch.arange(256)
+    both[256:] = torch.tensor([3, 1, 0, 2])
+    reorder_slots([both[:256].view(4, 64)], both[256:].view(1, 4))
+    assert torch.equal(both[:256].view(4, 64).cpu(), torch.arange(256, dtype=torch.int32).view(4, 64)[[3, 1, 0, 2]])
