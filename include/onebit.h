@@ -586,7 +586,7 @@ int onebit_attention_shared_rows(const void *q, const void *prefix_k, const void
  * [groups, keep].  A continuation of v = -inf or NaN (a banned token, a dead hypothesis, a row with a NaN or +inf) is none; places that remain
  * hold -inf, -1, -1.  beams 1 .. 32, keep 1 .. 64, vocab <= 2^20, groups * beams <= 65535.  scratch: onebit_beam_select_scratch_bytes(groups * beams, vocab, keep)
  * bytes or more, 16-byte aligned, ZERO-FILLED ONCE (4096 int32 in front of it are zero again after every call); not shared by calls that may run at the
- * same time. */
+ * same time.  Outputs and scratch overlap no input and not each other (refused). */
 size_t onebit_beam_select_scratch_bytes(int64_t rows, int64_t vocab, int32_t keep);
 int onebit_beam_select(const void *logits, int64_t ld, int dtype, const float *scores, int64_t groups, int32_t beams, int64_t vocab, int32_t keep,
                        float *out_scores, int32_t *out_beams, int32_t *out_tokens, void *scratch, size_t scratch_bytes, void *stream);

@@ -266,6 +266,13 @@ extern "C" int onebit_beam_select(const void *logits, int64_t ld, int dtype, con
     const int64_t rows = groups * beams;
     const size_t need = onebit_beam_select_scratch_bytes(rows, vocab, keep);
     if (!scratch || scratch_bytes < need || !ob_aligned(scratch, 16)) return ob_fail(ONEBIT_E_WSPACE, "beam_select: needs %zu bytes of zero-initialised, 16-byte aligned scratch", need);
+    // (a group's results are written while others' scores and logits are still read)
+    const unsigned __int128 n_out = (unsigned __int128)groups * keep * 4;
+    const ObMem mem[] = {{out_scores, n_out}, {out_beams, n_out}, {out_tokens, n_out}, {scratch, need}, {scores, (unsigned __int128)rows * 4},
+                         {logits, ((unsigned __int128)(rows - 1) * ld + vocab) * (dtype == ONEBIT_F16 ? 2 : 4)}};
+    for (int i = 0; i < 4; ++i)
+        for (int j = i + 1; j < 6; ++j)
+            if (ob_overlap(mem[i], mem[j])) return ob_fail(ONEBIT_E_ARG, "beam_select: outputs and scratch memory overlap nothing else");
     ObBsArgs a = {};
     const ObBsPlan p = ob_bs_plan(groups, beams, vocab, keep);
     a.logits = logits; a.ld = ld; a.scores = scores; a.beams = beams; a.keep = keep; a.vocab = (int)vocab; a.chunks = p.chunks; a.vecs = p.vecs;

@@ -230,3 +230,22 @@ def test_reorder_refuses_parents_inside_a_buffer():
         bufs = (ctypes.c_void_p * 2)(p[first], p[1 - first])
         for at in (p[0] - 12, p[0], p[0] + 1020):
             assert lib.onebit_reorder_slots(bufs, 2, at, 1, 4, 256, 2, 128, 0, 128, None) == E_ARG and b"overlap" in lib.onebit_last_error()
+
+
+def test_select_refuses_overlaps():
+    """2 groups of 4 rows of 100 fp32 logits (pitch 128: 3984 bytes), 8 kept: one entry into any other piece of memory, from either end."""
+    keep, p = _pieces()
+    lib = _lib.load()
+    size = dict(out=64, beam=64, token=64, ws=lib.onebit_beam_select_scratch_bytes(8, 100, 8), scores=32, x=(7 * 128 + 100) * 4)
+    at = dict(zip(size, p))
+
+    def call(**kw):
+        w = {**at, **kw}
+        return lib.onebit_beam_select(w["x"], 128, 1, w["scores"], 2, 4, 100, 8, w["out"], w["beam"], w["token"], w["ws"], size["ws"], None)
+    for written in ("out", "beam", "token", "ws"):
+        step = 16 if written == "ws" else 4
+        for other in size:
+            if other == written:
+                continue
+            for where in (at[other], at[other] - size[written] + step, at[other] + (size[other] - 1) // step * step):
+                assert call(**{written: where // step * step}) == E_ARG and b"overlap" in lib.onebit_last_error(), (written, other, where - at[other])
