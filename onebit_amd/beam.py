@@ -2,7 +2,8 @@
 hypotheses from their logits, and their states brought to the slots that go on with them.
 
 All three enqueue on the current stream of their tensors' device and never synchronise; they can be captured into a HIP graph (host
-arguments -- the groups, lengths, positions -- are fixed by the capture, device tensors are read by every replay).  A workspace may be kept
+arguments -- the groups, lengths, positions -- are fixed by the capture, device tensors are read by every replay).  Results carry no
+gradients; tensors that require them are refused unless gradients are off.  A workspace may be kept
 between calls; calls that may run at the same time (other streams, graphs replayed next to each other) need one each.  There is no CPU fallback."""
 from __future__ import annotations
 
@@ -45,6 +46,7 @@ def _call(name: str, index: int, *args):
         _lib.check(rc, name)
 
 
+_grad = torch.is_grad_enabled
 _get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _raw_stream = _raw if _raw is not None else lambda index: _stream_ptr(torch.device("cuda", index))
 _F16, _F32, _I32, _U8 = torch.float16, torch.float32, torch.int32, torch.uint8
@@ -54,6 +56,10 @@ def _on(index: int, what: str, *tensors):
     for t in tensors:
         if t is not None and t.get_device() != index:
             raise ValueError(f"{what}: tensors on cuda:{index} and {t.device}")
+
+
+def _no_gradient(what: str):
+    raise ValueError(f"{what}: serves only, there is no backward pass: call it under torch.no_grad(), or with tensors that do not require gradients")
 
 
 def _check_rows(what: str, rows: int, **tensors):
@@ -86,6 +92,9 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: Optional[torch.Tensor], p
     or position lies outside is idle and keeps what ``out`` holds (zeros without ``out``).  ``out`` overlaps no input.  ``max_own``: bound on the rows' own positions, those
     beyond it are not attended (None: all that fit the cache).  ``h_next`` [heads * D]: the result times this."""
     what = "shared_prefix_attention"
+    if _grad() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad or (prefix_k is not None and prefix_k.requires_grad) or
+                    (prefix_v is not None and prefix_v.requires_grad) or (h_next is not None and h_next.requires_grad) or (out is not None and out.requires_grad)):
+        _no_gradient(what)
     _require_gpu(q, what)
     shape = q.shape
     if len(shape) != 3 or q.dtype is not _F16 or not q.is_contiguous():
@@ -151,6 +160,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, keep: in
     float32 (rows may be strided), ``scores`` float32 [groups * beams], the hypotheses' sums of log probabilities.  Returns scores (float32), beams and
     tokens (int32), [groups, keep] each, best first: views of one int32 tensor [3, groups, keep].  Values are ranked in 64 bits; equal ones by beam, logit,
     token.  A continuation of probability zero is none: places that remain hold -inf, -1, -1."""
+    if _grad() and (logits.requires_grad or scores.requires_grad):
+        _no_gradient("beam_select")
     _require_gpu(logits, "beam_select")
     shape = logits.shape
     if len(shape) != 2 or (shape[1] > 1 and logits.stride(1) != 1):
@@ -186,6 +197,9 @@ def reorder_slots(buffers: Sequence[torch.Tensor], parents: torch.Tensor, slot0:
     buffers are caches [slots, heads, positions, D] of which positions ``first`` .. ``first + count - 1`` move.  Any dtype; buffers overlap neither each other nor ``parents``."""
     if parents.dim() != 2 or parents.dtype is not _I32 or not parents.is_contiguous():
         raise ValueError("reorder_slots: parents must be a contiguous int32 [groups, beams]")
+    buffers = list(buffers)
+    if _grad() and True in [t.requires_grad for t in buffers]:
+        _no_gradient("reorder_slots")
     _require_gpu(parents, "reorder_slots")
     groups, beams = parents.shape
     if not 1 <= beams <= MAX_BEAMS:

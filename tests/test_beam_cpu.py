@@ -249,3 +249,23 @@ def test_select_refuses_overlaps():
                 continue
             for where in (at[other], at[other] - size[written] + step, at[other] + (size[other] - 1) // step * step):
                 assert call(**{written: where // step * step}) == E_ARG and b"overlap" in lib.onebit_last_error(), (written, other, where - at[other])
+
+
+def test_tensors_that_require_gradients_are_refused():
+    half = lambda *s: torch.zeros(*s, dtype=torch.float16)
+    pos, groups = torch.zeros(2, dtype=torch.int32), [(0, 2, 0, 4, 0)]
+    for i in range(6):
+        t = [half(2, 4, 64), half(1, 4, 4, 64), half(1, 4, 4, 64), half(2, 4, 16, 64), half(2, 4, 16, 64), half(256)]
+        t[i].requires_grad_()
+        call = lambda: shared_prefix_attention(t[0], t[1], t[2], t[3], t[4], groups, None, pos, h_next=t[5])
+        with pytest.raises(ValueError, match="no backward"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU fallback"):                    # (refused for the next reason only)
+            call()
+    for i in range(2):
+        t = [torch.zeros(4, 10), torch.zeros(4)]
+        t[i].requires_grad_()
+        with pytest.raises(ValueError, match="no backward"):
+            beam_select(t[0], t[1], 4, 8)
+    with pytest.raises(ValueError, match="no backward"):
+        reorder_slots([half(2, 8), half(2, 8).requires_grad_()], torch.zeros(1, 2, dtype=torch.int32))
