@@ -160,6 +160,12 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, keep: in
     float32 (rows may be strided), ``scores`` float32 [groups * beams], the hypotheses' sums of log probabilities.  Returns scores (float32), beams and
     tokens (int32), [groups, keep] each, best first: views of one int32 tensor [3, groups, keep].  Values are ranked in 64 bits; equal ones by beam, logit,
     token.  A continuation of probability zero is none: places that remain hold -inf, -1, -1."""
+    values, beam, token = select_packed(logits, scores, beams, keep, workspace).unbind(0)
+    return values.view(_F32), beam, token
+
+
+def select_packed(logits: torch.Tensor, scores: torch.Tensor, beams: int, keep: int, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``beam_select``'s int32 tensor [3, groups, keep] as one: the scores' bits, beams, tokens."""
     if _grad() and (logits.requires_grad or scores.requires_grad):
         _no_gradient("beam_select")
     _require_gpu(logits, "beam_select")
@@ -187,8 +193,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, keep: in
         ld = max(ld, vocab)
     _call("onebit_beam_select", index, logits.data_ptr(), ld, _dtype_code(logits.dtype), scores.data_ptr(), groups, beams, vocab, keep, p,
           p + 4 * groups * keep, p + 8 * groups * keep, workspace.data_ptr(), workspace.numel())
-    values, beam, token = packed.unbind(0)
-    return values.view(_F32), beam, token
+    return packed
 
 
 def reorder_slots(buffers: Sequence[torch.Tensor], parents: torch.Tensor, slot0: int = 0, first: int = 0, count: Optional[int] = None) -> None:

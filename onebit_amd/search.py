@@ -12,7 +12,7 @@ from typing import Dict, List, Optional, Sequence, Set, Tuple
 
 import torch
 
-from .beam import MAX_BEAMS, MAX_KEEP, beam_select, beam_select_workspace, reorder_slots
+from .beam import MAX_BEAMS, MAX_KEEP, beam_select_workspace, reorder_slots, select_packed
 
 _PRIME_ROWS = 8192          # prompt tokens of one step, unless a single prompt has more
 
@@ -166,7 +166,8 @@ def beam_search(engine, prompts: Sequence[Sequence[int]], max_new_tokens: int, e
     states = [_Prompt(W, length_penalty, early_stopping) for _ in prompts]
     live, scores, per = list(range(B)), torch.zeros(B, dtype=torch.float32, device=engine.device), 1
     for step in range(max_new_tokens):
-        v, b, t = (x.tolist() for x in beam_select(logits, scores, per, keep, workspace=workspace))
+        found = select_packed(logits, scores, per, keep, workspace).cpu()
+        v, b, t = found[0].view(torch.float32).tolist(), found[1].tolist(), found[2].tolist()
         moves, moved = [list(range(W)) for _ in range(B)], False
         for g, i in enumerate(live):
             moves[i] = states[i].take(list(zip(v[g], b[g], t[g])), eos)

@@ -112,6 +112,17 @@ def test_search_under_another_default_type(default):
         torch.set_default_dtype(torch.float32)
 
 
+def test_one_copy_to_the_host_a_step(monkeypatch):
+    copies = []
+    for name in ("tolist", "cpu", "item"):
+        def count(self, *args, _plain=getattr(torch.Tensor, name), **kw):
+            copies.append(self.is_cuda)
+            return _plain(self, *args, **kw)
+        monkeypatch.setattr(torch.Tensor, name, count)
+    beam_search(Table(3, 1, 41, seed=5), [[1], [2], [3]], 7)          # (one hypothesis each: nothing moves)
+    assert sum(copies) == 7
+
+
 def test_search_refusals():
     eng = Table(2, 3, 11, seed=1)
     for prompts, n in (([[1]], 4), ([[1], []], 4), ([[1], [2]], 1000)):
