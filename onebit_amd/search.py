@@ -170,8 +170,10 @@ def beam_search(engine, prompts: Sequence[Sequence[int]], max_new_tokens: int, e
         v, b, t = found[0].view(torch.float32).tolist(), found[1].tolist(), found[2].tolist()
         moves, moved = [list(range(W)) for _ in range(B)], False
         for g, i in enumerate(live):
-            moves[i] = states[i].take(list(zip(v[g], b[g], t[g])), eos)
-            moved = moved or moves[i] != list(range(W))
+            parents = states[i].take(list(zip(v[g], b[g], t[g])), eos)
+            if not states[i].done:                                       # (nobody reads an ended prompt's slots again)
+                moves[i] = parents
+                moved = moved or parents != list(range(W))
         live = [i for i in live if not states[i].done]
         if not live or step + 1 == max_new_tokens:
             break

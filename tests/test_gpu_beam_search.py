@@ -123,6 +123,32 @@ def test_one_copy_to_the_host_a_step(monkeypatch):
     assert sum(copies) == 7
 
 
+class Script(Table):
+    """Logits as given, by step and row."""
+
+    def __init__(self, batch, beams, steps):
+        super().__init__(batch, beams, len(steps[0][0]), seed=1)
+        self.steps = [torch.tensor(s).cuda() for s in steps]
+
+    def prime(self, prompts):
+        return self.steps.pop(0)
+
+    def advance(self, live, slots, tokens, positions, lengths):
+        return self.steps.pop(0)
+
+
+def test_a_prompt_that_has_ended_moves_nothing():
+    """In the second step the first prompt's two hypotheses end and its better one would go on twice; the second prompt's go on where they are."""
+    low = -30.0
+    first = [[low, 1.0, 0.0, low, low], [low, 1.0, 0.0, low, low]]
+    both = [[5.0, low, 0.0, -0.1, low], [5.0, low, -9.0, low, low], [low, low, 5.0, low, low], [low, low, low, 5.0, low]]
+    last = [[low, low, 5.0, low, low], [low, low, low, 5.0, low]]
+    eng = Script(2, 2, [first, both, last])
+    found = beam_search(eng, [[1], [2]], 3, eos={0}, early_stopping=True)
+    assert [t for _, t in found[0]] == [[1, 0], [2, 0]] and [t for _, t in found[1]] == [[1, 2, 2], [2, 3, 3]]
+    assert eng.moves == 0
+
+
 def test_search_refusals():
     eng = Table(2, 3, 11, seed=1)
     for prompts, n in (([[1]], 4), ([[1], []], 4), ([[1], [2]], 1000)):
