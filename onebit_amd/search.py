@@ -142,6 +142,13 @@ class _Prompt:
         return self.finished
 
 
+def _candidates(beams: int, eos: Optional[Set[int]]) -> int:
+    keep = (1 + max(1, len(eos or ()))) * beams
+    if keep > MAX_KEEP:
+        raise ValueError(f"beam_search: {beams} beams with {len(eos or ())} end tokens look at {keep} candidates a step, at most {MAX_KEEP} are kept")
+    return keep
+
+
 @torch.no_grad()
 def beam_search(engine, prompts: Sequence[Sequence[int]], max_new_tokens: int, eos: Optional[Set[int]] = None, length_penalty: float = 1.0,
                 early_stopping: bool = False) -> List[List[Tuple[float, List[int]]]]:
@@ -155,9 +162,7 @@ def beam_search(engine, prompts: Sequence[Sequence[int]], max_new_tokens: int, e
     if max(len(p) for p in prompts) + max_new_tokens > engine.max_len:
         raise ValueError("beam_search: prompt + max_new_tokens exceeds the engine's slots")
     lengths = [len(p) for p in prompts]
-    keep = (1 + max(1, len(eos or ()))) * W
-    if keep > MAX_KEEP:
-        raise ValueError(f"beam_search: {W} beams with {len(eos)} end tokens look at {keep} candidates a step, at most {MAX_KEEP} are kept")
+    keep = _candidates(W, eos)
     if max_new_tokens < 1:
         return [[(0.0, [])] for _ in prompts]
     workspace = beam_select_workspace(B * W, engine.vocab, keep, engine.device)
@@ -197,6 +202,9 @@ def beam_rows(model, prompts: List[List[int]], max_new_tokens: int, max_position
     """The best hypothesis of every prompt (its new tokens, an end token last if it ended), on slots kept per (prompts, beams, length bucket) in ``engines``."""
     if not 1 <= beams <= MAX_BEAMS:
         raise ValueError(f"num_beams must be in 1 .. {MAX_BEAMS}")
+    _candidates(beams, eos)                                              # (what a search would refuse, before its slots take memory)
+    if not prompts or not all(prompts):
+        raise ValueError("beam search needs prompts of at least one token")
     longest = max(len(p) for p in prompts) + max_new_tokens
     if longest > max_positions:
         raise ValueError("prompt + max_new_tokens exceeds max_position_embeddings")

@@ -269,3 +269,17 @@ def test_tensors_that_require_gradients_are_refused():
             beam_select(t[0], t[1], 4, 8)
     with pytest.raises(ValueError, match="no backward"):
         reorder_slots([half(2, 8), half(2, 8).requires_grad_()], torch.zeros(1, 2, dtype=torch.int32))
+
+
+def test_what_a_search_refuses_takes_no_memory(monkeypatch):
+    """More end tokens than candidates are kept, a prompt of no token: no engine is built, and none is kept."""
+    from onebit_amd import search
+
+    def build(*args):
+        raise AssertionError("an engine for a search that is refused")
+    monkeypatch.setattr(search, "LlamaBeams", build)
+    engines = {}
+    for prompts, beams, eos in (([[1, 2]], 32, {3, 4}), ([[1], []], 2, None), ([], 2, None)):
+        with pytest.raises(ValueError):
+            search.beam_rows(object(), prompts, 5, 100, engines, beams, eos)
+    assert not engines
