@@ -199,7 +199,8 @@ def beam_search(engine, prompts: Sequence[Sequence[int]], max_new_tokens: int, e
 
 def beam_rows(model, prompts: List[List[int]], max_new_tokens: int, max_positions: int, engines: Dict, beams: int, eos=None, length_penalty: float = 1.0,
               early_stopping: bool = False) -> List[List[int]]:
-    """The best hypothesis of every prompt (its new tokens, an end token last if it ended), on slots kept per (prompts, beams, length bucket) in ``engines``."""
+    """The best hypothesis of every prompt (its new tokens, an end token last if it ended), on slots that stay in ``engines`` until a search of other
+    (prompts, beams, length bucket) needs its own."""
     if not 1 <= beams <= MAX_BEAMS:
         raise ValueError(f"num_beams must be in 1 .. {MAX_BEAMS}")
     _candidates(beams, eos)                                              # (what a search would refuse, before its slots take memory)
@@ -211,6 +212,8 @@ def beam_rows(model, prompts: List[List[int]], max_new_tokens: int, max_position
     key = ("beams", len(prompts), beams, min(-(-longest // 256) * 256, max_positions))
     eng = engines.get(key)
     if eng is None:
+        for k in [k for k in engines if k[0] == "beams"]:                # (prompts x (beams + 1) slots of the whole length each: one search's at a time)
+            del engines[k]
         if len(engines) >= 4:
             engines.clear()
         from .hybrid import HybridDecoder

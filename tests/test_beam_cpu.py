@@ -283,3 +283,20 @@ def test_what_a_search_refuses_takes_no_memory(monkeypatch):
         with pytest.raises(ValueError):
             search.beam_rows(object(), prompts, 5, 100, engines, beams, eos)
     assert not engines
+
+
+def test_slots_of_one_search_at_a_time(monkeypatch):
+    """An engine that is kept serves the next search of its sizes; one for other sizes takes its place, next to what greedy generation keeps."""
+    from onebit_amd import search
+    built, engines, greedy = [], {(2, 256): "greedy"}, {(2, 256)}
+
+    class Engine:
+        def __init__(self, model, batch, beams, max_len):
+            assert set(engines) == greedy                            # (the old one's memory is free before the new one's is taken)
+            built.append((batch, beams, max_len))
+    monkeypatch.setattr(search, "LlamaBeams", Engine)
+    monkeypatch.setattr(search, "beam_search", lambda eng, prompts, *a: [[(0.0, [1])] for _ in prompts])
+    for prompts, new in (([[1]], 5), ([[1]], 9), ([[1]], 300), ([[1], [2]], 300), ([[1]], 5)):
+        search.beam_rows(object(), prompts, new, 1000, engines, 4)
+        assert len(engines) == 2
+    assert built == [(1, 4, 256), (1, 4, 512), (2, 4, 512), (1, 4, 256)]
