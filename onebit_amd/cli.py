@@ -34,7 +34,7 @@ def main(argv=None) -> int:
     g.add_argument("--dtype", choices=["bfloat16", "float16", "float32"], help="default: the family's serving format")
     g.add_argument("--prompt", action="append", required=True, help="token ids, comma-separated; repeat for more requests")
     g.add_argument("--max-new-tokens", type=int, default=32)
-    g.add_argument("--max-batch", type=int, default=32)
+    g.add_argument("--max-batch", type=int, default=32, help="requests at a time (of a beam search: prompts)")
     g.add_argument("--prefill-chunk", type=int, help="prompt tokens of a request per step (default: whole prompts)")
     g.add_argument("--num-beams", type=int, default=1, help="hypotheses per prompt of a beam search (default: greedy)")
     g.add_argument("--length-penalty", type=float, default=1.0)
@@ -49,12 +49,16 @@ def main(argv=None) -> int:
     from .serving import ContinuousBatcher
     if a.num_beams == 1 and (a.eos or a.length_penalty != 1.0):
         ap.error("--eos and --length-penalty belong to a beam search: --num-beams")
+    if a.num_beams != 1 and a.prefill_chunk is not None:
+        ap.error("--prefill-chunk belongs to greedy generation: a beam search (--num-beams) takes whole prompts")
     model = load_model(a.model, dtype=None if a.dtype is None else getattr(torch, a.dtype))
     prompts = [[int(t) for t in p.replace(",", " ").split()] for p in a.prompt]
     if a.num_beams != 1:
         from .registry import find_family
         from .search import beam_rows
-        rows = beam_rows(model, prompts, a.max_new_tokens, find_family(a.model).max_positions(model), {}, a.num_beams, set(a.eos) if a.eos else None, a.length_penalty)
+        limit, engines, rows = find_family(a.model).max_positions(model), {}, []
+        for i in range(0, len(prompts), max(a.max_batch, 1)):
+            rows += beam_rows(model, prompts[i:i + max(a.max_batch, 1)], a.max_new_tokens, limit, engines, a.num_beams, set(a.eos) if a.eos else None, a.length_penalty)
         for i, row in enumerate(rows):
             print(json.dumps({"request": i, "tokens": row}))
         return 0

@@ -300,3 +300,28 @@ def test_slots_of_one_search_at_a_time(monkeypatch):
         search.beam_rows(object(), prompts, new, 1000, engines, 4)
         assert len(engines) == 2
     assert built == [(1, 4, 256), (1, 4, 512), (2, 4, 512), (1, 4, 256)]
+
+
+def test_command_line_searches_max_batch_prompts_at_a_time(monkeypatch, capsys):
+    import types
+
+    import onebit_amd.registry as registry
+    import onebit_amd.search as search
+    from onebit_amd.cli import main
+    calls = []
+
+    def rows(model, prompts, new, limit, engines, beams, eos, penalty):
+        calls.append((prompts, id(engines)))
+        return [[p[0] + 100] for p in prompts]
+    monkeypatch.setattr(search, "beam_rows", rows)
+    monkeypatch.setattr(registry, "load_model", lambda *a, **kw: None)
+    monkeypatch.setattr(registry, "find_family", lambda path: types.SimpleNamespace(max_positions=lambda model: 64))
+    argv = ["generate", "--model", "none", "--num-beams", "3"] + [x for i in range(5) for x in ("--prompt", str(i))]
+    assert main(argv + ["--max-batch", "2"]) == 0
+    assert [p for p, _ in calls] == [[[0], [1]], [[2], [3]], [[4]]] and len({e for _, e in calls}) == 1
+    assert capsys.readouterr().out.splitlines() == [f'{{"request": {i}, "tokens": [{100 + i}]}}' for i in range(5)]
+    calls.clear()
+    assert main(argv) == 0 and len(calls) == 1
+    with pytest.raises(SystemExit):
+        main(argv + ["--prefill-chunk", "8"])
+    assert "--prefill-chunk" in capsys.readouterr().err
