@@ -463,6 +463,18 @@ def test_more_candidates_than_a_list_holds(vocab, beams, keep, banned, values):
     _check_select(x, scores, beams, keep)
 
 
+@pytest.mark.parametrize("vocab", [600000, (1 << 20) - 3])
+@pytest.mark.parametrize("values", ["many", "few"])
+def test_more_lists_than_the_pick_chooses_from_first(vocab, values):
+    """32 hypotheses of 74 and of 128 chunks each: every place of every list is looked at."""
+    g = torch.Generator(device="cuda").manual_seed(vocab % 97)
+    x = 2 * torch.randn(32, vocab, generator=g, device="cuda")
+    if values == "few":
+        x = x.round()
+    x[:, :vocab // 3] = -math.inf
+    _check_select(x.half(), -10 - 2 * torch.rand(32, generator=g, device="cuda"), 32, 64)
+
+
 def test_equal_rows_at_every_alignment_have_equal_values():
     """Rows of an odd pitch begin at all alignments; the sums must not depend on it, or ties between beams would break."""
     g = torch.Generator(device="cuda").manual_seed(1)
