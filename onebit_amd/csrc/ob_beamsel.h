@@ -111,21 +111,22 @@ __device__ __forceinline__ bool ob_bs_before(const ObBsCand &a, const ObBsCand &
 
 #define OB_BS_PLACES 8                                                            // candidate places of a thread of the pick that stay in registers
 
-// THREADS: 256 or 1024
+// THREADS: 256, where their registers hold all places of a group, or 1024
 template <int THREADS, bool AGENT>
 __device__ __forceinline__ void ob_bs_pick(const ObBsArgs &A, int group)
 {
     constexpr int WAVES = THREADS / 64, NS = OB_BS_PLACES, RANKED = THREADS;       // candidates that are ranked by counting
+    constexpr bool MORE = THREADS > 256;                                          // places beyond the registers
     __shared__ double row_v[OB_BS_MAX_BEAMS], cand_v[RANKED];                     // lse of a beam; NaN: it offers nothing
     __shared__ float pub[WAVES * (OB_BS_MAX_KEEP + 2)], t_s, row_s[OB_BS_MAX_BEAMS];
     __shared__ ObBsCand cand[RANKED];
     __shared__ int n_s, lists_s;
-    __shared__ unsigned short live[OB_BS_LISTS];
+    __shared__ unsigned short live[MORE ? OB_BS_LISTS : 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int room = ob_bs_list(A.keep), lists = A.beams * A.chunks, total = lists * room;
     // more places than registers, in many lists: a threshold from the lists' largest logits first, then the lists that reach it alone (32 rows of 128256, 64 kept: 84 ->
     // 42 us of both kernels)
-    const bool by_lists = total > THREADS * NS && lists <= OB_BS_LISTS && lists >= 2 * A.keep;
+    const bool by_lists = MORE && total > THREADS * NS && lists <= OB_BS_LISTS && lists >= 2 * A.keep;
     const int64_t list0 = (int64_t)group * A.beams * A.chunks;
     if (tid == 0) { n_s = 0; lists_s = 0; t_s = -INFINITY; }
     // place e of list l: its logit (NaN behind the list's end) and token
@@ -174,7 +175,7 @@ __device__ __forceinline__ void ob_bs_pick(const ObBsArgs &A, int group)
 #pragma unroll
     for (int k = 0; k < NS; ++k) pv[k] = value(px[k], min(beam_of(ob_bs_div(tid + THREADS * k, A.inv_room)), A.beams - 1));
     const auto others = [&](auto f) {
-        for (int i = tid + (by_lists ? 0 : THREADS * NS); i < total; i += THREADS) {
+        if constexpr (MORE) for (int i = tid + (by_lists ? 0 : THREADS * NS); i < total; i += THREADS) {
             const int l = ob_bs_div(i, A.inv_room);
             ObBsCand c;
             fetch(l, i - l * room, c.x, c.tok);
@@ -188,7 +189,7 @@ __device__ __forceinline__ void ob_bs_pick(const ObBsArgs &A, int group)
         if (k < RANKED) { cand_v[k] = c.v; cand[k] = c; }
     };
     float best = -INFINITY;
-    if (by_lists) {
+    if (MORE && by_lists) {
         constexpr int NL = OB_BS_LISTS / THREADS;
         float top[NL];
 #pragma unroll
