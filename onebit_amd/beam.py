@@ -202,9 +202,6 @@ def reorder_slots(buffers: Sequence[torch.Tensor], parents: torch.Tensor, slot0:
     buffers are caches [slots, heads, positions, D] of which positions ``first`` .. ``first + count - 1`` move.  Any dtype; buffers overlap neither each other nor ``parents``."""
     if parents.dim() != 2 or parents.dtype is not _I32 or not parents.is_contiguous():
         raise ValueError("reorder_slots: parents must be a contiguous int32 [groups, beams]")
-    buffers = list(buffers)
-    if _grad() and True in [t.requires_grad for t in buffers]:
-        _no_gradient("reorder_slots")
     _require_gpu(parents, "reorder_slots")
     groups, beams = parents.shape
     if not 1 <= beams <= MAX_BEAMS:
@@ -216,7 +213,10 @@ def reorder_slots(buffers: Sequence[torch.Tensor], parents: torch.Tensor, slot0:
     index, slots = parents.get_device(), slot0 + groups * beams
     shapes: dict = {}
     shape = dtype = into = None
+    grad = _grad()
     for t in buffers:
+        if grad and t.requires_grad:
+            _no_gradient("reorder_slots")
         if not t.is_contiguous() or t.get_device() != index:
             raise ValueError(f"reorder_slots: a buffer {tuple(t.shape)} on {t.device} must be contiguous and on {parents.device}")
         if t.shape != shape or t.dtype != dtype:

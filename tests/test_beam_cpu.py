@@ -267,8 +267,6 @@ def test_tensors_that_require_gradients_are_refused():
         t[i].requires_grad_()
         with pytest.raises(ValueError, match="no backward"):
             beam_select(t[0], t[1], 4, 8)
-    with pytest.raises(ValueError, match="no backward"):
-        reorder_slots([half(2, 8), half(2, 8).requires_grad_()], torch.zeros(1, 2, dtype=torch.int32))
 
 
 def test_what_a_search_refuses_takes_no_memory(monkeypatch):

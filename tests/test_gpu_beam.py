@@ -660,3 +660,13 @@ def test_reorder_refuses_parents_inside_a_buffer():
     both[256:] = torch.tensor([3, 1, 0, 2])
     reorder_slots([both[:256].view(4, 64)], both[256:].view(1, 4))
     assert torch.equal(both[:256].view(4, 64).cpu(), torch.arange(256, dtype=torch.int32).view(4, 64)[[3, 1, 0, 2]])
+
+
+def test_reorder_refuses_buffers_that_require_gradients():
+    t, p = torch.arange(8.0, device="cuda").view(4, 2), torch.tensor([[1, 0, 2, 2]], dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="no backward"):
+        reorder_slots([t, t.clone().requires_grad_()], p)
+    assert torch.equal(t, torch.arange(8.0, device="cuda").view(4, 2))
+    with torch.no_grad():
+        reorder_slots(iter([t, t.clone().requires_grad_()]), p)
+    assert t.tolist() == [[2.0, 3.0], [0.0, 1.0], [4.0, 5.0], [4.0, 5.0]]
