@@ -581,9 +581,11 @@ int onebit_attention_shared_rows(const void *q, const void *prefix_k, const void
                                  int64_t n_prefix_slots, int64_t prefix_max_len, int64_t n_slots, int64_t max_len, int64_t max_own,
                                  void *scratch, size_t scratch_bytes, void *stream);
 /* onebit_beam_select: logits [groups * beams, vocab] (dtype, row pitch ld elements), scores fp32 [groups * beams] the hypotheses' sums of log
- * probabilities.  Continuing hypothesis b of a group by token t is worth v = score_b + (x_t - ln sum_u e^{x_u}), in 64 bits; the group's `keep`
- * best in the order (v descending, beam, logit descending, token) are written to out_scores (v rounded to fp32) / out_beams / out_tokens
- * [groups, keep].  A continuation of v = -inf or NaN (a banned token, a dead hypothesis, a row with a NaN or +inf) is none; places that remain
+ * probabilities.  Continuing hypothesis b of a group by token t is worth v = score_b + (x_t - ln sum_u e^{x_u}), added and compared in 64 bits, the sum's
+ * terms e^d, d = x_u - max, in fp32: ln is off by at most 2^-23 (1 + 9/8 mean |d|), the mean over the row's probabilities, and values of two rows that lie closer
+ * can come in either order (equal rows are equal to the bit, and within a row the logits order).  The group's `keep`
+ * best in the order (v descending, beam, logit descending, token) are written to out_scores (v rounded to fp32) / out_beams / out_tokens [groups, keep].
+ * A continuation of v = -inf or NaN (a banned token, a dead hypothesis, a row with a NaN or +inf) is none; places that remain
  * hold -inf, -1, -1.  beams 1 .. 32, keep 1 .. 64, vocab <= 2^20, groups * beams <= 65535.  scratch: onebit_beam_select_scratch_bytes(groups * beams, vocab, keep)
  * bytes or more, 16-byte aligned, ZERO-FILLED ONCE (4096 int32 in front of it are zero again after every call); not shared by calls that may run at the
  * same time.  Outputs and scratch overlap no input and not each other (refused). */

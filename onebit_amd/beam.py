@@ -158,8 +158,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, keep: in
                 workspace: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The ``keep`` best continuations of every group of ``beams`` hypotheses (``onebit_beam_select``): ``logits`` [groups * beams, vocab] float16 or
     float32 (rows may be strided), ``scores`` float32 [groups * beams], the hypotheses' sums of log probabilities.  Returns scores (float32), beams and
-    tokens (int32), [groups, keep] each, best first: views of one int32 tensor [3, groups, keep].  Values are ranked in 64 bits; equal ones by beam, logit,
-    token.  A continuation of probability zero is none: places that remain hold -inf, -1, -1."""
+    tokens (int32), [groups, keep] each, best first: views of one int32 tensor [3, groups, keep].  Values are added and compared in 64 bits, equal ones by
+    beam, logit, token; a row's log-sum in them is off by some 1e-7 (bound: ``onebit_beam_select``), which is how far the order between rows is exact.  A continuation of probability zero is none: places that remain hold -inf, -1, -1."""
     values, beam, token = select_packed(logits, scores, beams, keep, workspace).unbind(0)
     return values.view(_F32), beam, token
 

@@ -510,6 +510,32 @@ def test_far_below_the_maximum():
     _check_select(logits, torch.zeros(8, device="cuda"), 4, 20)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("kind", ["normal", "narrow", "wide", "equal", "two"])
+def test_the_logarithm_of_a_row_s_sum(kind, dtype):
+    """How far values are from 64 bits.  A term e^d, d = x - max, is off by 2^-24 |d| twice (the difference and its product with log2 e, rounded), by 2^-26 |d| (the constant) and by 2^-23
+    (the exponential), so the logarithm of the sum by 2^-23 (1 + 9/8 mean |d|), the mean over the row's probabilities."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    n, vocab = 40, 32003
+    x = torch.randn(n, vocab, generator=g, device="cuda")
+    if kind == "equal":
+        x = torch.linspace(-9, 0, n, device="cuda")[:, None].repeat(1, vocab)
+    elif kind == "two":                                              # half of the row at each of two places: every term of a half is off by the same
+        x = torch.where(x < 0, torch.linspace(-20, 0, n, device="cuda")[:, None], torch.linspace(-5, -4, n, device="cuda")[:, None])
+    else:
+        x = x * {"normal": 2.0, "narrow": 0.1, "wide": 12.0}[kind]
+    x[:, 0] = x.amax(1) + torch.linspace(0, 9, n, device="cuda")
+    x = x.to(dtype)
+    d = x.double()
+    lse, top = torch.logsumexp(d, -1), d.amax(-1)
+    scores = (lse - top).float()                                     # the best value is then nearly zero, where fp32 shows small errors
+    v = beam_select(x, scores, 1, 1)[0][:, 0].double()
+    ref = scores.double() + (top - lse)
+    tol = 2.0 ** -23 * (1 + 9 / 8 * ((top[:, None] - d) * torch.softmax(d, -1)).sum(-1)) * 1.001
+    err = (v - ref).abs()
+    assert (err <= tol).all()
+
+
 def test_select_in_a_graph_and_with_a_kept_workspace():
     ws = beam_select_workspace(16, 40000, 64)
     g = torch.Generator(device="cuda").manual_seed(4)
