@@ -351,8 +351,8 @@ __device__ __forceinline__ ObShItem ob_sh_item(const ObShArgs &A, int block, int
 
 // More queries: the four waves share the queries out, 16 MT each, over tiles of 64 keys and values that they read from the LDS together (two tiles
 // there, brought by DMA; one barrier a tile).  The second half's keys are read while the first one's exponentials run.
-// MT = 2: 64 rows of 64 / 8 heads over 32768 keys 79 us, 0.87 PFLOP/s (tiles through registers 88; MT = 4 140: 490 registers, one wave a SIMD): products, exponentials and LDS
-// reads, 32, 40 and 37 us of them each, in turn.
+// MT = 2: 64 rows of 64 / 8 heads over 32768 keys 79 us, 0.87 PFLOP/s (tiles through registers 88; MT = 4 140: 490 registers, one wave a SIMD): products, vector
+// instructions and LDS reads, 31, 28 and 29 us of them each, mostly in turn.
 template <int DP, int MT, bool EXACT>
 __device__ __forceinline__ void ob_sh_wide(const ObShArgs &A, const ObShItem &I, const ObShGroup &G, _Float16 (*kv)[2][64 * DP])
 {

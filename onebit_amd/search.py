@@ -34,7 +34,8 @@ def _prime(step, first_slot: int, stride: int, prompts: Sequence[Sequence[int]])
 
 
 class LlamaBeams:
-    """Slots of a 1-bit LLaMA: hypothesis b of prompt i in slot i beams + b, the prompt itself in slot batch beams + i."""
+    """Slots of a 1-bit LLaMA: hypothesis b of prompt i in slot i beams + b, the prompt itself in slot batch beams + i.  Every slot is max_len long, since a token's place
+    in its slot is its position: batch (beams + 1) of them."""
 
     def __init__(self, model, batch: int, beams: int, max_len: int):
         from .engine import MixedStep
