@@ -205,7 +205,7 @@ def beam_rows(model, prompts: List[List[int]], max_new_tokens: int, max_position
     if not 1 <= beams <= MAX_BEAMS:
         raise ValueError(f"num_beams must be in 1 .. {MAX_BEAMS}")
     _candidates(beams, eos)                                              # (what a search would refuse, before its slots take memory)
-    if not prompts or not all(prompts):
+    if len(prompts) < 1 or any(len(p) < 1 for p in prompts):
         raise ValueError("beam search needs prompts of at least one token")
     longest = max(len(p) for p in prompts) + max_new_tokens
     if longest > max_positions:
